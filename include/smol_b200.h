@@ -509,6 +509,68 @@ SMOL_B200_API int smol_b200_gemm_bf16(void *stream, void *out, int64_t ldo, int 
 SMOL_B200_API int smol_b200_layer_norm(void *stream, void *out, int out_bf16, const float *x, const float *w,
                                        const float *b, int rows, int hidden, float eps);
 
+/* ===========================================================================
+ * Part 6 -- caches that sequences share, and caches held to a budget.  No counterpart
+ * in the reference, whose decoder keeps one private, growing cache per context
+ * (common/decoder/qkn_decoder.c:172-220).
+ *
+ * Both work on the pooled bf16-K / fp16-V cache of Part 3.  A cached row carries its
+ * rotary position inside K, so attention does not depend on the order of rows: rows may
+ * be shared by sequences, and a row may move to another slot of its sequence.
+ *
+ * Calls are asynchronous on `stream`, allocate nothing and can be captured in a graph.
+ * The workspace holds intermediate results of one call only: calls that may overlap on
+ * the GPU need workspaces of their own.  Running weights are
+ * fp32 [n_seqs][n_kv_heads][weights_stride]: entry j of a (sequence, KV head) belongs to
+ * cached row seq_row0 + j.  weights_out[j] = weights_in[j] + (what the call adds) for the
+ * rows the call covers; other entries of weights_out are not written.  weights_in NULL
+ * starts from zero, and weights_in may be weights_out (the arrays are otherwise disjoint).
+ * =========================================================================== */
+
+/* Batched single-query decode in which sequences share prefixes: sequences
+ * prefix_seq0[g] <= b < prefix_seq0[g+1] (device, n_prefixes + 1 ascending entries) attend
+ * pool rows [prefix_row0[g], prefix_row0[g] + prefix_len[g]) followed by their own rows
+ * [seq_row0[b], seq_row0[b] + kv_len[b]); a sequence outside every range has no prefix.
+ * Prefix rows are read once for all the sequences that share them.  kv_len[b] and
+ * prefix_len[g] may be 0; a sequence without any visible row gives zeros.  window > 0
+ * limits a sequence to the last `window` of its prefix and own rows together; softcap > 0
+ * caps scores as in Part 3.  max_kv_len, max_prefix_len and max_prefix_seqs (sequences of
+ * one prefix) bound the device values: what exceeds them is left out and flagged in the
+ * device error word.
+ * q: [n_seqs, n_heads*head_dim] fp32 or bf16 (q_is_bf16); out: the same shape, fp32 or
+ * bf16 (out_is_bf16); both and the pools 16-byte aligned.  fp32 queries enter with 24 bits,
+ * and an fp32 output is computed to fp32 accuracy from the cached values; a bf16 output is
+ * rounded once.  head_dim: 64, 128 or 256; scale > 0.  A row that a window hides from one
+ * sequence is still multiplied by 0 if another sequence of the same prefix sees it, so
+ * prefix rows must hold finite values (rows past every length may hold anything).
+ * weights_out (or NULL): the attention probabilities of the own rows, summed over the
+ * query heads of each KV head, are added to the running weights; weights_stride >=
+ * max_kv_len.
+ * The workspace of given counts and lengths serves every call with the same counts and
+ * shorter lengths. */
+SMOL_B200_API size_t smol_b200_decode_shared_workspace_bytes(int n_seqs, int max_kv_len, int n_prefixes,
+                                                             int max_prefix_len, int max_prefix_seqs, int n_heads,
+                                                             int n_kv_heads, int head_dim);
+SMOL_B200_API int smol_b200_decode_attention_shared(
+    void *stream, void *out, int out_is_bf16, const void *q, int q_is_bf16, const uint16_t *k_pool,
+    const uint16_t *v_pool, int64_t pool_rows, const int64_t *prefix_row0, const int *prefix_len,
+    const int *prefix_seq0, int n_prefixes, int max_prefix_len, int max_prefix_seqs, const int64_t *seq_row0,
+    const int *kv_len, int n_seqs, int max_kv_len, int n_heads, int n_kv_heads, int head_dim, float scale,
+    int window, float softcap, const float *weights_in, float *weights_out, int64_t weights_stride,
+    void *workspace, size_t workspace_bytes);
+
+/* The same without prefixes: smol_b200_decode_attention that also adds each cached row's
+ * attention probability, summed over the query heads of its KV head, to the running
+ * weights (every own row j < kv_len[b]; rows before the window add 0). */
+SMOL_B200_API size_t smol_b200_decode_weights_workspace_bytes(int n_seqs, int max_kv_len, int n_heads,
+                                                              int n_kv_heads, int head_dim);
+SMOL_B200_API int smol_b200_decode_attention_weights(
+    void *stream, void *out, int out_is_bf16, const void *q, int q_is_bf16, const uint16_t *k_pool,
+    const uint16_t *v_pool, int64_t pool_rows, const int64_t *seq_row0, const int *kv_len, int n_seqs,
+    int max_kv_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window, float softcap,
+    const float *weights_in, float *weights_out, int64_t weights_stride, void *workspace,
+    size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

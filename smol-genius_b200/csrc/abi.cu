@@ -762,6 +762,53 @@ int smol_b200_layer_norm(void *stream, void *out, int out_bf16, const float *x, 
 }
 
 // ---------------------------------------------------------------------------
+// Part 6
+// ---------------------------------------------------------------------------
+size_t smol_b200_decode_shared_workspace_bytes(int n_seqs, int max_kv_len, int n_prefixes, int max_prefix_len,
+                                               int max_prefix_seqs, int n_heads, int n_kv_heads, int head_dim)
+{
+    return decode_shared_workspace_bytes(n_seqs, max_kv_len, n_prefixes, max_prefix_len, max_prefix_seqs, n_heads,
+                                         n_kv_heads, head_dim, true);
+}
+
+int smol_b200_decode_attention_shared(void *stream, void *out, int out_is_bf16, const void *q, int q_is_bf16,
+                                      const uint16_t *k_pool, const uint16_t *v_pool, int64_t pool_rows,
+                                      const int64_t *prefix_row0, const int *prefix_len, const int *prefix_seq0,
+                                      int n_prefixes, int max_prefix_len, int max_prefix_seqs,
+                                      const int64_t *seq_row0, const int *kv_len, int n_seqs, int max_kv_len,
+                                      int n_heads, int n_kv_heads, int head_dim, float scale, int window,
+                                      float softcap, const float *weights_in, float *weights_out,
+                                      int64_t weights_stride, void *workspace, size_t workspace_bytes)
+{
+    return record(decode_attention_shared(static_cast<cudaStream_t>(stream), out, out_is_bf16, q, q_is_bf16, k_pool,
+                                          v_pool, pool_rows, prefix_row0, prefix_len, prefix_seq0, n_prefixes,
+                                          max_prefix_len, max_prefix_seqs, seq_row0, kv_len, n_seqs, max_kv_len,
+                                          n_heads, n_kv_heads, head_dim, scale, window, softcap, weights_in,
+                                          weights_out, weights_stride, workspace, workspace_bytes),
+                  "smol_b200_decode_attention_shared");
+}
+
+size_t smol_b200_decode_weights_workspace_bytes(int n_seqs, int max_kv_len, int n_heads, int n_kv_heads, int head_dim)
+{
+    return decode_shared_workspace_bytes(n_seqs, max_kv_len, 0, 0, 0, n_heads, n_kv_heads, head_dim, true);
+}
+
+int smol_b200_decode_attention_weights(void *stream, void *out, int out_is_bf16, const void *q, int q_is_bf16,
+                                       const uint16_t *k_pool, const uint16_t *v_pool, int64_t pool_rows,
+                                       const int64_t *seq_row0, const int *kv_len, int n_seqs, int max_kv_len,
+                                       int n_heads, int n_kv_heads, int head_dim, float scale, int window,
+                                       float softcap, const float *weights_in, float *weights_out,
+                                       int64_t weights_stride, void *workspace, size_t workspace_bytes)
+{
+    if (n_seqs > 0 && !weights_out) return record(SMOL_B200_ERR_ARGS, "smol_b200_decode_attention_weights");
+    return record(decode_attention_shared(static_cast<cudaStream_t>(stream), out, out_is_bf16, q, q_is_bf16, k_pool,
+                                          v_pool, pool_rows, nullptr, nullptr, nullptr, 0, 0, 0, seq_row0, kv_len,
+                                          n_seqs, max_kv_len, n_heads, n_kv_heads, head_dim, scale, window, softcap,
+                                          weights_in, weights_out, weights_stride, workspace, workspace_bytes),
+                  "smol_b200_decode_attention_weights");
+}
+
+// ---------------------------------------------------------------------------
 // Part 4
 // ---------------------------------------------------------------------------
 size_t smol_b200_qkn_prefill_workspace_bytes(const smol_b200_qkn_model *model, int n_tokens)

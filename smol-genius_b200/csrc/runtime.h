@@ -170,4 +170,15 @@ size_t siglip_workspace_bytes(const smol_b200_siglip_model *m, int n_images);
 int siglip_forward(cudaStream_t st, float *out, const float *images, int n_images, const smol_b200_siglip_model *m,
                    void *workspace, size_t workspace_bytes);
 
+// decode_shared.cu: decode over shared prefixes, with attention weights (Part 6 of smol_b200.h)
+size_t decode_shared_workspace_bytes(int n_seqs, int max_kv_len, int n_prefixes, int max_prefix_len,
+                                     int max_prefix_seqs, int n_heads, int n_kv_heads, int head_dim, bool weights);
+int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const void *q, int q_is_bf16,
+                            const uint16_t *k_pool, const uint16_t *v_pool, int64_t pool_rows,
+                            const int64_t *prefix_row0, const int *prefix_len, const int *prefix_seq0, int n_prefixes,
+                            int max_prefix_len, int max_prefix_seqs, const int64_t *seq_row0, const int *kv_len,
+                            int n_seqs, int max_kv_len, int n_heads, int n_kv_heads, int head_dim, float scale,
+                            int window, float softcap, const float *weights_in, float *weights_out,
+                            int64_t weights_stride, void *workspace, size_t workspace_bytes);
+
 }  // namespace smolb200

@@ -127,6 +127,16 @@ _SIGNATURES = {
                                      _c_void, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "smol_b200_layer_norm": (_c_int, [_c_void, _c_void, _c_int, _c_void, _c_void, _c_void, _c_int, _c_int,
                                       _c_float]),
+    # Part 6 (shared prefixes, attention weights)
+    "smol_b200_decode_shared_workspace_bytes": (_c_size, [_c_int] * 8),
+    "smol_b200_decode_attention_shared": (
+        _c_int, [_c_void, _c_void, _c_int, _c_void, _c_int, _c_void, _c_void, _c_i64, _c_void, _c_void, _c_void, _c_int,
+                 _c_int, _c_int, _c_void, _c_void, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_float,
+                 _c_void, _c_void, _c_i64, _c_void, _c_size]),
+    "smol_b200_decode_weights_workspace_bytes": (_c_size, [_c_int] * 5),
+    "smol_b200_decode_attention_weights": (
+        _c_int, [_c_void, _c_void, _c_int, _c_void, _c_int, _c_void, _c_void, _c_i64, _c_void, _c_void, _c_int, _c_int,
+                 _c_int, _c_int, _c_int, _c_float, _c_int, _c_float, _c_void, _c_void, _c_i64, _c_void, _c_size]),
 }
 
 
@@ -529,3 +539,46 @@ def layer_norm(out, x, w, b, rows, hidden, eps, out_bf16=False, stream=None):
     check(lib().smol_b200_layer_norm(_stream(stream), _ptr(out), int(out_bf16), _ptr(x), _ptr(w), _ptr(b), rows,
                                      hidden, eps),
           "smol_b200_layer_norm")
+
+
+# ---------------------------------------------------------------------------
+# Part 6: shared prefixes, attention weights
+# ---------------------------------------------------------------------------
+def decode_shared_workspace_bytes(n_seqs, max_kv_len, n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads,
+                                  head_dim) -> int:
+    return lib().smol_b200_decode_shared_workspace_bytes(n_seqs, max_kv_len, n_prefixes, max_prefix_len,
+                                                         max_prefix_seqs, n_heads, n_kv_heads, head_dim)
+
+
+def decode_attention_shared(out, q, k_pool, v_pool, pool_rows, prefix_row0, prefix_len, prefix_seq0, n_prefixes,
+                            max_prefix_len, max_prefix_seqs, seq_row0, kv_len, n_seqs, max_kv_len, n_heads, n_kv_heads,
+                            head_dim, scale, workspace, window=0, softcap=0.0, weights_in=None, weights_out=None,
+                            weights_stride=0, stream=None):
+    """q and out: fp32 or bf16 [n_seqs, n_heads*head_dim] each; prefix_row0 int64 and prefix_len int32
+    [n_prefixes], prefix_seq0 int32 [n_prefixes + 1]; weights fp32 [n_seqs, n_kv_heads, weights_stride] or None."""
+    import torch
+    rc = lib().smol_b200_decode_attention_shared(
+        _stream(stream), _ptr(out), int(out.dtype == torch.bfloat16), _ptr(q), int(q.dtype == torch.bfloat16),
+        _ptr(k_pool), _ptr(v_pool), pool_rows, _ptr(prefix_row0), _ptr(prefix_len), _ptr(prefix_seq0), n_prefixes,
+        max_prefix_len, max_prefix_seqs, _ptr(seq_row0), _ptr(kv_len), n_seqs, max_kv_len, n_heads, n_kv_heads,
+        head_dim, scale, window, softcap, _ptr(weights_in), _ptr(weights_out), weights_stride, _ptr(workspace),
+        workspace.numel() * workspace.element_size())
+    check(rc, "smol_b200_decode_attention_shared")
+
+
+def decode_weights_workspace_bytes(n_seqs, max_kv_len, n_heads, n_kv_heads, head_dim) -> int:
+    return lib().smol_b200_decode_weights_workspace_bytes(n_seqs, max_kv_len, n_heads, n_kv_heads, head_dim)
+
+
+def decode_attention_weights(out, q, k_pool, v_pool, pool_rows, seq_row0, kv_len, n_seqs, max_kv_len, n_heads,
+                             n_kv_heads, head_dim, scale, weights_in, weights_out, weights_stride, workspace, window=0,
+                             softcap=0.0, stream=None):
+    """decode_attention that adds each own row's attention probability (summed over the query heads of its KV
+    head) to weights_in (None: zero), into weights_out (may be weights_in)."""
+    import torch
+    rc = lib().smol_b200_decode_attention_weights(
+        _stream(stream), _ptr(out), int(out.dtype == torch.bfloat16), _ptr(q), int(q.dtype == torch.bfloat16),
+        _ptr(k_pool), _ptr(v_pool), pool_rows, _ptr(seq_row0), _ptr(kv_len), n_seqs, max_kv_len, n_heads, n_kv_heads,
+        head_dim, scale, window, softcap, _ptr(weights_in), _ptr(weights_out), weights_stride, _ptr(workspace),
+        workspace.numel() * workspace.element_size())
+    check(rc, "smol_b200_decode_attention_weights")
