@@ -147,7 +147,7 @@ struct PrefixShape {
 };
 
 struct PrefixBars {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done, mma_done;
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done, o_final, mma_done;
     uint32_t tmem_base;
     int lo_min;
 };
@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
             mbar_init(smem_u32(&bars->p_full[s]), kBM);
         }
         mbar_init(smem_u32(&bars->o_done), 1);
+        mbar_init(smem_u32(&bars->o_final), 1);
         mbar_init(smem_u32(&bars->mma_done), 1);
         fence_mbar_init();
     }
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
             umma_commit_elect(smem_u32(&bars->k_empty[st]));
             if (j >= 1) ok = issue_pv(j - 1);
         }
-        if (ok) issue_pv(n_tiles - 1);
+        if (ok && issue_pv(n_tiles - 1)) umma_commit_elect(smem_u32(&bars->o_final));
         // every MMA must be complete before TMEM is released
         umma_commit_elect(smem_u32(&bars->mma_done));
         mbar_wait_warp(smem_u32(&bars->mma_done), 0, p.err, kErrDrain);
@@ -460,7 +461,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
             tc_fence_before();
             mbar_arrive(smem_u32(&bars->p_full[sb]));
         }
-        if (ok) ok = mbar_wait_warp(smem_u32(&bars->o_done), (n_tiles - 1) & 1, p.err, kErrWaitMma);
+        // o_done may be two phases behind here (a parity wait could not tell), hence o_final
+        if (ok) ok = mbar_wait_warp(smem_u32(&bars->o_final), 0, p.err, kErrWaitMma);
         if (ok) {
             tc_fence_after();
             float *dst = p.part_o + slot * HD;

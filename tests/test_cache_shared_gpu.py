@@ -179,6 +179,17 @@ def test_shared_sizes(cuda, seqs, plen, own):
     no_error()
 
 
+@pytest.mark.parametrize("q_bf16,out_bf16", [(True, True), (True, False), (False, False), (False, True)])
+@pytest.mark.parametrize("hq,hkv,hd", [(16, 8, 128), (8, 1, 256), (4, 2, 64)])
+def test_full_query_tiles_over_several_key_tiles(cuda, hq, hkv, hd, q_bf16, out_bf16):
+    # every row of a query tile in use and many key tiles to a part
+    seqs = 128 * hkv // hq + 3
+    c = Case(cuda, [i % 5 for i in range(seqs)], plens=[8192], cut=[0, seqs], hq=hq, hkv=hkv, hd=hd, q_bf16=q_bf16,
+             out_bf16=out_bf16, seed=15)
+    c.check(c.run())
+    no_error()
+
+
 @pytest.mark.parametrize("window", [1, 2, 10, 64, 100, 333, 5000])
 @pytest.mark.parametrize("hq,hkv,hd", [(16, 8, 128), (8, 1, 256)])
 def test_window_over_prefix_and_own_rows(cuda, window, hq, hkv, hd):
