@@ -123,7 +123,7 @@ __device__ __forceinline__ void own_range(const SharedParams &p, int b, int &ks,
 // Row r of tile t is query head (r' % group) of sequence s0 + r'/group, r' = 128 t + r.
 constexpr int kBM = 128;
 constexpr int kPrefixThreads = 192;
-constexpr float kSumLimit = 32768.0f;   // a tile's row sum beyond this moves the row's reference (P must fit fp16)
+constexpr float kMoveLog2 = 8.0f;
 
 template <int HD, int QT>
 struct PrefixShape {
@@ -269,8 +269,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
 #pragma unroll
                 for (int kk = 0; kk < BN / 16; ++kk) {
                     const uint64_t bd = umma_sdesc_sw128(v_addr + kk * 16 * 128, S::kKvSubBytes, 1024);
-                    umma_ts_elect(tmem + S::kTmO, tmem + sb * BN + t * (BN / 2) + kk * 8, bd, idesc_pv,
-                                  (j > 0 || t < PT - 1 || kk > 0) ? 1u : 0u);
+                    // columns of P: see the softmax (32-key groups: 16 of values, 16 of remainders)
+                    umma_ts_elect(tmem + S::kTmO, tmem + sb * BN + (kk >> 1) * 32 + t * 16 + (kk & 1) * 8, bd,
+                                  idesc_pv, (j > 0 || t < PT - 1 || kk > 0) ? 1u : 0u);
                 }
             umma_commit_elect(smem_u32(&bars->o_done));
             umma_commit_elect(smem_u32(&bars->v_empty[st]));
@@ -303,46 +304,59 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
         mbar_wait_warp(smem_u32(&bars->mma_done), 0, p.err, kErrDrain);
     } else {
         // ================= softmax =================
-        {   // this warp's 32 query rows, as QT bf16 terms in the 128B-swizzled K-major layout
-            constexpr int kVecs = HD / 8;   // 8 elements at a time
-            for (int i = lane; i < 32 * kVecs; i += 32) {
-                const int r = warp * 32 + i / kVecs, e = (i % kVecs) * 8;
-                const int rr = qt * kBM + r;
-                const int rb = s0 + rr / p.group, rh = kvh * p.group + rr % p.group;
-                float x[8];
-                if (rb < s1) {
-                    const long long off = (static_cast<long long>(rb) * p.n_heads + rh) * HD + e;
-                    if (p.q_is_bf16) {
-                        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + off));
-                        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        // This warp's query rows as QT bf16 terms in the 128B-swizzled K-major layout, kLoad
+        // 8-element pieces in flight per lane (one at a time took 11 us of an 18 us call at
+        // 512 prefix keys).  Rows past the last sequence stay unwritten: a row of Q only
+        // reaches its own row of S and O, and those rows are neither used nor stored.
+        const bool warp_live = s0 + (qt * kBM + warp * 32) / p.group < s1;
+        if (warp_live) {
+            constexpr int kVecs = HD / 8, kLoad = 4;
+            for (int i0 = lane; i0 < 32 * kVecs; i0 += 32 * kLoad) {
+                uint4 raw[kLoad][2];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            x[2 * k] = bf16lo_f32(u[k]);
-                            x[2 * k + 1] = bf16hi_f32(u[k]);
+                for (int n = 0; n < kLoad; ++n) {
+                    const int i = i0 + 32 * n;
+                    const int rr = qt * kBM + warp * 32 + i / kVecs;
+                    const int rb = s0 + rr / p.group, rh = kvh * p.group + rr % p.group;
+                    const long long off = (static_cast<long long>(rb) * p.n_heads + rh) * HD + (i % kVecs) * 8;
+                    if (rb < s1) {
+                        if (p.q_is_bf16) {
+                            raw[n][0] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + off));
+                        } else {
+                            const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const float *>(p.q) + off);
+                            raw[n][0] = __ldg(src);
+                            raw[n][1] = __ldg(src + 1);
                         }
-                    } else {
-                        const float4 a = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + off));
-                        const float4 d =
-                            __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + off + 4));
-                        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-                        x[4] = d.x, x[5] = d.y, x[6] = d.z, x[7] = d.w;
                     }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) x[k] = 0.f;
                 }
-                uint32_t t[4][QT];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) split_bf16<QT>(x[2 * k], x[2 * k + 1], t[k]);
-                const uint32_t at = (e / 64) * S::kQSubBytes + sw128_offset(r, (e % 64) / 8);
+                for (int n = 0; n < kLoad; ++n) {
+                    const int i = i0 + 32 * n;
+                    const int r = warp * 32 + i / kVecs, e = (i % kVecs) * 8;
+                    if (s0 + (qt * kBM + r) / p.group >= s1) continue;
+                    const uint32_t at = (e / 64) * S::kQSubBytes + sw128_offset(r, (e % 64) / 8);
+                    const uint32_t u[8] = {raw[n][0].x, raw[n][0].y, raw[n][0].z, raw[n][0].w,
+                                           raw[n][1].x, raw[n][1].y, raw[n][1].z, raw[n][1].w};
+                    uint32_t t[4][QT];
 #pragma unroll
-                for (int q = 0; q < QT; ++q)
-                    *reinterpret_cast<uint4 *>(smem + q * S::kQTermBytes + at) =
-                        make_uint4(t[0][q], t[1][q], t[2][q], t[3][q]);
+                    for (int k = 0; k < 4; ++k) {
+                        if (p.q_is_bf16) {
+                            t[k][0] = u[k];
+#pragma unroll
+                            for (int q = 1; q < QT; ++q) t[k][q] = 0u;
+                        } else {
+                            split_bf16<QT>(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]), t[k]);
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < QT; ++q)
+                        *reinterpret_cast<uint4 *>(smem + q * S::kQTermBytes + at) =
+                            make_uint4(t[0][q], t[1][q], t[2][q], t[3][q]);
+                }
             }
-            fence_proxy_async_smem();
-            mbar_arrive(smem_u32(&bars->q_full));
         }
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(&bars->q_full));
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
         const float cap = p.softcap, inv_cap = cap > 0.f ? 1.f / cap : 0.f;
         const float mul = cap > 0.f ? 1.f : p.scale * kLog2e;
@@ -352,98 +366,101 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
             const int sb = j & 1;
             ok = mbar_wait_warp(smem_u32(&bars->s_full[sb]), (j >> 1) & 1, p.err, kErrWaitMma);
             if (!ok) break;
+            if (!warp_live && key_hi - (key_lo + j * BN) >= BN) {   // no row here, no V rows to clear
+                mbar_arrive(smem_u32(&bars->p_full[sb]));
+                continue;
+            }
             tc_fence_after();
             const uint32_t s_col = lane_base + sb * BN;
-            float t[BN];
-            {
-                uint32_t rr[BN / 32][32];
-#pragma unroll
-                for (int q = 0; q < BN / 32; ++q) tmem_ld32(s_col + q * 32, rr[q]);
-                tmem_ld_wait();
-#pragma unroll
-                for (int q = 0; q < BN / 32; ++q)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) t[q * 32 + i] = __uint_as_float(rr[q][i]);
-            }
             const int key0 = key_lo + j * BN;
-            if (cap > 0.f) {
+            const bool whole = __all_sync(0xffffffffu, row_valid && key0 >= lo && key0 + BN <= key_hi);
+            // The row's keys in groups of 32 columns, once for the maximum and once for the
+            // exponentials: S is read twice, but the code stays small (fully unrolled over the
+            // tile it was fetched from memory for every short call).
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int q = 0; q < BN / 32; ++q) {
+                uint32_t rr[32];
+                tmem_ld32(s_col + q * 32, rr);
+                tmem_ld_wait();
+                if (!whole) {
 #pragma unroll
-                for (int i = 0; i < BN; ++i) t[i] = cap * tanhf(t[i] * p.scale * inv_cap) * kLog2e;
-            }
-            if (!(row_valid && key0 >= lo && key0 + BN <= key_hi)) {
-#pragma unroll
-                for (int i = 0; i < BN; ++i)
-                    if (!row_valid || key0 + i < lo || key0 + i >= key_hi) t[i] = -INFINITY;
-            }
-            auto row_max = [&]() -> float {
-                float pm[8];
-#pragma unroll
-                for (int q = 0; q < 8; ++q) pm[q] = fmaxf(t[2 * q], t[2 * q + 1]);
-#pragma unroll
-                for (int i = 16; i < BN; i += 16)
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) pm[q] = fmaxf(pm[q], fmaxf(t[i + 2 * q], t[i + 2 * q + 1]));
-                return mul * fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])),
-                                   fmaxf(fmaxf(pm[4], pm[5]), fmaxf(pm[6], pm[7])));
-            };
-            // The reference m of a row is the maximum of the first tile it sees; it moves only
-            // when a tile's sum against it passes 2^15, so O is rescaled rarely.
-            const bool fresh = m == -INFINITY && row_valid && key0 + BN > lo;
-            if (__any_sync(0xffffffffu, fresh)) {
-                const float mx = row_max();
-                if (fresh) m = mx;
-            }
-            float lt = 0.f;
-#pragma unroll
-            for (int pass = 0; pass < 2; ++pass) {
-                const float negm = m != -INFINITY ? -m : 0.f;
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                constexpr int kGrp = BN < 64 ? BN / 2 : 32;   // pairs per TMEM store
-#pragma unroll
-                for (int q = 0; q < BN / (2 * kGrp); ++q) {
-                    uint32_t hi[32], rem[32];
-#pragma unroll
-                    for (int i = 0; i < kGrp; ++i) {
-                        const float e0 = fast_exp2(fmaf(t[(q * kGrp + i) * 2], mul, negm));
-                        const float e1 = fast_exp2(fmaf(t[(q * kGrp + i) * 2 + 1], mul, negm));
-                        acc[i & 3] += e0 + e1;
-                        if (PT == 2) split_f16(e0, e1, hi[i], rem[i]);
-                        else hi[i] = pack_f16x2(e0, e1);
-                    }
-                    if constexpr (kGrp == 32) {
-                        tmem_st32(s_col + q * 32, hi);
-                        if (PT == 2) tmem_st32(s_col + BN / 2 + q * 32, rem);
-                    } else {   // BN = 32: 16 columns of values, then 16 of remainders
-#pragma unroll
-                        for (int i = 0; i < kGrp; ++i) hi[kGrp + i] = PT == 2 ? rem[i] : 0u;
-                        tmem_st32(s_col, hi);
+                    for (int i = 0; i < 32; ++i) {
+                        const int key = key0 + q * 32 + i;
+                        if (!row_valid || key < lo || key >= key_hi) rr[i] = 0xff800000u;   // -inf
                     }
                 }
-                lt = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-                const bool over = !(lt <= kSumLimit);   // also NaN
-                if (pass == 1 || !__any_sync(0xffffffffu, over)) break;
-                const float mx = row_max();
-                const float f = over ? fast_exp2(m - mx) : 1.f;
-                if (over) m = mx;
-                if (j > 0) {   // O holds the earlier tiles' P V: scale it once they are complete
-                    ok = mbar_wait_warp(smem_u32(&bars->o_done), (j - 1) & 1, p.err, kErrWaitMma);
-                    if (!ok) break;
-                    tc_fence_after();
-                    uint32_t ro[32];
+                float pm[4];
 #pragma unroll
-                    for (int q = 0; q < HD / 32; ++q) {
-                        tmem_ld32(lane_base + S::kTmO + q * 32, ro);
-                        tmem_ld_wait();
+                for (int i = 0; i < 4; ++i) pm[i] = fmaxf(__uint_as_float(rr[2 * i]), __uint_as_float(rr[2 * i + 1]));
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) ro[i] = __float_as_uint(__uint_as_float(ro[i]) * f);
-                        tmem_st32(lane_base + S::kTmO + q * 32, ro);
-                    }
-                }
+                for (int i = 8; i < 32; i += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        pm[k] = fmaxf(pm[k], fmaxf(__uint_as_float(rr[i + 2 * k]), __uint_as_float(rr[i + 2 * k + 1])));
+                mx = fmaxf(mx, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])));
+            }
+            if (cap > 0.f) {   // the cap is monotonic: the maximum's capped score is the capped maximum
+                if (mx != -INFINITY) mx = cap * tanhf(mx * p.scale * inv_cap) * kLog2e;
+            } else {
+                mx *= mul;
+            }
+            // The reference m of a row is the first maximum it meets; it moves only when a
+            // maximum passes it by more than 2^8 (P stays below 256 in fp16), so O is rescaled
+            // rarely.  NaN scores keep m and reach P.
+            const bool fresh = m == -INFINITY;
+            const bool move = mx > m + kMoveLog2 || (fresh && mx != -INFINITY);
+            if (__any_sync(0xffffffffu, move && !fresh)) {
+                const float f = move && !fresh ? fast_exp2(m - mx) : 1.f;
                 l *= f;
-                tmem_st_wait();
+                // j > 0 here; O holds the earlier tiles' P V: scale it once they are complete
+                ok = mbar_wait_warp(smem_u32(&bars->o_done), (j - 1) & 1, p.err, kErrWaitMma);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int q = 0; q < HD / 32; ++q) {
+                    uint32_t ro[32];
+                    tmem_ld32(lane_base + S::kTmO + q * 32, ro);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) ro[i] = __float_as_uint(__uint_as_float(ro[i]) * f);
+                    tmem_st32(lane_base + S::kTmO + q * 32, ro);
+                }
             }
-            if (!ok) break;
-            l += lt;
+            if (move) m = mx;
+            const float negm = m != -INFINITY ? -m : 0.f;
+            // P over S, in place by groups: columns 32q .. 32q+15 take the fp16 pairs of the
+            // group's 32 keys, 32q+16 .. 32q+31 what their rounding left (PT == 2).
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int q = 0; q < BN / 32; ++q) {
+                uint32_t rr[32];
+                tmem_ld32(s_col + q * 32, rr);
+                tmem_ld_wait();
+                if (cap > 0.f) {
+#pragma unroll 4
+                    for (int i = 0; i < 32; ++i)
+                        rr[i] = __float_as_uint(cap * tanhf(__uint_as_float(rr[i]) * p.scale * inv_cap) * kLog2e);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int key = key0 + q * 32 + i;
+                        if (!row_valid || key < lo || key >= key_hi) rr[i] = 0xff800000u;
+                    }
+                }
+                uint32_t w[32];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e0 = fast_exp2(fmaf(__uint_as_float(rr[2 * i]), mul, negm));
+                    const float e1 = fast_exp2(fmaf(__uint_as_float(rr[2 * i + 1]), mul, negm));
+                    acc[i & 3] += e0 + e1;
+                    if (PT == 2) split_f16(e0, e1, w[i], w[16 + i]);
+                    else w[i] = pack_f16x2(e0, e1), w[16 + i] = 0u;
+                }
+                tmem_st32(s_col + q * 32, w);
+            }
+            l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
             // Rows of the V tile past the part's last key may hold anything (another
             // sequence's rows, unwritten memory): 0 * NaN would reach O, so they are zeroed.
             const int nv = key_hi - key0;
@@ -772,106 +789,151 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
 // ===========================================================================
 // merge
 // ===========================================================================
-// CTA = (block of own keys, KV head, sequence): the row's M and L from the parts; block 0
-// also joins the outputs; with weights every block adds the probabilities of its keys.
+// CTA = (part of the work of one KV head, KV head, sequence).  The first out_blocks CTAs
+// join 128 outputs of one query head each: warp w takes every 8th part (512 contiguous
+// bytes), then the warps meet in shared memory.  The others, with weights, add the
+// probabilities of kMergeKeys own keys each.  Every warp finds the M and L it needs
+// itself: the (m, l) pairs of a head are few and the warps of a CTA share them in L1.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeKeys = 1024;
+constexpr int kMergeOuts = 128;
+
+// M and 1/L of a head whose parts [first, last) have the pairs ml (the whole warp).
+__device__ __forceinline__ void head_sum(const float2 *ml, int first, int last, float &M, float &inv)
+{
+    const int lane = threadIdx.x % 32;
+    M = -INFINITY;
+    for (int c = first + lane; c < last; c += 32) M = fmaxf(M, ml[c].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float L = 0.f;
+    for (int c = first + lane; c < last; c += 32) {
+        const float2 v = ml[c];
+        if (v.x != -INFINITY) L += fast_exp2(v.x - M) * v.y;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    inv = L != 0.f ? 1.f / L : 0.f;   // NaN stays NaN
+}
 
 template <int HD>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ SharedParams p)
 {
     griddep_wait();
     griddep_trigger();
-    extern __shared__ float fac[];   // [8][slots]: 2^(m_part - M) of the heads of this round
-    __shared__ float s_M[8], s_inv[8];
     const int b = blockIdx.z, kvh = blockIdx.y;
     int ks, n;
     own_range(p, b, ks, n);
-    const int j0 = blockIdx.x * kMergeKeys;
-    if (blockIdx.x > 0 && j0 >= n) return;
+    const int out_blocks = (p.group * HD + kMergeOuts - 1) / kMergeOuts;
+    const int j0 = (static_cast<int>(blockIdx.x) - out_blocks) * kMergeKeys;
+    if (j0 >= 0 && j0 >= n) return;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0 && (p.kv_len[b] > p.max_kv_len || p.kv_len[b] < 0))
         atomicOr(p.err, kErrBadArgs);
     // whether the sequence has a prefix (its parts were then all written)
     bool has_prefix = false;
-    for (int g = 0; g < p.n_prefixes && !has_prefix; ++g) {
+    for (int g = lane; g < p.n_prefixes; g += 32) {
         int s0, s1, len;
         prefix_range(p, g, s0, s1, len, false);
-        has_prefix = b >= s0 && b < s1;
+        has_prefix |= b >= s0 && b < s1;
     }
+    has_prefix = __any_sync(0xffffffffu, has_prefix);
     const int first = has_prefix ? 0 : p.prefix_slots;
     const int last = p.prefix_slots + (n > ks ? (n - ks + p.chunk - 1) / p.chunk : 0);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    float w[kMergeKeys / kMergeThreads];
-#pragma unroll
-    for (int i = 0; i < kMergeKeys / kMergeThreads; ++i) w[i] = 0.f;
+    const long long row0 = static_cast<long long>(b) * p.n_heads + kvh * p.group;
 
+    if (j0 < 0) {
+        // four outputs per lane; head dim 64: two heads per CTA
+        __shared__ float4 red[kMergeThreads];
+        const int e = blockIdx.x * kMergeOuts + lane * 4;
+        constexpr int kHeads = HD < kMergeOuts ? kMergeOuts / HD : 1;   // heads in this CTA
+        const int h0 = blockIdx.x * kMergeOuts / HD;
+        float M = -INFINITY, inv = 0.f;
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            if (h0 + i >= p.group) break;
+            float Mi, invi;
+            head_sum(p.part_ml + (row0 + h0 + i) * p.slots, first, last, Mi, invi);
+            if (e / HD == h0 + i) M = Mi, inv = invi;
+        }
+        const bool live = e / HD < p.group;
+        const float2 *ml = p.part_ml + (row0 + e / HD) * p.slots;
+        const float *src = p.part_o + (row0 + e / HD) * p.slots * HD + e % HD;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int kLoad = 4, kWarps = kMergeThreads / 32;   // parts in flight, parts side by side
+        for (int c0 = first + warp; live && c0 < last; c0 += kLoad * kWarps) {
+            float f[kLoad];
+            float4 v[kLoad];
+#pragma unroll
+            for (int i = 0; i < kLoad; ++i) {
+                const int c = c0 + i * kWarps;
+                f[i] = c < last ? ml[c].x : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < kLoad; ++i) {   // an empty part has no output written
+                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (f[i] != -INFINITY)
+                    v[i] = *reinterpret_cast<const float4 *>(src + static_cast<long long>(c0 + i * kWarps) * HD);
+                f[i] = f[i] != -INFINITY ? fast_exp2(f[i] - M) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < kLoad; ++i)
+                a.x += f[i] * v[i].x, a.y += f[i] * v[i].y, a.z += f[i] * v[i].z, a.w += f[i] * v[i].w;
+        }
+        red[threadIdx.x] = a;
+        __syncthreads();
+        if (warp != 0 || !live) return;
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+            const float4 v = red[w * 32 + lane];
+            a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+        }
+        a.x *= inv, a.y *= inv, a.z *= inv, a.w *= inv;
+        const long long at = row0 * HD + e;
+        if (p.out_is_bf16)
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) =
+                make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+        else
+            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = a;
+        return;
+    }
+    __shared__ float s_M[8], s_inv[8];
+    constexpr int kPer = kMergeKeys / kMergeThreads;
+    float w[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) w[i] = 0.f;
+    const long long own = static_cast<long long>(b) * p.n_kv_heads + kvh;
     for (int h0 = 0; h0 < p.group; h0 += 8) {
         const int nh = min(8, p.group - h0);
-        const long long row0 = static_cast<long long>(b) * p.n_heads + kvh * p.group + h0;
         if (warp < nh) {
-            const float2 *ml = p.part_ml + (row0 + warp) * p.slots;
-            float M = -INFINITY;
-            for (int c = first + lane; c < last; c += 32) M = fmaxf(M, ml[c].x);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-            float L = 0.f;
-            for (int c = first + lane; c < last; c += 32) {
-                const float2 v = ml[c];
-                const float f = v.x == -INFINITY ? 0.f : fast_exp2(v.x - M);
-                fac[warp * p.slots + c] = f;
-                L += f * v.y;
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-            if (lane == 0) {
-                s_M[warp] = M;
-                s_inv[warp] = L != 0.f ? 1.f / L : 0.f;   // NaN stays NaN
-            }
+            float M, inv;
+            head_sum(p.part_ml + (row0 + h0 + warp) * p.slots, first, last, M, inv);
+            if (lane == 0) s_M[warp] = M, s_inv[warp] = inv;
         }
         __syncthreads();
-        if (blockIdx.x == 0) {
-            for (int e = threadIdx.x * 4; e < nh * HD; e += kMergeThreads * 4) {
-                const int h = e / HD, d = e % HD;
-                const float *src = p.part_o + (row0 + h) * p.slots * HD + d;
-                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int c = first; c < last; ++c) {
-                    const float f = fac[h * p.slots + c];
-                    if (f == 0.f) continue;   // an empty part has no output written
-                    const float4 v = *reinterpret_cast<const float4 *>(src + static_cast<long long>(c) * HD);
-                    a.x += f * v.x, a.y += f * v.y, a.z += f * v.z, a.w += f * v.w;
-                }
-                const float inv = s_inv[h];
-                a.x *= inv, a.y *= inv, a.z *= inv, a.w *= inv;
-                const long long at = (row0 + h) * HD + d;
-                if (p.out_is_bf16)
-                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) =
-                        make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
-                else
-                    *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = a;
-            }
-        }
-        if (p.scores) {
-            const float *sc = p.scores +
-                              (static_cast<long long>(b) * p.n_kv_heads + kvh) * p.score_rows * p.score_cols + h0;
+        const float *sc = p.scores + own * p.score_rows * p.score_cols + h0;
+        for (int h = 0; h < nh; h += 2) {   // score_cols is even: a pair is one 8-byte load
+            float2 x[kPer];
 #pragma unroll
-            for (int i = 0; i < kMergeKeys / kMergeThreads; ++i) {
+            for (int i = 0; i < kPer; ++i) {
                 const int j = j0 + i * kMergeThreads + static_cast<int>(threadIdx.x);
-                if (j >= ks && j < n)
-                    for (int h = 0; h < nh; ++h) {
-                        const float x = sc[static_cast<long long>(j) * p.score_cols + h];
-                        if (x != -INFINITY) w[i] += fast_exp2(x - s_M[h]) * s_inv[h];
-                    }
+                x[i] = j >= ks && j < n
+                           ? *reinterpret_cast<const float2 *>(sc + static_cast<long long>(j) * p.score_cols + h)
+                           : make_float2(-INFINITY, -INFINITY);
+            }
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (x[i].x != -INFINITY) w[i] += fast_exp2(x[i].x - s_M[h]) * s_inv[h];
+                if (h + 1 < nh && x[i].y != -INFINITY) w[i] += fast_exp2(x[i].y - s_M[h + 1]) * s_inv[h + 1];
             }
         }
         __syncthreads();
     }
-    if (p.scores) {
-        const long long base = (static_cast<long long>(b) * p.n_kv_heads + kvh) * p.weights_stride;
+    const long long base = own * p.weights_stride;
 #pragma unroll
-        for (int i = 0; i < kMergeKeys / kMergeThreads; ++i) {
-            const int j = j0 + i * kMergeThreads + static_cast<int>(threadIdx.x);
-            if (j < n) p.weights_out[base + j] = (p.weights_in ? p.weights_in[base + j] : 0.f) + w[i];
-        }
+    for (int i = 0; i < kPer; ++i) {
+        const int j = j0 + i * kMergeThreads + static_cast<int>(threadIdx.x);
+        if (j < n) p.weights_out[base + j] = (p.weights_in ? p.weights_in[base + j] : 0.f) + w[i];
     }
 }
 
@@ -900,8 +962,10 @@ int own_slots(long long units, int max_kv_len)
     return small > big ? small : big;
 }
 
-// Parts of a prefix: enough CTAs (one per SM) for the query tiles and KV heads of all
-// prefixes, no part under 128 keys.
+// Parts of a prefix: one CTA per SM over the query tiles and KV heads of all prefixes, no
+// part under 128 keys, and none over kMaxPart: the tensor core truncates when it adds to an
+// accumulator, which left a part of 6208 keys 1.3e-5 off (1024: 2e-6).
+constexpr int kMaxPart = 1024;
 int prefix_parts(int n_prefixes, int max_prefix_len, int max_prefix_seqs, int n_heads, int n_kv_heads)
 {
     if (n_prefixes <= 0 || max_prefix_len <= 0 || max_prefix_seqs <= 0) return 0;
@@ -909,8 +973,8 @@ int prefix_parts(int n_prefixes, int max_prefix_len, int max_prefix_seqs, int n_
                             div_up(static_cast<long long>(max_prefix_seqs) * (n_heads / n_kv_heads), kBM);
     int parts = static_cast<int>(kSms / units);
     if (parts < 1) parts = 1;
-    const int most = div_up(max_prefix_len, 128);
-    return parts < most ? parts : most;
+    const int most = div_up(max_prefix_len, 128), least = div_up(max_prefix_len, kMaxPart);
+    return parts < least ? least : parts < most ? parts : most;
 }
 
 struct SharedLayout {
@@ -979,9 +1043,9 @@ int launch_shared(cudaStream_t st, SharedParams &p, const uint16_t *k_pool, cons
         if (launch_kernel(split_kernel<HD, QT, PT>, grid, dim3(kSplitThreads), S::kSmemBytes, st, p) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
     }
-    const int blocks = p.scores ? div_up(p.max_kv_len > 0 ? p.max_kv_len : 1, kMergeKeys) : 1;
-    if (launch_kernel(merge_kernel<HD>, dim3(blocks, p.n_kv_heads, p.n_seqs), dim3(kMergeThreads),
-                      static_cast<size_t>(8) * p.slots * 4, st, p) != cudaSuccess)
+    const int blocks = div_up(p.group * HD, kMergeOuts) + (p.scores ? div_up(p.max_kv_len, kMergeKeys) : 0);
+    if (launch_kernel(merge_kernel<HD>, dim3(blocks, p.n_kv_heads, p.n_seqs), dim3(kMergeThreads), 0, st, p) !=
+        cudaSuccess)
         return SMOL_B200_ERR_CUDA;
     return SMOL_B200_OK;
 }
@@ -1055,7 +1119,6 @@ int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const v
                                                       n_heads, n_kv_heads, head_dim, weights_out != nullptr);
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return SMOL_B200_ERR_WORKSPACE;
-    if (p.slots > 1500) return SMOL_B200_ERR_ARGS;   // the merge keeps 8 factors per part in shared memory
     const SharedLayout L = shared_layout(n_seqs, max_kv_len, p.slots, n_heads, n_kv_heads, head_dim,
                                          weights_out != nullptr);
     uint8_t *base = static_cast<uint8_t *>(workspace);
