@@ -114,15 +114,17 @@ __device__ __forceinline__ void own_range(const SharedParams &p, int b, int &ks,
 // ===========================================================================
 // prefix
 // ===========================================================================
-// CTA = (query tile, KV head and chunk of keys, prefix).  Warps 0-3: softmax, one packed
-// row per thread (thread = TMEM lane); warp 4: TMA producer; warp 5: tcgen05 issuer.
-//   S = Q K^T  (QT bf16 terms of Q, fp32 in TMEM, two buffers: S of the next key tile is
-//              computed during this tile's softmax)
+// CTA = (query tile, KV head and chunk of keys, prefix): softmax warpgroups of one packed
+// row per thread (thread = TMEM lane), a TMA producer warp and a tcgen05 issuer warp.
+//   S = Q K^T  (QT bf16 terms of Q, fp32 in TMEM, two buffers)
 //   P = 2^(S*scale*log2e - m) as PT fp16 terms over S's columns
 //   O += P V
+// Head dims 64 and 128 run two softmax warpgroups on alternate key tiles, each with an O
+// and a reference point of its own, joined at the end: the exponentials of a tile take
+// longer than its products (one warpgroup left the tensor pipe 34 % busy).  Head dim 256,
+// whose O fills half of TMEM, runs one.
 // Row r of tile t is query head (r' % group) of sequence s0 + r'/group, r' = 128 t + r.
 constexpr int kBM = 128;
-constexpr int kPrefixThreads = 192;
 constexpr float kMoveLog2 = 8.0f;
 
 template <int HD, int QT>
@@ -142,21 +144,27 @@ struct PrefixShape {
     static_assert(kUsed <= 227 * 1024, "shared memory");
     // one CTA per SM: each allocates all 512 TMEM columns
     static constexpr int kSmemBytes = kUsed > 118 * 1024 ? kUsed : 118 * 1024;
-    static constexpr int kTmO = 2 * BN;
+    static constexpr int kGroups = HD == 256 ? 1 : 2;   // softmax warpgroups
+    static constexpr int kSoftmax = kGroups * kBM;
+    static constexpr int kThreads = kSoftmax + 64;
+    static constexpr int kTmO = 2 * BN;                 // O of warpgroup w at kTmO + w * HD
     static constexpr int kTmCols = 512;
+    static_assert(kTmO + kGroups * HD <= kTmCols, "TMEM");
 };
 
 struct PrefixBars {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done, o_final, mma_done;
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], o_final, mma_done;
     uint32_t tmem_base;
     int lo_min;
 };
 
 template <int HD, int QT, int PT>
-__global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_constant__ SharedParams p)
+__global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kernel(const __grid_constant__ SharedParams p)
 {
     using S = PrefixShape<HD, QT>;
-    constexpr int BN = S::BN, ST = S::kStages;
+    constexpr int BN = S::BN, ST = S::kStages, NG = S::kGroups;
+    constexpr int kProducer = NG * 4, kIssuer = kProducer + 1;
+    static_assert(sizeof(PrefixBars) <= 256, "barriers");
     griddep_wait();
     griddep_trigger();
     const int qt = blockIdx.x;
@@ -171,10 +179,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
     PrefixBars *bars = reinterpret_cast<PrefixBars *>(smem + S::kOffBar);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
-    // this thread's packed row (threads 0-127) and its first visible prefix key
-    const int pr = qt * kBM + static_cast<int>(threadIdx.x);
+    // this softmax thread's packed row and its first visible prefix key
+    const int pr = qt * kBM + static_cast<int>(threadIdx.x) % kBM;
     const int b = s0 + pr / p.group, head = kvh * p.group + pr % p.group;
-    const bool row_valid = threadIdx.x < kBM && b < s1;
+    const bool row_valid = warp < kProducer && b < s1;
     int lo = 0;
     if (row_valid && p.window > 0) {
         int ks, n;
@@ -183,7 +191,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
     }
     if (threadIdx.x == 0) {
         bars->lo_min = plen;
-        mbar_init(smem_u32(&bars->q_full), kBM);
+        mbar_init(smem_u32(&bars->q_full), S::kSoftmax);
         for (int s = 0; s < 2; ++s) {
             mbar_init(smem_u32(&bars->k_full[s]), 1);
             mbar_init(smem_u32(&bars->k_empty[s]), 1);
@@ -191,8 +199,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
             mbar_init(smem_u32(&bars->v_empty[s]), 1);
             mbar_init(smem_u32(&bars->s_full[s]), 1);
             mbar_init(smem_u32(&bars->p_full[s]), kBM);
+            mbar_init(smem_u32(&bars->o_done[s]), 1);
         }
-        mbar_init(smem_u32(&bars->o_done), 1);
         mbar_init(smem_u32(&bars->o_final), 1);
         mbar_init(smem_u32(&bars->mma_done), 1);
         fence_mbar_init();
@@ -206,12 +214,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
     const int n_tiles = key_hi > key_lo ? (key_hi - key_lo + BN - 1) / BN : 0;
     const long long slot = (static_cast<long long>(b) * p.n_heads + head) * p.slots + c;
     if (n_tiles == 0) {
-        if (row_valid) p.part_ml[slot] = make_float2(-INFINITY, 0.f);
+        if (row_valid && threadIdx.x < kBM) p.part_ml[slot] = make_float2(-INFINITY, 0.f);
         return;
     }
     const long long row_base = p.prefix_row0[g] + key_lo;
 
-    if (warp == 5) {
+    if (warp == kIssuer) {
         tmem_alloc(smem_u32(&bars->tmem_base), S::kTmCols);
         tmem_relinquish();
     }
@@ -222,7 +230,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
     uint8_t *sK = smem + S::kOffK;
     uint8_t *sV = smem + S::kOffV;
 
-    if (warp == 4) {
+    if (warp == kProducer) {
         // ================= TMA producer =================
         if (lane == 0) {
             tma_prefetch_desc(&p.tk);
@@ -252,7 +260,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
             for (int j = max(0, nv - ST); j < nv; ++j)
                 if (!mbar_wait(smem_u32(&bars->v_full[j % ST]), (j / ST) & 1, p.err, kErrDrain)) break;
         }
-    } else if (warp == 5) {
+    } else if (warp == kIssuer) {
         // ================= tcgen05 issuer (converged warp, one elected lane issues) =================
         constexpr uint32_t idesc_s = umma_idesc_f16(kBM, BN, true, false);
         constexpr uint32_t idesc_pv = umma_idesc_f16(kBM, HD, false, true);
@@ -270,16 +278,19 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                 for (int kk = 0; kk < BN / 16; ++kk) {
                     const uint64_t bd = umma_sdesc_sw128(v_addr + kk * 16 * 128, S::kKvSubBytes, 1024);
                     // columns of P: see the softmax (32-key groups: 16 of values, 16 of remainders)
-                    umma_ts_elect(tmem + S::kTmO, tmem + sb * BN + (kk >> 1) * 32 + t * 16 + (kk & 1) * 8, bd,
-                                  idesc_pv, (j > 0 || t < PT - 1 || kk > 0) ? 1u : 0u);
+                    umma_ts_elect(tmem + S::kTmO + (j % NG) * HD, tmem + sb * BN + (kk >> 1) * 32 + t * 16 + (kk & 1) * 8, bd,
+                                  idesc_pv, (j >= NG || t < PT - 1 || kk > 0) ? 1u : 0u);
                 }
-            umma_commit_elect(smem_u32(&bars->o_done));
+            umma_commit_elect(smem_u32(&bars->o_done[j % NG]));
             umma_commit_elect(smem_u32(&bars->v_empty[st]));
             return true;
         };
         bool ok = mbar_wait_warp(smem_u32(&bars->q_full), 0, p.err, kErrWaitSoftmax);
+        // Two warpgroups: P V of tile j - 2, whose P lies in the buffer of S(j), goes before
+        // S(j).  One: S(j) goes first, so that it runs during the softmax of tile j - 1.
         for (int j = 0; j < n_tiles && ok; ++j) {
             const int st = j % ST;
+            if (NG == 2 && j >= 2 && !(ok = issue_pv(j - 2))) break;
             if (!(ok = mbar_wait_warp(smem_u32(&bars->k_full[st]), (j / ST) & 1, p.err, kErrWaitTmaFull))) break;
             tc_fence_after();
             const uint32_t k_addr = smem_u32(sK + st * S::kKvBytes);
@@ -296,8 +307,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                 }
             umma_commit_elect(smem_u32(&bars->s_full[j & 1]));
             umma_commit_elect(smem_u32(&bars->k_empty[st]));
-            if (j >= 1) ok = issue_pv(j - 1);
+            if (NG == 1 && j >= 1) ok = issue_pv(j - 1);
         }
+        if (ok && NG == 2 && n_tiles >= 2) ok = issue_pv(n_tiles - 2);
         if (ok && issue_pv(n_tiles - 1)) umma_commit_elect(smem_u32(&bars->o_final));
         // every MMA must be complete before TMEM is released
         umma_commit_elect(smem_u32(&bars->mma_done));
@@ -308,15 +320,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
         // 8-element pieces in flight per lane (one at a time took 11 us of an 18 us call at
         // 512 prefix keys).  Rows past the last sequence stay unwritten: a row of Q only
         // reaches its own row of S and O, and those rows are neither used nor stored.
-        const bool warp_live = s0 + (qt * kBM + warp * 32) / p.group < s1;
-        if (warp_live) {
-            constexpr int kVecs = HD / 8, kLoad = 4;
-            for (int i0 = lane; i0 < 32 * kVecs; i0 += 32 * kLoad) {
+        constexpr int kVecs = HD / 8, kLoad = 4, kRows = 32 / NG;   // rows loaded by a warp
+        const int lr = warp * kRows;
+        if (s0 + (qt * kBM + lr) / p.group < s1) {
+            for (int i0 = lane; i0 < kRows * kVecs; i0 += 32 * kLoad) {
                 uint4 raw[kLoad][2];
 #pragma unroll
                 for (int n = 0; n < kLoad; ++n) {
                     const int i = i0 + 32 * n;
-                    const int rr = qt * kBM + warp * 32 + i / kVecs;
+                    const int rr = qt * kBM + lr + i / kVecs;
                     const int rb = s0 + rr / p.group, rh = kvh * p.group + rr % p.group;
                     const long long off = (static_cast<long long>(rb) * p.n_heads + rh) * HD + (i % kVecs) * 8;
                     if (rb < s1) {
@@ -332,7 +344,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
 #pragma unroll
                 for (int n = 0; n < kLoad; ++n) {
                     const int i = i0 + 32 * n;
-                    const int r = warp * 32 + i / kVecs, e = (i % kVecs) * 8;
+                    const int r = lr + i / kVecs, e = (i % kVecs) * 8;
                     if (s0 + (qt * kBM + r) / p.group >= s1) continue;
                     const uint32_t at = (e / 64) * S::kQSubBytes + sw128_offset(r, (e % 64) / 8);
                     const uint32_t u[8] = {raw[n][0].x, raw[n][0].y, raw[n][0].z, raw[n][0].w,
@@ -357,12 +369,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
         }
         fence_proxy_async_smem();
         mbar_arrive(smem_u32(&bars->q_full));
-        const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+        const int wg = warp / 4;
+        const bool warp_live = s0 + (qt * kBM + (warp % 4) * 32) / p.group < s1;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
+        const uint32_t o_col = lane_base + S::kTmO + wg * HD;
         const float cap = p.softcap, inv_cap = cap > 0.f ? 1.f / cap : 0.f;
         const float mul = cap > 0.f ? 1.f : p.scale * kLog2e;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int j = 0; j < n_tiles; ++j) {
+        for (int j = wg; j < n_tiles; j += NG) {
             const int sb = j & 1;
             ok = mbar_wait_warp(smem_u32(&bars->s_full[sb]), (j >> 1) & 1, p.err, kErrWaitMma);
             if (!ok) break;
@@ -413,18 +428,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
             if (__any_sync(0xffffffffu, move && !fresh)) {
                 const float f = move && !fresh ? fast_exp2(m - mx) : 1.f;
                 l *= f;
-                // j > 0 here; O holds the earlier tiles' P V: scale it once they are complete
-                ok = mbar_wait_warp(smem_u32(&bars->o_done), (j - 1) & 1, p.err, kErrWaitMma);
+                // not the first tile; O holds the earlier ones' P V: scale it once they are complete
+                ok = mbar_wait_warp(smem_u32(&bars->o_done[wg]), (j / NG - 1) & 1, p.err, kErrWaitMma);
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll 1
                 for (int q = 0; q < HD / 32; ++q) {
                     uint32_t ro[32];
-                    tmem_ld32(lane_base + S::kTmO + q * 32, ro);
+                    tmem_ld32(o_col + q * 32, ro);
                     tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 32; ++i) ro[i] = __float_as_uint(__uint_as_float(ro[i]) * f);
-                    tmem_st32(lane_base + S::kTmO + q * 32, ro);
+                    tmem_st32(o_col + q * 32, ro);
                 }
             }
             if (move) m = mx;
@@ -438,7 +453,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                 tmem_ld32(s_col + q * 32, rr);
                 tmem_ld_wait();
                 if (cap > 0.f) {
-#pragma unroll 4
+#pragma unroll
                     for (int i = 0; i < 32; ++i)
                         rr[i] = __float_as_uint(cap * tanhf(__uint_as_float(rr[i]) * p.scale * inv_cap) * kLog2e);
                 }
@@ -468,7 +483,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                 ok = mbar_wait_warp(smem_u32(&bars->v_full[j % ST]), (j / ST) & 1, p.err, kErrWaitTmaFull);
                 if (!ok) break;
                 uint8_t *vt = sV + (j % ST) * S::kKvBytes;
-                for (int i = threadIdx.x; i < (BN - nv) * 8 * S::kSub; i += kBM) {
+                for (int i = threadIdx.x % kBM; i < (BN - nv) * 8 * S::kSub; i += kBM) {
                     const int sub = i / ((BN - nv) * 8), k = i % ((BN - nv) * 8);
                     *reinterpret_cast<uint4 *>(vt + sub * S::kKvSubBytes + nv * 128 + k * 16) = make_uint4(0, 0, 0, 0);
                 }
@@ -480,27 +495,49 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
         }
         // o_done may be two phases behind here (a parity wait could not tell), hence o_final
         if (ok) ok = mbar_wait_warp(smem_u32(&bars->o_final), 0, p.err, kErrWaitMma);
-        if (ok) {
+        // after a wait that ran out the part counts as empty (the device error word is set)
+        if (!ok) m = -INFINITY, l = 0.f;
+        float M = m, f[2] = {1.f, 0.f};   // the row's reference, and each warpgroup's factor to it
+        const int half = threadIdx.x % kBM;
+        if (NG == 2) {
+            float2 *ml = reinterpret_cast<float2 *>(sK);   // the K tiles are no longer needed
+            ml[wg * kBM + half] = make_float2(m, l);
+            named_bar_sync(1, S::kSoftmax);
+            const float2 a = ml[half], d = ml[kBM + half];
+            M = fmaxf(a.x, d.x);
+            f[0] = a.x == -INFINITY ? 0.f : fast_exp2(a.x - M);
+            f[1] = d.x == -INFINITY ? 0.f : fast_exp2(d.x - M);
+            l = f[0] * a.y + f[1] * d.y;
+        }
+        if (__any_sync(0xffffffffu, row_valid && M != -INFINITY)) {
             tc_fence_after();
             float *dst = p.part_o + slot * HD;
-#pragma unroll
-            for (int q = 0; q < HD / 32; ++q) {
-                uint32_t ro[32];
-                tmem_ld32(lane_base + S::kTmO + q * 32, ro);
+#pragma unroll 1
+            for (int c0 = wg * (HD / NG); c0 < (wg + 1) * (HD / NG); c0 += 32) {
+                uint32_t r0[32], r1[32];
+                tmem_ld32(lane_base + S::kTmO + c0, r0);
+                if (NG == 2 && n_tiles > 1) tmem_ld32(lane_base + S::kTmO + HD + c0, r1);
                 tmem_ld_wait();
+                if (NG == 2) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        float x = f[0] != 0.f ? f[0] * __uint_as_float(r0[i]) : 0.f;
+                        if (n_tiles > 1 && f[1] != 0.f) x += f[1] * __uint_as_float(r1[i]);
+                        r0[i] = __float_as_uint(x);
+                    }
+                }
                 if (row_valid) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4 *>(dst + q * 32 + i) = make_uint4(ro[i], ro[i + 1], ro[i + 2], ro[i + 3]);
+                        *reinterpret_cast<uint4 *>(dst + c0 + i) = make_uint4(r0[i], r0[i + 1], r0[i + 2], r0[i + 3]);
                 }
             }
         }
-        // after a wait that ran out the part counts as empty (the device error word is set)
-        if (row_valid) p.part_ml[slot] = ok ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+        if (row_valid && wg == 0) p.part_ml[slot] = make_float2(M, l);
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == 5) {
+    if (warp == kIssuer) {
         tc_fence_after();
         tmem_dealloc(tmem, S::kTmCols);
     }
@@ -536,7 +573,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
 {
     using S = SplitShape<HD>;
     constexpr int KSTEPS = HD / 16;
-    griddep_wait();
+    // After a prefix kernel, whose CTAs have all passed their own wait when this grid starts,
+    // the inputs are complete and nothing here depends on it: the two run side by side, and
+    // this grid only may not end before it (the merge waits for this grid alone).
+    if (p.prefix_slots == 0) griddep_wait();
     griddep_trigger();
     const int b = blockIdx.z;
     const int kvh = blockIdx.y / p.n_qgroups, qg = blockIdx.y % p.n_qgroups;
@@ -544,7 +584,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
     int ks, n;
     own_range(p, b, ks, n);
     const int key0 = ks + c * p.chunk;
-    if (key0 >= n) return;
+    if (key0 >= n) {
+        if (p.prefix_slots > 0) griddep_wait();
+        return;
+    }
     const int nkeys = min(p.chunk, n - key0);
     const int ntiles = (nkeys + kKeysPerTile - 1) / kKeysPerTile;
     const int h_first = kvh * p.group + qg * 8;
@@ -784,6 +827,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
         p.part_o[slot * HD + d] = acc;
         if (d == 0) p.part_ml[slot] = make_float2(M, sum);
     }
+    if (p.prefix_slots > 0) griddep_wait();
 }
 
 // ===========================================================================
@@ -903,24 +947,33 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
 #pragma unroll
     for (int i = 0; i < kPer; ++i) w[i] = 0.f;
     const long long own = static_cast<long long>(b) * p.n_kv_heads + kvh;
+    auto load_pair = [&](const float *sc, int h, float2 (&x)[kPer]) {   // score_cols is even: 8-byte loads
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int j = j0 + i * kMergeThreads + static_cast<int>(threadIdx.x);
+            x[i] = j >= ks && j < n ? *reinterpret_cast<const float2 *>(sc + static_cast<long long>(j) * p.score_cols + h)
+                                    : make_float2(-INFINITY, -INFINITY);
+        }
+    };
+    float w_in[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int j = j0 + i * kMergeThreads + static_cast<int>(threadIdx.x);
+        w_in[i] = p.weights_in && j < n ? p.weights_in[own * p.weights_stride + j] : 0.f;
+    }
     for (int h0 = 0; h0 < p.group; h0 += 8) {
         const int nh = min(8, p.group - h0);
+        const float *sc = p.scores + own * p.score_rows * p.score_cols + h0;
+        float2 x[kPer];
+        load_pair(sc, 0, x);   // in flight while the sums are found
         if (warp < nh) {
             float M, inv;
             head_sum(p.part_ml + (row0 + h0 + warp) * p.slots, first, last, M, inv);
             if (lane == 0) s_M[warp] = M, s_inv[warp] = inv;
         }
         __syncthreads();
-        const float *sc = p.scores + own * p.score_rows * p.score_cols + h0;
-        for (int h = 0; h < nh; h += 2) {   // score_cols is even: a pair is one 8-byte load
-            float2 x[kPer];
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int j = j0 + i * kMergeThreads + static_cast<int>(threadIdx.x);
-                x[i] = j >= ks && j < n
-                           ? *reinterpret_cast<const float2 *>(sc + static_cast<long long>(j) * p.score_cols + h)
-                           : make_float2(-INFINITY, -INFINITY);
-            }
+        for (int h = 0; h < nh; h += 2) {
+            if (h > 0) load_pair(sc, h, x);
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 if (x[i].x != -INFINITY) w[i] += fast_exp2(x[i].x - s_M[h]) * s_inv[h];
@@ -933,7 +986,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int j = j0 + i * kMergeThreads + static_cast<int>(threadIdx.x);
-        if (j < n) p.weights_out[base + j] = (p.weights_in ? p.weights_in[base + j] : 0.f) + w[i];
+        if (j < n) p.weights_out[base + j] = w_in[i] + w[i];
     }
 }
 
@@ -1030,7 +1083,7 @@ int launch_shared(cudaStream_t st, SharedParams &p, const uint16_t *k_pool, cons
             return SMOL_B200_ERR_CUDA;
         const dim3 grid(div_up(static_cast<long long>(p.max_prefix_seqs) * p.group, kBM),
                         p.n_kv_heads * p.prefix_slots, p.n_prefixes);
-        if (launch_kernel(prefix_kernel<HD, QT, PT>, grid, dim3(kPrefixThreads), S::kSmemBytes, st, p) != cudaSuccess)
+        if (launch_kernel(prefix_kernel<HD, QT, PT>, grid, dim3(S::kThreads), S::kSmemBytes, st, p) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
     }
     if (p.max_kv_len > 0) {
