@@ -571,6 +571,51 @@ SMOL_B200_API int smol_b200_decode_attention_weights(
     const float *weights_in, float *weights_out, int64_t weights_stride, void *workspace,
     size_t workspace_bytes);
 
+/* Attention weights of prompt rows: for every key j < seq_k of batch element b, the
+ * probabilities with which the rows given (queries i of all heads of j's KV head) attend
+ * it are summed and added to weights [batch][n_kv_heads][weights_stride], weights_stride
+ * >= seq_k.  q, k, strides, scale, mask_kind (causal, prefix-LM or full), q_offset,
+ * prefix_len, window and softcap as in smol_b200_prefill_attention, so k may be the cache
+ * itself; to count the last rows of a prompt only, pass those rows with their q_offset.
+ * Rows that see no key add nothing; with seq_q == 0 weights_out is weights_in.  head_dim:
+ * any multiple of 8 up to 256; at most 128 query heads to a KV head; scale > 0; lengths
+ * and |q_offset| up to 2^29. */
+SMOL_B200_API size_t smol_b200_prefill_weights_workspace_bytes(int batch, int seq_q, int seq_k, int n_heads,
+                                                               int n_kv_heads, int head_dim);
+SMOL_B200_API int smol_b200_prefill_attention_weights(
+    void *stream, const float *weights_in, float *weights_out, int64_t weights_stride, const uint16_t *q,
+    int64_t q_row_stride, int64_t q_batch_stride, const uint16_t *k, int64_t k_row_stride, int64_t k_batch_stride,
+    int batch, int seq_q, int seq_k, int n_heads, int n_kv_heads, int head_dim, float scale, int mask_kind,
+    int q_offset, int prefix_len, int window, float softcap, void *workspace, size_t workspace_bytes);
+
+/* Brings every (sequence, KV head) of a batch to at most `budget` cached rows.  Sequence b
+ * holds kv_len_in[b] rows from pool row seq_row0[b] on, slot j of KV head h with running
+ * weight weights_in[b][h][j] and position positions_in[b][h][j] (int32, same stride), and
+ * has seen seq_pos[b] tokens.  A negative position stands for a row appended since the
+ * last eviction: it is seq_pos[b] - kv_len_in[b] + j, since rows are appended in order.  So
+ * a caller fills weights with 0 and positions with -1 once, appends at slot kv_len with
+ * RoPE position seq_pos, and advances both counters.
+ * What stays, separately for every KV head: positions below `sink`, positions >= seq_pos -
+ * `recent`, then the largest weights (equal ones: the lower slot first; NaN last), budget
+ * rows in all; sink + recent <= budget, budget >= 1.  The kept rows end in slots [0, budget)
+ * in no particular order: dropped slots below `budget`, in order, take the rows of the kept
+ * slots from `budget` on, in order, and no other row moves.  So a cache under eviction is
+ * for attention without a window (a window counts slots).
+ * weights_out / positions_out: the kept rows' weights and positions (all positions now
+ * explicit), 0 / -1 in the slots freed; kv_len_out[b] = min(kv_len_in[b], budget).  A
+ * sequence within its budget is copied as it is.  Each output may be its input; otherwise
+ * the arrays are disjoint, entries from kv_len_in[b] on are not written, and slots from
+ * `budget` on keep their K and V.  Sequences must not share rows.  max_kv_len bounds
+ * kv_len_in (at most 262144) and is <= stride; a length beyond it, or rows outside the
+ * pool, leave that sequence's rows where they are and are flagged in the device error word.
+ * head_dim: a multiple of 8 up to 256; pools 16-byte aligned. */
+SMOL_B200_API size_t smol_b200_cache_evict_workspace_bytes(int n_seqs, int max_kv_len, int n_kv_heads);
+SMOL_B200_API int smol_b200_cache_evict(
+    void *stream, uint16_t *k_pool, uint16_t *v_pool, int64_t pool_rows, const int64_t *seq_row0,
+    const float *weights_in, float *weights_out, const int *positions_in, int *positions_out, int64_t stride,
+    const int *kv_len_in, int *kv_len_out, const int *seq_pos, int n_seqs, int max_kv_len, int n_kv_heads,
+    int head_dim, int budget, int sink, int recent, void *workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -808,6 +808,45 @@ int smol_b200_decode_attention_weights(void *stream, void *out, int out_is_bf16,
                   "smol_b200_decode_attention_weights");
 }
 
+size_t smol_b200_prefill_weights_workspace_bytes(int batch, int seq_q, int seq_k, int n_heads, int n_kv_heads,
+                                                 int head_dim)
+{
+    return prefill_weights_workspace_bytes(batch, seq_q, seq_k, n_heads, n_kv_heads, head_dim);
+}
+
+int smol_b200_prefill_attention_weights(void *stream, const float *weights_in, float *weights_out,
+                                        int64_t weights_stride, const uint16_t *q, int64_t q_row_stride,
+                                        int64_t q_batch_stride, const uint16_t *k, int64_t k_row_stride,
+                                        int64_t k_batch_stride, int batch, int seq_q, int seq_k, int n_heads,
+                                        int n_kv_heads, int head_dim, float scale, int mask_kind, int q_offset,
+                                        int prefix_len, int window, float softcap, void *workspace,
+                                        size_t workspace_bytes)
+{
+    return record(prefill_attention_weights(static_cast<cudaStream_t>(stream), weights_in, weights_out,
+                                            weights_stride, q, q_row_stride, q_batch_stride, k, k_row_stride,
+                                            k_batch_stride, batch, seq_q, seq_k, n_heads, n_kv_heads, head_dim, scale,
+                                            mask_kind, q_offset, prefix_len, window, softcap, workspace,
+                                            workspace_bytes),
+                  "smol_b200_prefill_attention_weights");
+}
+
+size_t smol_b200_cache_evict_workspace_bytes(int n_seqs, int max_kv_len, int n_kv_heads)
+{
+    return cache_evict_workspace_bytes(n_seqs, max_kv_len, n_kv_heads);
+}
+
+int smol_b200_cache_evict(void *stream, uint16_t *k_pool, uint16_t *v_pool, int64_t pool_rows,
+                          const int64_t *seq_row0, const float *weights_in, float *weights_out,
+                          const int *positions_in, int *positions_out, int64_t stride, const int *kv_len_in,
+                          int *kv_len_out, const int *seq_pos, int n_seqs, int max_kv_len, int n_kv_heads,
+                          int head_dim, int budget, int sink, int recent, void *workspace, size_t workspace_bytes)
+{
+    return record(cache_evict(static_cast<cudaStream_t>(stream), k_pool, v_pool, pool_rows, seq_row0, weights_in,
+                              weights_out, positions_in, positions_out, stride, kv_len_in, kv_len_out, seq_pos, n_seqs,
+                              max_kv_len, n_kv_heads, head_dim, budget, sink, recent, workspace, workspace_bytes),
+                  "smol_b200_cache_evict");
+}
+
 // ---------------------------------------------------------------------------
 // Part 4
 // ---------------------------------------------------------------------------

@@ -181,4 +181,18 @@ int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const v
                             int window, float softcap, const float *weights_in, float *weights_out,
                             int64_t weights_stride, void *workspace, size_t workspace_bytes);
 
+// prefill_weights.cu, cache_evict.cu: attention weights of a prompt, eviction to a budget (Part 6)
+size_t prefill_weights_workspace_bytes(int batch, int seq_q, int seq_k, int n_heads, int n_kv_heads, int head_dim);
+int prefill_attention_weights(cudaStream_t st, const float *weights_in, float *weights_out, int64_t weights_stride,
+                              const uint16_t *q, int64_t q_row_stride, int64_t q_batch_stride, const uint16_t *k,
+                              int64_t k_row_stride, int64_t k_batch_stride, int batch, int seq_q, int seq_k,
+                              int n_heads, int n_kv_heads, int head_dim, float scale, int mask_kind, int q_offset,
+                              int prefix_len, int window, float softcap, void *workspace, size_t workspace_bytes);
+size_t cache_evict_workspace_bytes(int n_seqs, int max_kv_len, int n_kv_heads);
+int cache_evict(cudaStream_t st, uint16_t *k_pool, uint16_t *v_pool, int64_t pool_rows, const int64_t *seq_row0,
+                const float *weights_in, float *weights_out, const int *positions_in, int *positions_out,
+                int64_t stride, const int *kv_len_in, int *kv_len_out, const int *seq_pos, int n_seqs, int max_kv_len,
+                int n_kv_heads, int head_dim, int budget, int sink, int recent, void *workspace,
+                size_t workspace_bytes);
+
 }  // namespace smolb200

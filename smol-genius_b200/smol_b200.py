@@ -127,7 +127,7 @@ _SIGNATURES = {
                                      _c_void, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "smol_b200_layer_norm": (_c_int, [_c_void, _c_void, _c_int, _c_void, _c_void, _c_void, _c_int, _c_int,
                                       _c_float]),
-    # Part 6 (shared prefixes, attention weights)
+    # Part 6 (shared prefixes, attention weights, eviction)
     "smol_b200_decode_shared_workspace_bytes": (_c_size, [_c_int] * 8),
     "smol_b200_decode_attention_shared": (
         _c_int, [_c_void, _c_void, _c_int, _c_void, _c_int, _c_void, _c_void, _c_i64, _c_void, _c_void, _c_void, _c_int,
@@ -137,6 +137,14 @@ _SIGNATURES = {
     "smol_b200_decode_attention_weights": (
         _c_int, [_c_void, _c_void, _c_int, _c_void, _c_int, _c_void, _c_void, _c_i64, _c_void, _c_void, _c_int, _c_int,
                  _c_int, _c_int, _c_int, _c_float, _c_int, _c_float, _c_void, _c_void, _c_i64, _c_void, _c_size]),
+    "smol_b200_prefill_weights_workspace_bytes": (_c_size, [_c_int] * 6),
+    "smol_b200_prefill_attention_weights": (
+        _c_int, [_c_void, _c_void, _c_void, _c_i64, _c_void, _c_i64, _c_i64, _c_void, _c_i64, _c_i64, _c_int, _c_int,
+                 _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void, _c_size]),
+    "smol_b200_cache_evict_workspace_bytes": (_c_size, [_c_int] * 3),
+    "smol_b200_cache_evict": (
+        _c_int, [_c_void, _c_void, _c_void, _c_i64, _c_void, _c_void, _c_void, _c_void, _c_void, _c_i64, _c_void,
+                 _c_void, _c_void, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void, _c_size]),
 }
 
 
@@ -542,7 +550,7 @@ def layer_norm(out, x, w, b, rows, hidden, eps, out_bf16=False, stream=None):
 
 
 # ---------------------------------------------------------------------------
-# Part 6: shared prefixes, attention weights
+# Part 6: shared prefixes, attention weights, eviction
 # ---------------------------------------------------------------------------
 def decode_shared_workspace_bytes(n_seqs, max_kv_len, n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads,
                                   head_dim) -> int:
@@ -582,3 +590,39 @@ def decode_attention_weights(out, q, k_pool, v_pool, pool_rows, seq_row0, kv_len
         head_dim, scale, window, softcap, _ptr(weights_in), _ptr(weights_out), weights_stride, _ptr(workspace),
         workspace.numel() * workspace.element_size())
     check(rc, "smol_b200_decode_attention_weights")
+
+
+def prefill_weights_workspace_bytes(batch, seq_q, seq_k, n_heads, n_kv_heads, head_dim) -> int:
+    return lib().smol_b200_prefill_weights_workspace_bytes(batch, seq_q, seq_k, n_heads, n_kv_heads, head_dim)
+
+
+def prefill_attention_weights(weights_in, weights_out, weights_stride, q, k, batch, seq_q, seq_k, n_heads, n_kv_heads,
+                              head_dim, scale, workspace, mask_kind=MASK_CAUSAL, q_offset=0, prefix_len=0, window=0,
+                              softcap=0.0, strides=None, stream=None):
+    """q / k: bf16 [batch, seq, heads*hd] (contiguous unless `strides` = ((q_row, q_batch), (k_row, k_batch)) in
+    elements); weights fp32 [batch, n_kv_heads, weights_stride], weights_in None for zero."""
+    if strides is None:
+        qw, kw = n_heads * head_dim, n_kv_heads * head_dim
+        strides = ((qw, seq_q * qw), (kw, seq_k * kw))
+    (qrs, qbs), (krs, kbs) = strides
+    rc = lib().smol_b200_prefill_attention_weights(
+        _stream(stream), _ptr(weights_in), _ptr(weights_out), weights_stride, _ptr(q), qrs, qbs, _ptr(k), krs, kbs,
+        batch, seq_q, seq_k, n_heads, n_kv_heads, head_dim, scale, mask_kind, q_offset, prefix_len, window, softcap,
+        _ptr(workspace), workspace.numel() * workspace.element_size())
+    check(rc, "smol_b200_prefill_attention_weights")
+
+
+def cache_evict_workspace_bytes(n_seqs, max_kv_len, n_kv_heads) -> int:
+    return lib().smol_b200_cache_evict_workspace_bytes(n_seqs, max_kv_len, n_kv_heads)
+
+
+def cache_evict(k_pool, v_pool, pool_rows, seq_row0, weights_in, weights_out, positions_in, positions_out, stride,
+                kv_len_in, kv_len_out, seq_pos, n_seqs, max_kv_len, n_kv_heads, head_dim, budget, sink, recent,
+                workspace, stream=None):
+    """Weights fp32 and positions int32 [n_seqs, n_kv_heads, stride]; each output may be its input."""
+    rc = lib().smol_b200_cache_evict(
+        _stream(stream), _ptr(k_pool), _ptr(v_pool), pool_rows, _ptr(seq_row0), _ptr(weights_in), _ptr(weights_out),
+        _ptr(positions_in), _ptr(positions_out), stride, _ptr(kv_len_in), _ptr(kv_len_out), _ptr(seq_pos), n_seqs,
+        max_kv_len, n_kv_heads, head_dim, budget, sink, recent, _ptr(workspace),
+        workspace.numel() * workspace.element_size())
+    check(rc, "smol_b200_cache_evict")
