@@ -21,12 +21,12 @@
 #include <mutex>
 
 #include "b200_common.cuh"
+#include "fast_math.cuh"
 #include "runtime.h"
 
 namespace smolb200 {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 128;
 constexpr int kMaxTiles = 16;
 constexpr int kExpThreads = 256;              // two warpgroups, on alternate tiles
@@ -43,7 +43,8 @@ struct WShape {
     static constexpr int kStages = HD == 64 ? 4 : 2;
     static constexpr int kOffY = kTileBytes;
     static constexpr int kOffCols = kOffY + kStages * kTileBytes;
-    static constexpr int kColBytes = 2 * kTile * 12;         // per warpgroup: lse, first and past-last key of 128 rows
+    // per warpgroup, twice: -lse, first and past-last visible key of 128 rows
+    static constexpr int kColBytes = 2 * 2 * kTile * 12;
     static constexpr int kOffBar = kOffCols + kColBytes;
     static constexpr int kSmemBytes = kOffBar + 256 + 1024;
     static constexpr int kCtas = HD == 256 ? 1 : 2;          // per SM
@@ -73,11 +74,26 @@ struct WBars {
     uint32_t tmem_base;
 };
 
-__device__ __forceinline__ float fast_exp2(float x)
+// sum += 2^(v*mul + off) for 16 columns; kPoly of every 8 pairs on the FMA pipe, the rest on
+// MUFU.  A pair takes 16 MUFU cycles of a scheduler, or 12 issue slots on the FMA pipe.
+#ifndef SMOL_WEIGHTS_POLY
+#define SMOL_WEIGHTS_POLY 3
+#endif
+constexpr int kPoly = SMOL_WEIGHTS_POLY;
+__device__ __forceinline__ void add_exp2(const uint32_t (&v)[16], float mul, const float (&off)[16], float (&acc)[4])
 {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float x0, x1, e0, e1;
+        pair_fma(x0, x1, __uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), mul, mul, off[2 * i], off[2 * i + 1]);
+        if ((i * kPoly) % 8 < kPoly) {
+            pair_exp2_poly(x0, x1, e0, e1);
+        } else {
+            e0 = fast_exp2f(x0);
+            e1 = fast_exp2f(x1);
+        }
+        pair_add(acc[2 * (i & 1)], acc[2 * (i & 1) + 1], acc[2 * (i & 1)], acc[2 * (i & 1) + 1], e0, e1);
+    }
 }
 
 // Keys [lo, hi) that query i sees (both non-decreasing in i).
@@ -234,30 +250,40 @@ __global__ void __launch_bounds__(kThreads, WShape<HD>::kCtas) weights_kernel(co
         const float cap = p.softcap, inv_cap = cap > 0.f ? 1.f / cap : 0.f;
         const float mul = cap > 0.f ? 1.f : p.scale * kLog2e;
         const long long rows = static_cast<long long>(p.seq_q) * p.group;
-        float *col_lse = reinterpret_cast<float *>(smem + S::kOffCols) + wg * kTile;
-        int *col_lo = reinterpret_cast<int *>(smem + S::kOffCols + 2 * kTile * 4) + wg * kTile;
-        int *col_hi = col_lo + 2 * kTile;
+        // this warpgroup's two column sets: -lse, then the first and the past-last visible key
+        float *cols = reinterpret_cast<float *>(smem + S::kOffCols) + wg * 2 * 3 * kTile;
         // A wait that runs out (the device error word is set) skips the tiles that follow, but
         // every warp keeps to the barriers it shares with the others.
         bool ok = true;
-        auto capped = [&](uint32_t (&v)[32]) {
+        auto capped = [&](uint32_t (&v)[16]) {
             if (cap > 0.f) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
+                for (int i = 0; i < 16; ++i)
                     v[i] = __float_as_uint(cap * tanhf(__uint_as_float(v[i]) * p.scale * inv_cap) * kLog2e);
             }
         };
-        // row tile t: this thread's column of S^T into shared memory (lse, visible keys)
-        auto load_cols = [&](int t) {
-            const int i = t * p.qp + r / p.group;
-            const bool valid = r < p.qp * p.group && i < p.seq_q;
+        const int r_query = r / p.group;   // query of this thread's row or column within a row tile
+        const bool r_used = r < p.qp * p.group;
+        // -lse of this thread's column of row tile t (-inf: nothing is added)
+        auto neg_lse = [&](int t) -> float {
+            const bool valid = r_used && t * p.qp + r_query < p.seq_q;
+            return valid ? -p.lse[unit * rows + static_cast<long long>(t) * p.qp * p.group + r] : -INFINITY;
+        };
+        // Column set `set` = row tile t.  One barrier: a set is written again two tiles later.
+        // Returns whether a NaN is among the lse: it has to reach the weights.
+        auto load_cols = [&](int t, int set, float nl) -> bool {
             int lo = 0, hi = 0;
-            if (valid) row_keys(p, i, lo, hi);
-            named_bar_sync(1 + wg, kTile);   // the warpgroup has read the last tile's columns
-            col_lse[r] = valid ? p.lse[unit * rows + static_cast<long long>(t) * p.qp * p.group + r] : INFINITY;
-            col_lo[r] = lo;
-            col_hi[r] = hi;
-            named_bar_sync(1 + wg, kTile);
+            if (r_used && t * p.qp + r_query < p.seq_q) row_keys(p, t * p.qp + r_query, lo, hi);
+            float *c = cols + set * 3 * kTile;
+            c[r] = nl;
+            reinterpret_cast<int *>(c)[kTile + r] = lo;
+            reinterpret_cast<int *>(c)[2 * kTile + r] = hi;
+            int any;
+            asm volatile("{ .reg .pred p, q; setp.ne.b32 p, %1, 0; barrier.cta.red.or.pred q, %2, %3, p; selp.b32 %0, 1, 0, q; }"
+                         : "=r"(any)
+                         : "r"(nl != nl ? 1 : 0), "r"(1 + wg), "r"(kTile)
+                         : "memory");
+            return any != 0;
         };
         // whether every row of row tile t sees all of keys [k0, k1)
         auto all_visible = [&](int t, int k0, int k1) -> bool {
@@ -268,8 +294,8 @@ __global__ void __launch_bounds__(kThreads, WShape<HD>::kCtas) weights_kernel(co
         };
 
         if constexpr (MODE == kStats) {
-            const int i = x * p.qp + r / p.group;
-            const bool valid = r < p.qp * p.group && i < p.seq_q;
+            const int i = x * p.qp + r_query;
+            const bool valid = r_used && i < p.seq_q;
             const bool live = __any_sync(0xffffffffu, valid);
             int lo = 0, hi = 0;
             if (valid) row_keys(p, i, lo, hi);
@@ -280,16 +306,13 @@ __global__ void __launch_bounds__(kThreads, WShape<HD>::kCtas) weights_kernel(co
                     tc_fence_after();
                     const uint32_t s_col = lane_base + wg * kTile;
                     const int key0 = (t0 + t) * kTile;
-                    const bool whole = __all_sync(0xffffffffu, key0 >= lo && key0 + kTile <= hi);
-                    auto group32 = [&](int q, uint32_t (&v)[32]) {
-                        tmem_ld32(s_col + q * 32, v);
-                        tmem_ld_wait();
+                    // rows past the last one may see anything: they are not stored
+                    const bool whole = __all_sync(0xffffffffu, !valid || (key0 >= lo && key0 + kTile <= hi));
+                    auto hide = [&](int c0, uint32_t (&v)[16]) {
                         if (!whole) {
 #pragma unroll
-                            for (int c = 0; c < 32; ++c) {
-                                const int key = key0 + q * 32 + c;
-                                if (key < lo || key >= hi) v[c] = 0xff800000u;
-                            }
+                            for (int c = 0; c < 16; ++c)
+                                if (key0 + c0 + c < lo || key0 + c0 + c >= hi) v[c] = 0xff800000u;   // -inf
                         }
                     };
                     // fp32 sums need no maximum close by, only no overflow: a row's reference is
@@ -299,40 +322,47 @@ __global__ void __launch_bounds__(kThreads, WShape<HD>::kCtas) weights_kernel(co
                     for (int pass = 0; pass < 2; ++pass) {
                         if (need) {
                             float mx = -INFINITY;
-#pragma unroll 1
-                            for (int q = 0; q < 4; ++q) {
-                                uint32_t v[32];
-                                group32(q, v);
+                            for_columns(s_col, kTile / 16, [&](int c0, uint32_t (&v)[16]) {
+                                hide(c0, v);
 #pragma unroll
-                                for (int c = 0; c < 32; ++c) mx = fmaxf(mx, __uint_as_float(v[c]));
-                            }
+                                for (int c = 0; c < 16; ++c) mx = fmaxf(mx, __uint_as_float(v[c]));
+                            });
                             if (mx != -INFINITY)
                                 mx = cap > 0.f ? cap * tanhf(mx * p.scale * inv_cap) * kLog2e : mx * mul;
                             const bool move = m == -INFINITY || (pass == 1 && !(lt <= kSumLimit));
                             if (move && mx != -INFINITY) {
-                                if (m != -INFINITY) l *= fast_exp2(m - mx);
+                                if (m != -INFINITY) l *= fast_exp2f(m - mx);
                                 m = mx;
                             }
                         }
                         const float negm = m != -INFINITY ? -m : 0.f;
                         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-                        for (int q = 0; q < 4; ++q) {
-                            uint32_t v[32];
-                            tmem_ld32(s_col + q * 32, v);
-                            tmem_ld_wait();
-                            capped(v);
-                            if (!whole) {
+                        if (whole && !need) {
+                            float off[16];
 #pragma unroll
-                                for (int c = 0; c < 32; ++c) {
-                                    const int key = key0 + q * 32 + c;
-                                    if (key < lo || key >= hi) v[c] = 0xff800000u;
-                                }
-                            }
+                            for (int c = 0; c < 16; ++c) off[c] = negm;
+                            // a score may still be far above m (the sum then passes the limit):
+                            // the polynomial's exponent must not wrap, so the scores' maximum is
+                            // kept beside the sum
+                            float top = -INFINITY;
+                            for_columns(s_col, kTile / 16, [&](int c0, uint32_t (&v)[16]) {
+                                capped(v);
 #pragma unroll
-                            for (int c = 0; c < 32; ++c) acc[c & 3] += fast_exp2(fmaf(__uint_as_float(v[c]), mul, negm));
+                                for (int c = 0; c < 16; c += 2)
+                                    top = fmaxf(top, fmaxf(__uint_as_float(v[c]), __uint_as_float(v[c + 1])));
+                                add_exp2(v, mul, off, acc);
+                            });
+                            lt = fmaf(top, mul, negm) > 60.f ? INFINITY : (acc[0] + acc[1]) + (acc[2] + acc[3]);
+                        } else {
+                            for_columns(s_col, kTile / 16, [&](int c0, uint32_t (&v)[16]) {
+                                capped(v);
+                                hide(c0, v);
+#pragma unroll
+                                for (int c = 0; c < 16; ++c)
+                                    acc[c & 3] += fast_exp2f(fmaf(__uint_as_float(v[c]), mul, negm));
+                            });
+                            lt = (acc[0] + acc[1]) + (acc[2] + acc[3]);
                         }
-                        lt = (acc[0] + acc[1]) + (acc[2] + acc[3]);
                         need = __any_sync(0xffffffffu, !(lt <= kSumLimit));
                         if (!need) break;
                     }
@@ -349,49 +379,53 @@ __global__ void __launch_bounds__(kThreads, WShape<HD>::kCtas) weights_kernel(co
                 const float2 o = other[r];
                 const float M = fmaxf(m, o.x);
                 float L = 0.f;
-                if (m != -INFINITY) L += l * fast_exp2(m - M);
-                if (o.x != -INFINITY) L += o.y * fast_exp2(o.x - M);
+                if (m != -INFINITY) L += l * fast_exp2f(m - M);
+                if (o.x != -INFINITY) L += o.y * fast_exp2f(o.x - M);
                 const long long row = unit * rows + static_cast<long long>(x) * p.qp * p.group + r;
                 if (p.n_stat_parts == 1) p.lse[row] = M == -INFINITY ? INFINITY : M + log2f(L);
                 else p.stat_parts[row * p.n_stat_parts + part] = make_float2(M, L);
             }
         } else {
-            // sum over this tile's columns of 2^(S - lse) for key `key`
-            auto tile_sum = [&](int key, bool whole) -> float {
+            // sum over the first n16 * 16 columns of the tile in this warpgroup's buffer, columns
+            // described by `set`, of 2^(S - lse) for key `key`; `whole`: the key sees them all
+            auto tile_sum = [&](int key, int set, int n16, bool whole) -> float {
+                const float *c = cols + set * 3 * kTile;
+                const int *c_lo = reinterpret_cast<const int *>(c) + kTile, *c_hi = c_lo + kTile;
                 float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t v[32];
-                    tmem_ld32(lane_base + wg * kTile + q * 32, v);
-                    tmem_ld_wait();
+                for_columns(lane_base + wg * kTile, n16, [&](int c0, uint32_t (&v)[16]) {
                     capped(v);
+                    float off[16];
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
-                        const float4 e = *reinterpret_cast<const float4 *>(col_lse + q * 32 + c);
-                        float y[4] = {fast_exp2(fmaf(__uint_as_float(v[c]), mul, -e.x)),
-                                      fast_exp2(fmaf(__uint_as_float(v[c + 1]), mul, -e.y)),
-                                      fast_exp2(fmaf(__uint_as_float(v[c + 2]), mul, -e.z)),
-                                      fast_exp2(fmaf(__uint_as_float(v[c + 3]), mul, -e.w))};
-                        if (!whole) {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (key < col_lo[q * 32 + c + k] || key >= col_hi[q * 32 + c + k]) y[k] = 0.f;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) acc[k] += y[k];
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 e = *reinterpret_cast<const float4 *>(c + c0 + i);
+                        off[i] = e.x, off[i + 1] = e.y, off[i + 2] = e.z, off[i + 3] = e.w;
                     }
-                }
+                    if (whole) {
+                        add_exp2(v, mul, off, acc);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float y = fast_exp2f(fmaf(__uint_as_float(v[i]), mul, off[i]));
+                            if (key >= c_lo[c0 + i] && key < c_hi[c0 + i]) acc[i & 3] += y;
+                        }
+                    }
+                });
                 return (acc[0] + acc[1]) + (acc[2] + acc[3]);
             };
+            // columns of row tile t that hold rows
+            auto used_cols = [&](int t) -> int { return min(p.qp, p.seq_q - t * p.qp) * p.group; };
             if constexpr (MODE == kSums) {
                 const int k0 = x * kTile, key = k0 + r, k1 = min(p.seq_k, k0 + kTile);
                 float sum = 0.f;
+                float nl = wg < n ? neg_lse(t0 + wg) : 0.f;
                 for (int t = wg; t < n; t += 2) {
-                    load_cols(t0 + t);
+                    const int set = (t >> 1) & 1, used = used_cols(t0 + t);
+                    const bool nan = load_cols(t0 + t, set, nl);
+                    if (t + 2 < n) nl = neg_lse(t0 + t + 2);   // in flight during this tile
                     if (ok) ok = mbar_wait_warp(smem_u32(&bars->d_full[wg]), (t / 2) & 1, p.err, kErrWaitMma);
                     if (ok) {
                         tc_fence_after();
-                        sum += tile_sum(key, all_visible(t0 + t, k0, k1));
+                        sum += tile_sum(key, set, (used + 15) / 16, !nan && used % 16 == 0 && all_visible(t0 + t, k0, k1));
                         tc_fence_before();
                     }
                     mbar_arrive(smem_u32(&bars->d_empty[wg]));
@@ -410,21 +444,22 @@ __global__ void __launch_bounds__(kThreads, WShape<HD>::kCtas) weights_kernel(co
                     }
                 }
             } else {
-                if (n > 0) load_cols(0);
+                const int used = used_cols(0);
+                const bool nan = n > 0 ? load_cols(0, 0, neg_lse(0)) : false;
                 for (int t = wg; t < n; t += 2) {
-                    if (ok) ok = mbar_wait_warp(smem_u32(&bars->d_full[wg]), (t / 2) & 1, p.err, kErrWaitMma);
                     const int k0 = (t0 + t) * kTile, key = k0 + r;
+                    const long long at = unit * p.weights_stride + key;
+                    const float before = p.weights_in && key < p.seq_k ? p.weights_in[at] : 0.f;
+                    if (ok) ok = mbar_wait_warp(smem_u32(&bars->d_full[wg]), (t / 2) & 1, p.err, kErrWaitMma);
                     float sum = 0.f;
                     if (ok) {
                         tc_fence_after();
-                        sum = tile_sum(key, all_visible(0, k0, min(p.seq_k, k0 + kTile)));
+                        sum = tile_sum(key, 0, (used + 15) / 16,
+                                       !nan && used % 16 == 0 && all_visible(0, k0, min(p.seq_k, k0 + kTile)));
                         tc_fence_before();
                     }
                     mbar_arrive(smem_u32(&bars->d_empty[wg]));
-                    if (key < p.seq_k) {
-                        const long long at = unit * p.weights_stride + key;
-                        p.weights_out[at] = (p.weights_in ? p.weights_in[at] : 0.f) + sum;
-                    }
+                    if (key < p.seq_k) p.weights_out[at] = before + sum;
                 }
             }
         }
@@ -439,21 +474,26 @@ __global__ void __launch_bounds__(kThreads, WShape<HD>::kCtas) weights_kernel(co
     }
 }
 
-// lse of every row from its parts.
-__global__ void __launch_bounds__(256) weights_lse_kernel(float *lse, const float2 *parts, long long rows, int n_parts)
+// lse of every row from its parts, `width` (a power of two up to 32) lanes to a row.
+__global__ void __launch_bounds__(256) weights_lse_kernel(float *lse, const float2 *parts, long long rows, int n_parts,
+                                                          int width)
 {
     griddep_wait();
     griddep_trigger();
-    const long long r = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    if (r >= rows) return;
-    float M = -INFINITY;
-    for (int c = 0; c < n_parts; ++c) M = fmaxf(M, parts[r * n_parts + c].x);
-    float L = 0.f;
-    for (int c = 0; c < n_parts; ++c) {
-        const float2 v = parts[r * n_parts + c];
-        if (v.x != -INFINITY) L += v.y * fast_exp2(v.x - M);
-    }
-    lse[r] = M == -INFINITY ? INFINITY : M + log2f(L);
+    const long long t = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    const long long r = t / width;
+    const int lane = static_cast<int>(t % width);
+    float M = -INFINITY, L = 0.f;
+    if (r < rows)
+        for (int c = lane; c < n_parts; c += width) M = fmaxf(M, parts[r * n_parts + c].x);
+    for (int o = width / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if (r < rows)
+        for (int c = lane; c < n_parts; c += width) {
+            const float2 v = parts[r * n_parts + c];
+            if (v.x != -INFINITY) L += v.y * fast_exp2f(v.x - M);
+        }
+    for (int o = width / 2; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (r < rows && lane == 0) lse[r] = M == -INFINITY ? INFINITY : M + log2f(L);
 }
 
 // weights_out = weights_in + the parts, in order (no parts: a copy).
@@ -472,14 +512,14 @@ __global__ void __launch_bounds__(256) weights_add_kernel(float *out, const floa
     out[unit * stride + j] = (in ? in[unit * stride + j] : 0.f) + s;
 }
 
-// How the two passes are cut: parts of at most kMaxTiles tiles, shorter ones while the CTAs
-// do not fill the GPU twice over.
+// How the two passes are cut: parts of at most kMaxTiles tiles, shorter ones where the CTAs
+// would not fill the GPU, but no more of them than run at once.
 struct WPlan {
     int qp, row_tiles, key_tiles, stat_tiles, n_stat_parts, sum_tiles, n_sum_parts;
     size_t lse, sum_parts, total;   // stat_parts at 0
 };
 
-WPlan weights_plan(int batch, int seq_q, int seq_k, int n_heads, int n_kv_heads)
+WPlan weights_plan(int batch, int seq_q, int seq_k, int n_heads, int n_kv_heads, int head_dim)
 {
     WPlan w;
     const int group = n_heads / n_kv_heads;
@@ -489,21 +529,19 @@ WPlan weights_plan(int batch, int seq_q, int seq_k, int n_heads, int n_kv_heads)
     w.qp = kTile / group;
     w.row_tiles = up(seq_q, w.qp);
     w.key_tiles = up(seq_k, kTile);
+    const long long at_once = 148 * (head_dim > 128 ? WShape<256>::kCtas : WShape<128>::kCtas);
     // tiles of a part for `stay` staying tiles per unit and `stream` streaming ones
-    auto cut = [&](long long stay, int stream) {
-        int tiles = kMaxTiles;
-        while (tiles > 2 && units * stay * up(stream, tiles) < 2 * 148) tiles /= 2;
-        return tiles;
+    auto cut = [&](long long stay, int stream, int &tiles, int &parts) {
+        long long n = units * stay > 0 ? at_once / (units * stay) : 1;
+        const int least = up(stream, kMaxTiles);
+        if (n < least) n = least;
+        if (n > stream) n = stream;
+        tiles = n > 0 ? up(stream, n) : 1;
+        parts = up(stream, tiles);
     };
-    w.stat_tiles = cut(w.row_tiles, w.key_tiles);
-    w.n_stat_parts = up(w.key_tiles, w.stat_tiles);
-    if (w.row_tiles == 1) {
-        w.sum_tiles = cut(1, w.key_tiles);
-        w.n_sum_parts = up(w.key_tiles, w.sum_tiles);
-    } else {
-        w.sum_tiles = cut(w.key_tiles, w.row_tiles);
-        w.n_sum_parts = up(w.row_tiles, w.sum_tiles);
-    }
+    cut(w.row_tiles, w.key_tiles, w.stat_tiles, w.n_stat_parts);
+    if (w.row_tiles == 1) cut(1, w.key_tiles, w.sum_tiles, w.n_sum_parts);
+    else cut(w.key_tiles, w.row_tiles, w.sum_tiles, w.n_sum_parts);
     const size_t rows = static_cast<size_t>(units) * seq_q * group;
     w.lse = w.n_stat_parts > 1 ? al(rows * w.n_stat_parts * 8) : 0;
     w.sum_parts = w.lse + al(rows * 4);
@@ -547,8 +585,10 @@ int launch_weights(cudaStream_t st, const WParams &p)
     if (rc != SMOL_B200_OK) return rc;
     if (p.n_stat_parts > 1) {
         const long long rows = static_cast<long long>(p.batch) * p.n_kv_heads * p.seq_q * p.group;
-        if (launch_kernel(weights_lse_kernel, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, st, p.lse,
-                          static_cast<const float2 *>(p.stat_parts), rows, p.n_stat_parts) != cudaSuccess)
+        int width = 1;
+        while (width < 32 && width < p.n_stat_parts) width *= 2;
+        if (launch_kernel(weights_lse_kernel, dim3(static_cast<unsigned>((rows * width + 255) / 256)), dim3(256), 0, st,
+                          p.lse, static_cast<const float2 *>(p.stat_parts), rows, p.n_stat_parts, width) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
     }
     if (p.row_tiles == 1) return launch_pass<HD, kSumsOneRowTile>(st, p, 1, p.n_sum_parts);
@@ -562,7 +602,7 @@ size_t prefill_weights_workspace_bytes(int batch, int seq_q, int seq_k, int n_he
     if (batch <= 0 || seq_q < 0 || seq_k < 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads ||
         n_heads / n_kv_heads > kTile || head_dim <= 0 || head_dim > 256 || head_dim % 8)
         return 0;
-    return weights_plan(batch, seq_q, seq_k, n_heads, n_kv_heads).total;
+    return weights_plan(batch, seq_q, seq_k, n_heads, n_kv_heads, head_dim).total;
 }
 
 int prefill_attention_weights(cudaStream_t st, const float *weights_in, float *weights_out, int64_t weights_stride,
@@ -587,7 +627,7 @@ int prefill_attention_weights(cudaStream_t st, const float *weights_in, float *w
     if (q_row_stride < static_cast<int64_t>(n_heads) * head_dim ||
         k_row_stride < static_cast<int64_t>(n_kv_heads) * head_dim)
         return SMOL_B200_ERR_ARGS;
-    const WPlan w = weights_plan(batch, seq_q, seq_k, n_heads, n_kv_heads);
+    const WPlan w = weights_plan(batch, seq_q, seq_k, n_heads, n_kv_heads, head_dim);
     if (!workspace || workspace_bytes < w.total || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return SMOL_B200_ERR_WORKSPACE;
     if (static_cast<long long>(w.row_tiles) * w.n_stat_parts > 0x7fffffffLL ||
