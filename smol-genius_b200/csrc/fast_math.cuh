@@ -1,5 +1,5 @@
-// fast_math.cuh -- exponentials of the attention-weight kernels to fp32 accuracy, on both
-// pipes that can compute them, and TMEM loads that overlap with them.
+// fast_math.cuh -- building blocks of the attention-weight kernels: exponentials of packed
+// score pairs, and TMEM loads that overlap with them.
 #pragma once
 
 #include "b200_common.cuh"
@@ -15,45 +15,36 @@ __device__ __forceinline__ float fast_exp2f(float x)   // MUFU: 16 a clock and S
     return y;
 }
 
-// d = a * b + c and d = a + b for pairs of floats (f32x2: twice the rate of scalar FMA).
-__device__ __forceinline__ void pair_fma(float &d0, float &d1, float a0, float a1, float b0, float b1, float c0,
-                                         float c1)
+// Two floats in a register pair.  Values that come from consecutive registers (a TMEM load)
+// and constants packed once outside a loop cost no moves.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi)
 {
-    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
-        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d0), "=f"(d1)
-        : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+    f32x2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
 }
-__device__ __forceinline__ void pair_add(float &d0, float &d1, float a0, float a1, float b0, float b1)
+__device__ __forceinline__ void unpack2(f32x2 v, float &lo, float &hi)
 {
-    asm("{\n\t.reg .b64 a, b, d;\n\t"
-        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d0), "=f"(d1)
-        : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
 }
-
-// 2^x for a pair on the FMA pipe: n = round(x) by adding 1.5 * 2^23, f = x - n in
-// [-1/2, 1/2], 2^f from a degree-5 polynomial fitted for relative error (7.5e-8; 2.1e-7
-// with its fp32 roundings, as ex2.approx), n added to the exponent.  x below -126 counts as
-// -126, so what should vanish is at most 2^-126; x must not exceed 127.
-__device__ __forceinline__ void pair_exp2_poly(float x0, float x1, float &e0, float &e1)
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c)
 {
-    constexpr float kMagic = 12582912.0f;
-    x0 = fmaxf(x0, -126.f);
-    x1 = fmaxf(x1, -126.f);
-    float j0, j1, n0, n1, f0, f1, p0, p1;
-    pair_add(j0, j1, x0, x1, kMagic, kMagic);
-    pair_add(n0, n1, j0, j1, -kMagic, -kMagic);
-    pair_fma(f0, f1, n0, n1, -1.f, -1.f, x0, x1);
-    pair_fma(p0, p1, 0x1.5c08e4p-10f, 0x1.5c08e4p-10f, f0, f1, 0x1.3d0c52p-7f, 0x1.3d0c52p-7f);
-    pair_fma(p0, p1, p0, p1, f0, f1, 0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f);
-    pair_fma(p0, p1, p0, p1, f0, f1, 0x1.ebf918p-3f, 0x1.ebf918p-3f);
-    pair_fma(p0, p1, p0, p1, f0, f1, 0x1.62e428p-1f, 0x1.62e428p-1f);
-    pair_fma(p0, p1, p0, p1, f0, f1, 0x1.000002p+0f, 0x1.000002p+0f);
-    e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(j0) << 23));
-    e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(j1) << 23));
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
+{
+    f32x2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ f32x2 exp2_2(f32x2 x)
+{
+    float a, b;
+    unpack2(x, a, b);
+    return pack2(fast_exp2f(a), fast_exp2f(b));
 }
 
 // 16 consecutive 32-bit TMEM columns (lane addressing as tmem_ld32), and the wait for every

@@ -333,6 +333,21 @@ def test_prompt_rising_scores_move_the_reference(cuda):
     no_error()
 
 
+@pytest.mark.parametrize("rows,row", [(300, 5), (300, 140), (20, 7)])
+def test_prompt_nan_row_reaches_the_keys_it_sees(cuda, rows, row):
+    keys = 300
+    g = torch.Generator(device=cuda).manual_seed(1)
+    q = torch.randn((1, rows, 4 * 64), device=cuda, generator=g).to(torch.bfloat16)
+    k = torch.randn((1, keys, 2 * 64), device=cuda, generator=g).to(torch.bfloat16)
+    q[0, row, 64:128] = float("nan")            # query head 1, of KV head 0
+    w = torch.empty((1, 2, keys), device=cuda)
+    ws = torch.empty(smol_b200.prefill_weights_workspace_bytes(1, rows, keys, 4, 2, 64), dtype=torch.uint8, device=cuda)
+    smol_b200.prefill_attention_weights(None, w, keys, q, k, 1, rows, keys, 4, 2, 64, 1.0 / 8, ws, q_offset=keys - rows)
+    torch.cuda.synchronize()
+    seen = keys - rows + row + 1
+    assert torch.isnan(w[0, 0, :seen]).all() and torch.isfinite(w[0, 0, seen:]).all() and torch.isfinite(w[0, 1]).all()
+
+
 def test_prompt_nothing_to_add(cuda):
     win, wout = torch.rand((2, 3, 50), device=cuda), torch.full((2, 3, 50), -3.0, device=cuda)
     q = torch.zeros(64, device=cuda, dtype=torch.bfloat16)
