@@ -47,6 +47,38 @@ __device__ __forceinline__ f32x2 exp2_2(f32x2 x)
     return pack2(fast_exp2f(a), fast_exp2f(b));
 }
 
+// 2^x for a pair on the FMA pipe: n = round(x) by adding 1.5 * 2^23, f = x - n in [-1/2, 1/2],
+// 2^f from a degree-5 polynomial fitted for relative error (7.5e-8; 2.1e-7 with its fp32
+// roundings, as ex2.approx), n added to the exponent field.  x outside [-126, 127] counts as
+// the nearer end; NaN gives the largest finite float, which no sum of probabilities reaches.
+__device__ __forceinline__ float clamp_exp(float x)
+{
+    float y;
+    asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(y) : "f"(x));   // -126
+    asm("min.NaN.f32 %0, %1, 0f42FE0000;" : "=f"(y) : "f"(y));   // 127
+    return y;
+}
+__device__ __forceinline__ f32x2 both(float c) { return pack2(c, c); }
+__device__ __forceinline__ f32x2 exp2_2_poly(f32x2 x)
+{
+    constexpr float kMagic = 12582912.0f;
+    float a, b;
+    unpack2(x, a, b);
+    x = pack2(clamp_exp(a), clamp_exp(b));
+    const f32x2 j = add2(x, both(kMagic));
+    const f32x2 f = fma2(add2(j, both(-kMagic)), both(-1.f), x);
+    f32x2 p = fma2(both(0x1.5c08e4p-10f), f, both(0x1.3d0c52p-7f));
+    p = fma2(p, f, both(0x1.c6b6e4p-5f));
+    p = fma2(p, f, both(0x1.ebf918p-3f));
+    p = fma2(p, f, both(0x1.62e428p-1f));
+    p = fma2(p, f, both(0x1.000002p+0f));
+    float p0, p1, j0, j1;
+    unpack2(p, p0, p1);
+    unpack2(j, j0, j1);
+    return pack2(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(j0) << 23)),
+                 __uint_as_float(__float_as_uint(p1) + (__float_as_uint(j1) << 23)));
+}
+
 // 16 consecutive 32-bit TMEM columns (lane addressing as tmem_ld32), and the wait for every
 // load of this thread; the wait names the registers, so no use of them moves above it.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])

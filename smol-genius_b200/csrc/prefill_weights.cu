@@ -12,12 +12,13 @@
 // The probabilities themselves are never stored.  Bound: two exponentials per visible
 // (row, key) pair at 16 per clock and SM; a tile's products take half as long.
 //
-// Both passes cut their long axis into parts of at most kMaxTiles streaming tiles, whose
-// results a small kernel joins in a fixed order, so that causal work spreads evenly and few
-// rows against many keys still fill the GPU.  One persistent CTA per SM takes the items
-// (staying tiles, part) in turn; its loads and products run ahead of the exponentials across
-// item ends.  Two tiles stay where they fit: streaming a tile for 128 rows alone is bound by
-// L2 (11.5 TB/s: 27 us of the stats pass at 4096 causal rows, 16/8 heads of 128).
+// One persistent CTA per SM.  The visible tiles of all staying tiles, laid end to end, are cut
+// into one contiguous run per CTA, so that causal work spreads evenly (whole items of up to
+// 8 tiles left the fullest CTA 40 % above the mean) and few rows against many keys still
+// fill the GPU; where a run ends inside a staying tile, the pieces are joined in a fixed
+// order by a small kernel.  Loads and products run ahead of the exponentials.  Two tiles
+// stay where they fit: streaming a tile for 128 rows alone is bound by L2 (11.5 TB/s: 27 us
+// of the stats pass at 4096 causal rows, 16/8 heads of 128).
 #include <string.h>
 
 #include <mutex>
@@ -30,21 +31,23 @@ namespace smolb200 {
 namespace {
 
 constexpr int kTile = 128;
-constexpr int kMaxTiles = 8;                  // streaming tiles of a part
 constexpr int kGroups = 4;                    // warpgroups of exponentials, a 128-column buffer of S each
 constexpr int kExpThreads = kGroups * 128;
 constexpr int kThreads = kExpThreads + 64;    // + TMA producer warp, tcgen05 issuer warp
 constexpr int kLseRing = 8;                   // row tiles whose lse are in shared memory
 constexpr float kSumLimit = 1.152921504606847e18f;   // 2^60: a tile's row sum beyond this moves the reference
 
-enum Mode { kStats = 0, kSums = 1, kSumsOneRowTile = 2 };
+// the *OneRowTile forms: at most 128 packed rows per (batch, KV head)
+enum Mode { kStats = 0, kSums = 1, kStatsOneRowTile = 2, kSumsOneRowTile = 3 };
 
 template <int HD, int MODE>
 struct WShape {
     static constexpr int kSub = HD / 64;
     static constexpr int kSubBytes = kTile * 128;
     static constexpr int kTileBytes = kSub * kSubBytes;
-    static constexpr int kStay = HD == 256 || MODE == kSumsOneRowTile ? 1 : 2;   // tiles that stay
+    static constexpr int kStay = HD == 256 || MODE >= kStatsOneRowTile ? 1 : 2;   // tiles that stay
+    // a staying tile's streaming tiles go to kWays warpgroups in turn: as many results per run
+    static constexpr int kWays = 4 / kStay;
     static constexpr int kXBytes = kStay * kTileBytes;
     static constexpr int kXStages = HD == 64 ? 2 : 1;
     static constexpr int kStages = HD == 256 ? 2 : 4;
@@ -59,17 +62,17 @@ struct WShape {
 
 struct WParams {
     CUtensorMap tq, tk;   // (column, head, row, batch); boxes 64 x group x qp x 1 and 64 x 1 x 128 x 1
-    float2 *stat_parts;   // [batch][n_kv_heads][rows][parts * pieces]: reference (log2 units), sum
+    float2 *stat_parts;   // [batch][n_kv_heads][rows][pieces]: reference (log2 units), sum
     float *nlse;          // [batch][n_kv_heads][row_tiles][128]: -lse, log2 units; -inf without keys or row
-    float *sum_parts;     // [parts * pieces][batch][n_kv_heads][seq_k]
+    float *sum_parts;     // [pieces][batch][n_kv_heads][seq_k]
     const float *weights_in;
     float *weights_out;
     long long weights_stride;
     unsigned *err;
     int batch, seq_q, seq_k, n_kv_heads, group, qp;   // qp: queries of a row tile
     int row_tiles, key_tiles;
-    int stay, tiles, parts;         // staying tiles per unit, streaming tiles of a part, parts
-    long long items;                // stay * parts * units
+    int stay, pieces;               // staying steps per unit; slots of partial results
+    long long unit_tiles, run;      // visible streaming tiles of a unit, of a CTA
     int mask_kind, q_offset, prefix_len, window;
     int q_bytes;                    // bytes of a row tile's boxes (all sub-tiles)
     float scale, softcap;
@@ -81,76 +84,173 @@ struct WBars {
 };
 
 // Keys [lo, hi) that query i sees (both non-decreasing in i).
-__device__ __forceinline__ void row_keys(const WParams &p, int i, int &lo, int &hi)
+__host__ __device__ __forceinline__ int imin(int a, int b) { return a < b ? a : b; }
+__host__ __device__ __forceinline__ int imax(int a, int b) { return a > b ? a : b; }
+
+__host__ __device__ __forceinline__ void row_keys(const WParams &p, int i, int &lo, int &hi)
 {
     const int pos = p.q_offset + i;
     hi = p.mask_kind == SMOL_MASK_CAUSAL      ? pos + 1
-         : p.mask_kind == SMOL_MASK_PREFIX_LM ? max(pos + 1, p.prefix_len)
+         : p.mask_kind == SMOL_MASK_PREFIX_LM ? imax(pos + 1, p.prefix_len)
                                               : p.seq_k;
-    hi = min(max(hi, 0), p.seq_k);
-    lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+    hi = imin(imax(hi, 0), p.seq_k);
+    lo = p.window > 0 ? imax(0, pos - p.window + 1) : 0;
     if (lo > hi) lo = hi;
 }
 
 // Row tiles [t0, t1) with a row that sees a key of [k0, k1).
-__device__ __forceinline__ void key_rows(const WParams &p, int k0, int k1, int &t0, int &t1)
+__host__ __device__ __forceinline__ void key_rows(const WParams &p, int k0, int k1, int &t0, int &t1)
 {
     int i0 = 0, i1 = p.seq_q;
     if (p.mask_kind == SMOL_MASK_CAUSAL || (p.mask_kind == SMOL_MASK_PREFIX_LM && k0 >= p.prefix_len))
-        i0 = max(0, k0 - p.q_offset);
+        i0 = imax(0, k0 - p.q_offset);
     if (p.window > 0) {   // lo < k1: pos <= k1 + window - 2
         const long long last = static_cast<long long>(k1) + p.window - 2 - p.q_offset;
-        if (last + 1 < i1) i1 = static_cast<int>(max(last + 1, 0ll));
+        if (last + 1 < i1) i1 = last + 1 > 0 ? static_cast<int>(last + 1) : 0;
     }
     t0 = i0 / p.qp;
     t1 = i1 > i0 ? (i1 + p.qp - 1) / p.qp : t0;
 }
 
-// Results per (row or key, part): a warpgroup each for the streaming tiles it took.
-template <int HD>
-constexpr int kPieces = HD == 256 ? 4 : 2;
+// Streaming tiles [t0, t1) of staying step x (kStay tiles of rows for the stats, of keys for
+// the sums).
+__host__ __device__ __forceinline__ void stream_range(const WParams &p, int mode, int kstay, int x, int &t0, int &t1)
+{
+    if (mode == kStats || mode == kStatsOneRowTile) {
+        int lo, hi, unused;
+        row_keys(p, x * kstay * p.qp, lo, unused);
+        const int last = (x + 1) * kstay < p.row_tiles ? (x + 1) * kstay * p.qp : p.seq_q;
+        row_keys(p, last - 1, unused, hi);
+        t0 = lo / kTile;
+        t1 = (hi + kTile - 1) / kTile;
+    } else if (mode == kSums) {
+        key_rows(p, x * kstay * kTile, (x + 1) * kstay < p.key_tiles ? (x + 1) * kstay * kTile : p.seq_k, t0, t1);
+    } else {
+        t0 = 0;
+        t1 = p.key_tiles;
+    }
+    if (t1 < t0) t1 = t0;
+}
 
-// One item: the staying tiles x*kStay .. of a (batch, KV head) against streaming tiles [t0, t0 + n).
-struct WItem {
-    int b, kvh, x, part, t0, n;
+// acc += 2^(v*mul + off) for 16 columns.  MUFU takes 16 cycles of a scheduler for a pair, the
+// FMA pipe 4 for its product and sum and 16 more for a polynomial: kPoly of every 8 pairs go
+// there.
+#ifndef SMOL_WEIGHTS_POLY
+#define SMOL_WEIGHTS_POLY 2
+#endif
+constexpr int kPoly = SMOL_WEIGHTS_POLY;
+template <typename Off>
+__device__ __forceinline__ void add_exp2(const uint32_t (&v)[16], f32x2 mul2, Off &&off, f32x2 &acc0, f32x2 &acc1)
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const f32x2 x = fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), mul2, off(i));
+        const f32x2 e = (i * kPoly) % 8 < kPoly ? exp2_2_poly(x) : exp2_2(x);
+        if (i & 1) acc1 = add2(acc1, e);
+        else acc0 = add2(acc0, e);
+    }
+}
+
+// One CTA's run, staying step by staying step: step x of unit (b, kvh) against streaming tiles
+// [t0, t0 + n), as piece `piece` of that step.
+struct WRun {
+    int unit, x, t0, n, piece;
+    int skip;             // tiles of step x before the run
+    long long left;       // tiles of the run from step x on
 };
 
 template <int HD, int MODE>
-__device__ __forceinline__ WItem item_geometry(const WParams &p, long long k)
+__device__ __forceinline__ bool run_step(const WParams &p, WRun &w)
 {
-    constexpr int NX = WShape<HD, MODE>::kStay;
-    WItem it;
-    const int units = p.batch * p.n_kv_heads;
-    const int unit = static_cast<int>(k % units);
-    const int r = static_cast<int>(k / units);
-    it.kvh = unit % p.n_kv_heads;
-    it.b = unit / p.n_kv_heads;
-    it.part = r % p.parts;
-    it.x = r / p.parts;
-    int t0, t1;
-    if constexpr (MODE == kStats) {
-        it.x = p.stay - 1 - it.x;   // causal rows see more keys the later they are: those first
-        int lo, hi, unused;
-        row_keys(p, it.x * NX * p.qp, lo, unused);
-        row_keys(p, min(p.seq_q, (it.x + 1) * NX * p.qp) - 1, unused, hi);
-        t0 = max(lo / kTile, it.part * p.tiles);
-        t1 = min((hi + kTile - 1) / kTile, (it.part + 1) * p.tiles);
-    } else if constexpr (MODE == kSums) {
-        key_rows(p, it.x * NX * kTile, min(p.seq_k, (it.x + 1) * NX * kTile), t0, t1);
-        t0 += it.part * p.tiles;
-        t1 = min(t1, t0 + p.tiles);
-    } else {
-        t0 = it.part * p.tiles;
-        t1 = min(p.key_tiles, t0 + p.tiles);
+    while (w.left > 0) {
+        if (w.x == p.stay) {
+            w.x = 0;
+            if (++w.unit == p.batch * p.n_kv_heads) return false;
+        }
+        int t0, t1;
+        stream_range(p, MODE, WShape<HD, MODE>::kStay, w.x, t0, t1);
+        w.t0 = t0 + w.skip;
+        w.n = static_cast<int>(min(static_cast<long long>(t1 - w.t0), w.left));
+        if (w.n > 0) return true;
+        ++w.x;
+        w.skip = 0;
+        w.piece = 0;
     }
-    it.t0 = t0;
-    it.n = max(0, t1 - t0);
-    return it;
+    return false;
+}
+__device__ __forceinline__ void run_next(WRun &w)
+{
+    w.left -= w.n;
+    ++w.x;
+    w.skip = 0;
+    w.piece = 0;
 }
 
-__device__ __forceinline__ const float *lse_of(const WParams &p, const WItem &it, int row_tile)
+// The run of CTA `cta`, found by one warp: tile number cta * run, then the staying step that
+// holds it by a scan over the steps of a unit.
+template <int HD, int MODE>
+__device__ WRun find_run(const WParams &p, int cta)
 {
-    return p.nlse + ((static_cast<long long>(it.b) * p.n_kv_heads + it.kvh) * p.row_tiles + row_tile) * kTile;
+    const int lane = threadIdx.x % 32;
+    WRun w;
+    const long long start = cta * p.run;
+    w.unit = static_cast<int>(start / p.unit_tiles);
+    const long long in_unit = start - w.unit * p.unit_tiles;
+    const long long all = p.unit_tiles * p.batch * p.n_kv_heads;
+    w.left = min(p.run, all - start);
+    w.x = 0, w.skip = 0, w.piece = 0, w.t0 = 0, w.n = 0;
+    long long before = 0;   // tiles of the steps before this batch of 32
+    for (int x0 = 0; x0 < p.stay; x0 += 32) {
+        int t0 = 0, t1 = 0;
+        if (x0 + lane < p.stay) stream_range(p, MODE, WShape<HD, MODE>::kStay, x0 + lane, t0, t1);
+        const int mine = t1 - t0;
+        int sum = mine;   // inclusive within the warp
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        const long long first = before + sum - mine;
+        const unsigned hit = __ballot_sync(0xffffffffu, first <= in_unit && in_unit < first + mine);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            const long long f = __shfl_sync(0xffffffffu, first, l);
+            w.x = x0 + l;
+            w.skip = static_cast<int>(in_unit - f);
+            w.piece = cta - static_cast<int>((w.unit * p.unit_tiles + f) / p.run);
+            return w;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    w.left = 0;
+    return w;
+}
+
+// Pieces of staying step x of `unit` (the whole block asks for one step): the runs that its
+// tiles lie in.
+__device__ int step_pieces(const WParams &p, int mode, int kstay, int unit, int x)
+{
+    __shared__ long long s_sum[32];
+    long long sum = 0;
+    for (int i = threadIdx.x; i < x; i += blockDim.x) {
+        int t0, t1;
+        stream_range(p, mode, kstay, i, t0, t1);
+        sum += t1 - t0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (threadIdx.x % 32 == 0) s_sum[threadIdx.x / 32] = sum;
+    __syncthreads();
+    long long f = unit * p.unit_tiles;
+    for (int i = 0; i < static_cast<int>(blockDim.x / 32); ++i) f += s_sum[i];
+    int t0, t1;
+    stream_range(p, mode, kstay, x, t0, t1);
+    return t1 > t0 ? static_cast<int>((f + t1 - t0 - 1) / p.run - f / p.run) + 1 : 0;
+}
+
+__device__ __forceinline__ const float *lse_of(const WParams &p, int unit, int row_tile)
+{
+    return p.nlse + (static_cast<long long>(unit) * p.row_tiles + row_tile) * kTile;
 }
 
 // `bytes` (a multiple of 16, both addresses too) from global to shared memory, counted by `bar`.
@@ -167,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     using S = WShape<HD, MODE>;
     constexpr int ST = S::kStages, XS = S::kXStages, NX = S::kStay;
     constexpr int kProducer = kGroups * 4, kIssuer = kProducer + 1;
-    constexpr bool kOne = MODE == kSumsOneRowTile;
+    constexpr bool kOne = MODE == kSumsOneRowTile, kRows = MODE == kStats || MODE == kStatsOneRowTile;
     griddep_wait();
     griddep_trigger();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -205,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = bars->tmem_base;
+    WRun w = find_run<HD, MODE>(p, blockIdx.x);
 
     if (warp == kProducer) {
         // ================= TMA producer =================
@@ -212,39 +313,37 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
             tma_prefetch_desc(&p.tq);
             tma_prefetch_desc(&p.tk);
             // 128 rows of the queries (rows: row tile t) or keys (key tile t); past the last: zeros
-            auto load = [&](uint32_t dst, uint32_t bar, bool rows, int t, const WItem &it) {
+            auto load = [&](uint32_t dst, uint32_t bar, bool rows, int t) {
+                const int b = w.unit / p.n_kv_heads, kvh = w.unit % p.n_kv_heads;
 #pragma unroll
                 for (int sub = 0; sub < S::kSub; ++sub) {
-                    if (rows)
-                        tma_load_4d(dst + sub * S::kSubBytes, &p.tq, bar, sub * 64, it.kvh * p.group, t * p.qp, it.b);
-                    else tma_load_4d(dst + sub * S::kSubBytes, &p.tk, bar, sub * 64, it.kvh, t * kTile, it.b);
+                    if (rows) tma_load_4d(dst + sub * S::kSubBytes, &p.tq, bar, sub * 64, kvh * p.group, t * p.qp, b);
+                    else tma_load_4d(dst + sub * S::kSubBytes, &p.tk, bar, sub * 64, kvh, t * kTile, b);
                 }
             };
-            int nx = 0, ny = 0;   // items with tiles, streaming tiles issued
+            int nx = 0, ny = 0;   // staying steps, streaming tiles issued
             bool ok = true;
-            for (long long k = blockIdx.x; k < p.items && ok; k += gridDim.x) {
-                const WItem it = item_geometry<HD, MODE>(p, k);
-                if (it.n == 0) continue;
+            for (; ok && run_step<HD, MODE>(p, w); run_next(w)) {
                 const int xs = nx % XS;
                 if (nx >= XS && !(ok = mbar_wait(smem_u32(&bars->x_empty[xs]), (nx / XS - 1) & 1, p.err, kErrWaitTmaEmpty)))
                     break;
                 const uint32_t xb = smem_u32(&bars->x_full[xs]);
                 mbar_arrive_expect_tx(xb, NX * (MODE == kSums ? S::kTileBytes : p.q_bytes) + (kOne ? kTile * 4 : 0));
-                if (kOne) bulk_load(smem_u32(smem + S::kOffLse) + nx % kLseRing * kTile * 4, lse_of(p, it, 0), kTile * 4, xb);
+                if (kOne) bulk_load(smem_u32(smem + S::kOffLse) + nx % kLseRing * kTile * 4, lse_of(p, w.unit, 0), kTile * 4, xb);
 #pragma unroll
                 for (int i = 0; i < NX; ++i)
-                    load(smem_u32(smem + xs * S::kXBytes + i * S::kTileBytes), xb, MODE != kSums, it.x * NX + i, it);
+                    load(smem_u32(smem + xs * S::kXBytes + i * S::kTileBytes), xb, MODE != kSums, w.x * NX + i);
                 ++nx;
-                for (int t = 0; t < it.n; ++t, ++ny) {
+                for (int t = 0; t < w.n; ++t, ++ny) {
                     const int st = ny % ST;
                     if (ny >= ST &&
                         !(ok = mbar_wait(smem_u32(&bars->y_empty[st]), (ny / ST - 1) & 1, p.err, kErrWaitTmaEmpty)))
                         break;
                     const uint32_t yb = smem_u32(&bars->y_full[st]);
                     mbar_arrive_expect_tx(yb, MODE == kSums ? p.q_bytes + kTile * 4 : S::kTileBytes);
-                    load(smem_u32(smem + S::kOffY + st * S::kTileBytes), yb, MODE == kSums, it.t0 + t, it);
+                    load(smem_u32(smem + S::kOffY + st * S::kTileBytes), yb, MODE == kSums, w.t0 + t);
                     if (MODE == kSums)   // a slot is free 8 tiles later: S of those was read before Y's slot was
-                        bulk_load(smem_u32(smem + S::kOffLse) + ny % kLseRing * kTile * 4, lse_of(p, it, it.t0 + t),
+                        bulk_load(smem_u32(smem + S::kOffLse) + ny % kLseRing * kTile * 4, lse_of(p, w.unit, w.t0 + t),
                                   kTile * 4, yb);
                 }
             }
@@ -258,12 +357,10 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
         constexpr uint32_t idesc = umma_idesc_f16(kTile, kTile, true, false);
         int nx = 0, ny = 0;
         bool ok = true;
-        for (long long k = blockIdx.x; k < p.items && ok; k += gridDim.x) {
-            const WItem it = item_geometry<HD, MODE>(p, k);
-            if (it.n == 0) continue;
+        for (; ok && run_step<HD, MODE>(p, w); run_next(w)) {
             const int xs = nx % XS;
             ok = mbar_wait_warp(smem_u32(&bars->x_full[xs]), (nx / XS) & 1, p.err, kErrWaitTmaFull);
-            for (int t = 0; t < it.n && ok; ++t, ++ny) {
+            for (int t = 0; t < w.n && ok; ++t, ++ny) {
                 const int st = ny % ST;
                 ok = mbar_wait_warp(smem_u32(&bars->y_full[st]), (ny / ST) & 1, p.err, kErrWaitTmaFull);
                 const uint32_t y_addr = smem_u32(smem + S::kOffY + st * S::kTileBytes);
@@ -293,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
         mbar_wait_warp(smem_u32(&bars->done), 0, p.err, kErrDrain);
     } else {
         // ================= exponentials: thread r of a warpgroup owns row r of S =================
-        // Use n of the buffers of S (streaming tile (g0 + t) of this CTA, staying tile i: n = (g0 + t) *
+        // Use n of the buffers of S (streaming tile g0 + t of this CTA, staying tile i: n = (g0 + t) *
         // NX + i) is buffer n % 4, and warpgroup n % 4 reads it.
         const int wg = warp / 4, r = threadIdx.x % kTile;
         const int stay = wg % NX;                       // the staying tile this warpgroup works for
@@ -326,29 +423,29 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
         // sum of 2^(S - lse) over columns [lo, hi) of this warpgroup's buffer, lse (negated) in
         // shared memory; `whole`: over all n16 * 16
         auto tile_sum = [&](const float *nl, int n16, bool whole, int lo, int hi) -> float {
-            f32x2 acc0 = 0, acc1 = 0;
+            if (whole) {
+                f32x2 acc0 = 0, acc1 = 0;
+                for_columns(s_col, n16, [&](int c0, uint32_t (&v)[16]) {
+                    capped(v);
+                    ulonglong2 o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = *reinterpret_cast<const ulonglong2 *>(nl + c0 + 4 * i);
+                    add_exp2(v, mul2, [&](int i) { return i & 1 ? o[i / 2].y : o[i / 2].x; }, acc0, acc1);
+                });
+                const float s = total(acc0, acc1);
+                // beyond any sum of 128 probabilities: a NaN or an infinity, which MUFU alone keeps
+                if (!__any_sync(0xffffffffu, !(s <= kSumLimit))) return s;
+            }
+            float s = 0.f;
             for_columns(s_col, n16, [&](int c0, uint32_t (&v)[16]) {
                 capped(v);
-                if (whole) {
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(nl + c0 + i);
-                        const f32x2 a = pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-                        const f32x2 b = pack2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-                        acc0 = add2(acc0, exp2_2(fma2(a, mul2, o.x)));
-                        acc1 = add2(acc1, exp2_2(fma2(b, mul2, o.y)));
-                    }
-                } else {
-                    float s = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float y = fast_exp2f(fmaf(__uint_as_float(v[i]), mul, nl[c0 + i]));
-                        if (c0 + i >= lo && c0 + i < hi) s += y;
-                    }
-                    acc0 = add2(acc0, pack2(s, 0.f));
+                for (int i = 0; i < 16; ++i) {
+                    const float y = fast_exp2f(fmaf(__uint_as_float(v[i]), mul, nl[c0 + i]));
+                    if (c0 + i >= lo && c0 + i < hi) s += y;
                 }
             });
-            return total(acc0, acc1);
+            return s;
         };
         // Columns [lo, hi) of row tile t whose rows see key `key` (rows see contiguous keys, in order,
         // so a key is seen by contiguous rows).
@@ -363,14 +460,13 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
             hi = static_cast<int>(min(max(last, 0ll), static_cast<long long>(used))) * p.group;
         };
 
-        int g0 = 0, items = 0;   // streaming tiles before this item; items with tiles before it
-        for (long long k = blockIdx.x; k < p.items; k += gridDim.x) {
-            const WItem it = item_geometry<HD, MODE>(p, k);
-            const int n = it.n;
-            const long long unit = static_cast<long long>(it.b) * p.n_kv_heads + it.kvh;
+        int g0 = 0, steps = 0;   // streaming tiles and staying steps before this one
+        for (; run_step<HD, MODE>(p, w); run_next(w), ++steps) {
+            const int n = w.n;
+            const long long unit = w.unit;
             const int first = (wg / NX - g0 % kStep + kStep) % kStep;
-            if constexpr (MODE == kStats) {
-                const int rt = it.x * NX + stay;
+            if constexpr (kRows) {
+                const int rt = w.x * NX + stay;
                 const int i = rt * p.qp + r / p.group;
                 const bool valid = r < p.qp * p.group && i < p.seq_q;
                 int lo = 0, hi = 0;
@@ -378,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                 float m = -INFINITY, l = 0.f;
                 for (int t = first; t < n; t += kStep) {
                     if (ok) ok = mbar_wait_warp(d_full, ((g0 + t) / kStep) & 1, p.err, kErrWaitMma);
-                    const int key0 = (it.t0 + t) * kTile;
+                    const int key0 = (w.t0 + t) * kTile;
                     // a warp none of whose rows sees a key of the tile skips it
                     if (ok && __any_sync(0xffffffffu, valid && key0 < hi && key0 + kTile > lo)) {
                         tc_fence_after();
@@ -407,19 +503,24 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                             }
                             const float negm = m != -INFINITY ? -m : 0.f;
                             const f32x2 neg2 = pack2(negm, negm);
-                            f32x2 acc0 = 0, acc1 = 0;
-                            for_columns(s_col, kTile / 16, [&](int c0, uint32_t (&v)[16]) {
-                                capped(v);
-                                if (!whole) hide(c0, v, lo - key0, hi - key0);
+                            if (whole && pass == 0) {
+                                f32x2 acc0 = 0, acc1 = 0;
+                                for_columns(s_col, kTile / 16, [&](int c0, uint32_t (&v)[16]) {
+                                    capped(v);
+                                    add_exp2(v, mul2, [&](int) { return neg2; }, acc0, acc1);
+                                });
+                                lt = total(acc0, acc1);
+                            } else {   // the border of the mask; scores that passed the limit, NaN among them
+                                float acc[2] = {0.f, 0.f};
+                                for_columns(s_col, kTile / 16, [&](int c0, uint32_t (&v)[16]) {
+                                    capped(v);
+                                    if (!whole) hide(c0, v, lo - key0, hi - key0);
 #pragma unroll
-                                for (int c = 0; c < 16; c += 4) {
-                                    const f32x2 a = pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-                                    const f32x2 b = pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
-                                    acc0 = add2(acc0, exp2_2(fma2(a, mul2, neg2)));
-                                    acc1 = add2(acc1, exp2_2(fma2(b, mul2, neg2)));
-                                }
-                            });
-                            lt = total(acc0, acc1);
+                                    for (int c = 0; c < 16; ++c)
+                                        acc[c & 1] += fast_exp2f(fmaf(__uint_as_float(v[c]), mul, negm));
+                                });
+                                lt = acc[0] + acc[1];
+                            }
                             need = __any_sync(0xffffffffu, !(lt <= kSumLimit));
                             if (!need) break;
                         }
@@ -429,14 +530,14 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                     mbar_arrive(d_empty);
                 }
                 if (valid)
-                    p.stat_parts[((unit * rows + static_cast<long long>(rt) * p.qp * p.group + r) * p.parts + it.part) *
-                                     kPieces<HD> + wg / NX] = ok ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+                    p.stat_parts[(unit * rows + static_cast<long long>(rt) * p.qp * p.group + r) * p.pieces +
+                                 w.piece * S::kWays + wg / NX] = ok ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
             } else {
                 const int used = kOne ? (min(p.qp, p.seq_q) * p.group + 15) / 16 : kTile / 16;
                 float sum = 0.f;
                 for (int t = first; t < n; t += kStep) {
                     // this thread's key, and the row tile
-                    const int key = (kOne ? it.t0 + t : it.x * NX + stay) * kTile + r, rt = kOne ? 0 : it.t0 + t;
+                    const int key = (kOne ? w.t0 + t : w.x * NX + stay) * kTile + r, rt = kOne ? 0 : w.t0 + t;
                     const long long at = unit * p.weights_stride + key;
                     const float before = kOne && p.weights_in && key < p.seq_k ? p.weights_in[at] : 0.f;
                     int lo, hi;
@@ -448,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                     if (ok && __any_sync(0xffffffffu, hi > lo && key < p.seq_k)) {
                         tc_fence_after();
                         const float *nl = reinterpret_cast<const float *>(smem + S::kOffLse) +
-                                          (kOne ? items : g0 + t) % kLseRing * kTile;
+                                          (kOne ? steps : g0 + t) % kLseRing * kTile;
                         one = tile_sum(nl, used, whole, lo, hi);
                         tc_fence_before();
                     }
@@ -457,14 +558,13 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                     else if (key < p.seq_k) p.weights_out[at] = before + one;
                 }
                 if (!kOne) {
-                    const int key = (it.x * NX + stay) * kTile + r;
+                    const int key = (w.x * NX + stay) * kTile + r;
                     if (key < p.seq_k)
-                        p.sum_parts[(static_cast<long long>(it.part * kPieces<HD> + wg / NX) * p.batch * p.n_kv_heads +
+                        p.sum_parts[(static_cast<long long>(w.piece * S::kWays + wg / NX) * p.batch * p.n_kv_heads +
                                      unit) * p.seq_k + key] = sum;
                 }
             }
             g0 += n;
-            items += n > 0;
         }
     }
     tc_fence_before();
@@ -475,57 +575,59 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     }
 }
 
-// -lse of every row from its parts, `width` (a power of two up to 32) lanes to a row, in the
-// layout of the row tiles: 128 entries each, -inf where no row is.
-__global__ void __launch_bounds__(256) weights_lse_kernel(float *nlse, const float2 *parts, long long entries, int n_parts,
-                                                          int width, int row_tiles, int tile_rows, int rows)
+// -lse of the rows of a row tile from their pieces, `width` (a power of two, 2 to 32) lanes to
+// a row and 256 / width rows to a block: 128 entries a tile, -inf where no row is.
+__global__ void __launch_bounds__(256) weights_lse_kernel(const __grid_constant__ WParams p, int mode, int kstay, int width)
 {
     griddep_wait();
     griddep_trigger();
-    const long long t = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    const long long e = t / width;
-    const int lane = static_cast<int>(t % width);
-    const int in_tile = static_cast<int>(e % kTile);
-    const long long tile = e / kTile;
-    const long long row = tile % row_tiles * tile_rows + in_tile;   // within the (batch, KV head)
-    const bool valid = e < entries && in_tile < tile_rows && row < rows;
-    const float2 *src = parts + (tile / row_tiles * rows + row) * n_parts;
+    const int blocks = kTile * width / 256;   // of a tile
+    const int unit = blockIdx.y, tile = blockIdx.x / blocks;
+    const int n = step_pieces(p, mode, kstay, unit, tile / kstay) * (4 / kstay);
+    const int lane = threadIdx.x % width, in_tile = blockIdx.x % blocks * (256 / width) + threadIdx.x / width;
+    const long long rows = static_cast<long long>(p.seq_q) * p.group;
+    const long long row = static_cast<long long>(tile) * p.qp * p.group + in_tile;
+    const bool valid = in_tile < p.qp * p.group && row < rows;
+    const float2 *src = p.stat_parts + (unit * rows + row) * p.pieces;
     float M = -INFINITY, L = 0.f;
     if (valid)
-        for (int c = lane; c < n_parts; c += width) M = fmaxf(M, src[c].x);
+        for (int c = lane; c < n; c += width) M = fmaxf(M, src[c].x);
     for (int o = width / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     if (valid)
-        for (int c = lane; c < n_parts; c += width) {
+        for (int c = lane; c < n; c += width) {
             const float2 v = src[c];
             if (v.x != -INFINITY) L += v.y * fast_exp2f(v.x - M);
         }
     for (int o = width / 2; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    if (e < entries && lane == 0) nlse[e] = M == -INFINITY ? -INFINITY : -(M + log2f(L));
+    if (lane == 0)
+        p.nlse[(static_cast<long long>(unit) * p.row_tiles + tile) * kTile + in_tile] =
+            M == -INFINITY ? -INFINITY : -(M + log2f(L));
 }
 
-// weights_out = weights_in + the parts, in order (no parts: a copy).
-__global__ void __launch_bounds__(256) weights_add_kernel(float *out, const float *in, long long stride,
-                                                          const float *parts, int n_parts, int seq_k, int n_kv_heads)
+// weights_out = weights_in + the pieces of each key tile, in order (kstay 0: a copy).
+__global__ void __launch_bounds__(kTile) weights_add_kernel(const __grid_constant__ WParams p, int kstay)
 {
     griddep_wait();
     griddep_trigger();
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    if (j >= seq_k) return;
-    const long long unit = static_cast<long long>(blockIdx.z) * n_kv_heads + blockIdx.y;
-    const long long units = static_cast<long long>(gridDim.z) * n_kv_heads;
+    const int unit = blockIdx.y;
+    const int j = blockIdx.x * kTile + threadIdx.x;
+    const int n = kstay > 0 ? step_pieces(p, kSums, kstay, unit, blockIdx.x / kstay) * (4 / kstay) : 0;
+    if (j >= p.seq_k) return;
+    const long long units = static_cast<long long>(p.batch) * p.n_kv_heads;
     float s = 0.f;
 #pragma unroll 4
-    for (int c = 0; c < n_parts; ++c) s += parts[(c * units + unit) * seq_k + j];
-    out[unit * stride + j] = (in ? in[unit * stride + j] : 0.f) + s;
+    for (int c = 0; c < n; ++c) s += p.sum_parts[(c * units + unit) * p.seq_k + j];
+    const long long at = unit * p.weights_stride + j;
+    p.weights_out[at] = (p.weights_in ? p.weights_in[at] : 0.f) + s;
 }
 
-// How the two passes are cut: parts of at most kMaxTiles streaming tiles, shorter ones where
-// the items would not fill the GPU, but then no more of them than SMs.
+// Sizes that do not depend on the mask.  A run is no shorter than a `most`-th of the streaming
+// tiles, so a staying step lies in at most most + 1 runs.
 struct WPlan {
     int qp, row_tiles, key_tiles;
-    int stat_stay, sum_stay;   // staying tiles per unit, in items
-    int stat_tiles, stat_parts, sum_tiles, sum_parts, pieces;
-    size_t lse, sums, total;   // the stats parts at 0
+    int stat_kstay, stat_stay, stat_most, sum_kstay, sum_stay, sum_most;
+    int stat_pieces, sum_pieces;
+    size_t lse, sums, total;   // the stats pieces at 0
 };
 
 WPlan weights_plan(int batch, int seq_q, int seq_k, int n_heads, int n_kv_heads, int head_dim)
@@ -533,30 +635,29 @@ WPlan weights_plan(int batch, int seq_q, int seq_k, int n_heads, int n_kv_heads,
     WPlan w;
     const int group = n_heads / n_kv_heads;
     const long long units = static_cast<long long>(batch) * n_kv_heads;
-    const int two = head_dim > 128 ? 1 : 2;
-    w.pieces = head_dim > 128 ? kPieces<256> : kPieces<128>;
     auto up = [](long long a, long long b) { return static_cast<int>((a + b - 1) / b); };
     auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
     w.qp = kTile / group;
     w.row_tiles = up(seq_q, w.qp);
     w.key_tiles = up(seq_k, kTile);
-    // for `stay` items per unit and `stream` tiles that stream
-    auto cut = [&](long long stay, int stream, int &tiles, int &parts) {
-        long long n = units * stay > 0 ? 148 / (units * stay) : 1;
-        const int least = up(stream, kMaxTiles);
-        if (n < least) n = least;
-        if (n > stream) n = stream;
-        tiles = n > 0 ? up(stream, n) : 1;
-        parts = up(stream, tiles);
+    const bool one = w.row_tiles <= 1;
+    const int two = head_dim > 128 ? 1 : 2;
+    auto most = [&](long long stay, int stream) {
+        const long long n = units * stay > 0 ? up(148, units * stay) : 1;
+        return static_cast<int>(n < 8 ? (stream < 8 ? stream : 8) : (n < stream ? n : stream));
     };
-    w.stat_stay = up(w.row_tiles, two);
-    cut(w.stat_stay, w.key_tiles, w.stat_tiles, w.stat_parts);
-    w.sum_stay = w.row_tiles == 1 ? 1 : up(w.key_tiles, two);
-    cut(w.sum_stay, w.row_tiles == 1 ? w.key_tiles : w.row_tiles, w.sum_tiles, w.sum_parts);
+    w.stat_kstay = one ? 1 : two;
+    w.stat_stay = up(w.row_tiles, w.stat_kstay);
+    w.stat_most = most(w.stat_stay, w.key_tiles);
+    w.stat_pieces = (w.stat_most + 1) * (4 / w.stat_kstay);
+    w.sum_kstay = one ? 1 : two;
+    w.sum_stay = one ? 1 : up(w.key_tiles, two);
+    w.sum_most = one ? up(148, units) : most(w.sum_stay, w.row_tiles);
+    w.sum_pieces = one ? 0 : (w.sum_most + 1) * (4 / w.sum_kstay);
     const size_t rows = static_cast<size_t>(units) * seq_q * group;
-    w.lse = al(rows * w.stat_parts * w.pieces * 8);
+    w.lse = al(rows * w.stat_pieces * 8);
     w.sums = w.lse + al(static_cast<size_t>(units) * w.row_tiles * kTile * 4);
-    w.total = w.sums + (w.row_tiles > 1 ? al(static_cast<size_t>(units) * seq_k * w.sum_parts * w.pieces * 4) : 0);
+    w.total = w.sums + al(static_cast<size_t>(units) * seq_k * w.sum_pieces * 4);
     return w;
 }
 
@@ -575,8 +676,9 @@ int sm_count()
     return cached[dev];
 }
 
+// Completes p for one pass (the runs, from the mask) and launches it.
 template <int HD, int MODE>
-int launch_pass(cudaStream_t st, WParams p, int stay, int tiles, int parts)
+int launch_pass(cudaStream_t st, WParams &p, int stay, int stream, int most, int pieces)
 {
     using S = WShape<HD, MODE>;
     static std::mutex mu;
@@ -598,32 +700,49 @@ int launch_pass(cudaStream_t st, WParams p, int stay, int tiles, int parts)
         }
     }
     p.stay = stay;
-    p.tiles = tiles;
-    p.parts = parts;
-    p.items = static_cast<long long>(stay) * parts * p.batch * p.n_kv_heads;
+    p.pieces = pieces;
+    p.unit_tiles = 0;
+    for (int x = 0; x < stay; ++x) {
+        int t0, t1;
+        stream_range(p, MODE, S::kStay, x, t0, t1);
+        p.unit_tiles += t1 - t0;
+    }
+    const long long all = p.unit_tiles * p.batch * p.n_kv_heads;
     const int sms = sm_count();
     if (sms <= 0) return SMOL_B200_ERR_CUDA;
-    const dim3 grid(static_cast<unsigned>(p.items < sms ? p.items : sms));
+    p.run = (all + sms - 1) / sms;
+    const long long least = (stream + most - 1) / (most > 0 ? most : 1);
+    if (p.run < least) p.run = least;
+    if (p.run < 1) p.run = 1;
+    if (all == 0) return SMOL_B200_OK;   // no row sees a key
+    const dim3 grid(static_cast<unsigned>((all + p.run - 1) / p.run));
     return launch_kernel(weights_kernel<HD, MODE>, grid, dim3(kThreads), S::kSmemBytes, st, p) == cudaSuccess
                ? SMOL_B200_OK
                : SMOL_B200_ERR_CUDA;
 }
 
 template <int HD>
-int launch_weights(cudaStream_t st, const WParams &p, const WPlan &w)
+int launch_weights(cudaStream_t st, WParams &p, const WPlan &w)
 {
-    const int rc = launch_pass<HD, kStats>(st, p, w.stat_stay, w.stat_tiles, w.stat_parts);
+    const unsigned units = static_cast<unsigned>(p.batch) * p.n_kv_heads;
+    const bool one = w.row_tiles == 1;
+    int rc = one ? launch_pass<HD, kStatsOneRowTile>(st, p, w.stat_stay, w.key_tiles, w.stat_most, w.stat_pieces)
+                 : launch_pass<HD, kStats>(st, p, w.stat_stay, w.key_tiles, w.stat_most, w.stat_pieces);
     if (rc != SMOL_B200_OK) return rc;
-    const int pieces = w.stat_parts * w.pieces;
-    int width = 1;
-    while (width < 32 && width < pieces) width *= 2;
-    const long long entries = static_cast<long long>(p.batch) * p.n_kv_heads * p.row_tiles * kTile;
-    if (launch_kernel(weights_lse_kernel, dim3(static_cast<unsigned>((entries * width + 255) / 256)), dim3(256), 0, st,
-                      p.nlse, static_cast<const float2 *>(p.stat_parts), entries, pieces, width, p.row_tiles,
-                      p.qp * p.group, p.seq_q * p.group) != cudaSuccess)
+    // about four pieces a lane: a step lies in at most key_tiles / run + 2 runs
+    long long pieces = (w.key_tiles / p.run + 2) * (4 / w.stat_kstay);
+    if (pieces > w.stat_pieces) pieces = w.stat_pieces;
+    int width = 2;
+    while (width < 32 && width * 4 < pieces) width *= 2;
+    if (launch_kernel(weights_lse_kernel, dim3(static_cast<unsigned>(w.row_tiles) * (kTile * width / 256), units),
+                      dim3(256), 0, st, p, one ? kStatsOneRowTile : kStats, w.stat_kstay, width) != cudaSuccess)
         return SMOL_B200_ERR_CUDA;
-    if (w.row_tiles == 1) return launch_pass<HD, kSumsOneRowTile>(st, p, 1, w.sum_tiles, w.sum_parts);
-    return launch_pass<HD, kSums>(st, p, w.sum_stay, w.sum_tiles, w.sum_parts);
+    if (one) return launch_pass<HD, kSumsOneRowTile>(st, p, 1, w.key_tiles, w.sum_most, 0);
+    rc = launch_pass<HD, kSums>(st, p, w.sum_stay, w.row_tiles, w.sum_most, w.sum_pieces);
+    if (rc != SMOL_B200_OK) return rc;
+    return launch_kernel(weights_add_kernel, dim3(w.key_tiles, units), dim3(kTile), 0, st, p, w.sum_kstay) == cudaSuccess
+               ? SMOL_B200_OK
+               : SMOL_B200_ERR_CUDA;
 }
 
 }  // namespace
@@ -661,13 +780,9 @@ int prefill_attention_weights(cudaStream_t st, const float *weights_in, float *w
     const WPlan w = weights_plan(batch, seq_q, seq_k, n_heads, n_kv_heads, head_dim);
     if (!workspace || workspace_bytes < w.total || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return SMOL_B200_ERR_WORKSPACE;
-    if (static_cast<long long>(w.row_tiles) * w.stat_parts > 0x7fffffffLL ||
-        static_cast<long long>(w.key_tiles) * w.sum_parts > 0x7fffffffLL ||
-        static_cast<long long>(batch) * n_kv_heads > 0x7fffffffLL ||
-        static_cast<long long>(seq_q) * (n_heads / n_kv_heads) > 0x7fffffffLL ||
-        static_cast<long long>(batch) * n_kv_heads * w.row_tiles * kTile > 0x7fffffffLL)
-        return SMOL_B200_ERR_ARGS;   // grid sizes and item numbers
-
+    if (static_cast<long long>(seq_q) * (n_heads / n_kv_heads) > 0x7fffffffLL ||
+        static_cast<long long>(batch) * n_kv_heads > 65535)
+        return SMOL_B200_ERR_ARGS;   // row numbers, the grids of the joining kernels
     WParams p;
     memset(&p, 0, sizeof(p));
     p.group = n_heads / n_kv_heads;
@@ -684,7 +799,6 @@ int prefill_attention_weights(cudaStream_t st, const float *weights_in, float *w
     p.nlse = reinterpret_cast<float *>(base + w.lse);
     p.sum_parts = reinterpret_cast<float *>(base + w.sums);
     PdlScope pdl(g_api_pdl);
-    const bool joined = w.row_tiles > 1;
     if (seq_q > 0) {
         const int kernel_hd = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
         const int64_t qb = batch > 1 ? q_batch_stride : static_cast<int64_t>(seq_q) * q_row_stride;
@@ -711,13 +825,9 @@ int prefill_attention_weights(cudaStream_t st, const float *weights_in, float *w
                                           : launch_weights<256>(st, p, w);
         if (rc != SMOL_B200_OK) return rc;
     }
-    if (seq_q == 0 || joined) {
-        if (launch_kernel(weights_add_kernel, dim3((seq_k + 255) / 256, n_kv_heads, batch), dim3(256), 0, st,
-                          weights_out, weights_in, static_cast<long long>(weights_stride),
-                          static_cast<const float *>(p.sum_parts), seq_q == 0 ? 0 : w.sum_parts * w.pieces, seq_k,
-                          n_kv_heads) != cudaSuccess)
-            return SMOL_B200_ERR_CUDA;
-    }
+    if (seq_q == 0 && launch_kernel(weights_add_kernel, dim3(w.key_tiles, batch * n_kv_heads), dim3(kTile), 0, st, p, 0) !=
+                          cudaSuccess)
+        return SMOL_B200_ERR_CUDA;
     return SMOL_B200_OK;
 }
 
