@@ -46,14 +46,20 @@ struct WShape {
     static constexpr int kSubBytes = kTile * 128;
     static constexpr int kTileBytes = kSub * kSubBytes;
     static constexpr int kStay = HD == 256 || MODE >= kStatsOneRowTile ? 1 : 2;   // tiles that stay
-    // a staying tile's streaming tiles go to kWays warpgroups in turn: as many results per run
+    // A staying tile's streaming tiles go to kWays warpgroups in turn.  Four meet in shared
+    // memory at the end of a step, two leave a result each.
     static constexpr int kWays = 4 / kStay;
+    static constexpr bool kMeet = kWays == 4 && MODE != kSumsOneRowTile;
+    static constexpr int kResults = kMeet ? 1 : kWays;
     static constexpr int kXBytes = kStay * kTileBytes;
-    static constexpr int kXStages = HD == 64 ? 2 : 1;
-    static constexpr int kStages = HD == 256 ? 2 : 4;
+    // the next staying tiles load ahead where there is room (stats need no lse beside them)
+    static constexpr int kXStages = HD == 64 || (HD == 128 && MODE != kSums) ? 2 : 1;
+    static constexpr int kStages = HD == 256 ? 2 : HD == 128 && MODE == kStats ? 3 : 4;
+    static constexpr int kRing = MODE == kSums || MODE == kSumsOneRowTile ? kLseRing : 0;
     static constexpr int kOffY = kXStages * kXBytes;
     static constexpr int kOffLse = kOffY + kStages * kTileBytes;
-    static constexpr int kOffBar = kOffLse + kLseRing * kTile * 4;
+    static constexpr int kOffMeet = kOffLse + kRing * kTile * 4;   // [step parity][warpgroup][128]
+    static constexpr int kOffBar = kOffMeet + (kMeet ? 2 * kGroups * kTile * 8 : 0);
     static constexpr int kUsed = kOffBar + 256 + 1024;
     static_assert(kUsed <= 227 * 1024, "shared memory");
     // one CTA per SM: each allocates all 512 TMEM columns
@@ -72,7 +78,9 @@ struct WParams {
     int batch, seq_q, seq_k, n_kv_heads, group, qp;   // qp: queries of a row tile
     int row_tiles, key_tiles;
     int stay, pieces;               // staying steps per unit; slots of partial results
-    long long unit_tiles, run;      // visible streaming tiles of a unit, of a CTA
+    long long unit_tiles, run;      // visible streaming tiles (and step costs) of a unit, of a CTA
+    long long stat_unit_tiles, stat_run;   // those of the stats pass, for the sums of one row tile
+    int stat_pieces;
     int mask_kind, q_offset, prefix_len, window;
     int q_bytes;                    // bytes of a row tile's boxes (all sub-tiles)
     float scale, softcap;
@@ -151,13 +159,25 @@ __device__ __forceinline__ void add_exp2(const uint32_t (&v)[16], f32x2 mul2, Of
     }
 }
 
+// Changing the staying tiles costs about as much as kStepCost streaming tiles (1.7 us against
+// 1.45 us a tile, head dim 128), so a step counts that many more, in front of its own, when
+// the runs are cut.
+constexpr int kStepCost = 1;
+
 // One CTA's run, staying step by staying step: step x of unit (b, kvh) against streaming tiles
 // [t0, t0 + n), as piece `piece` of that step.
 struct WRun {
     int unit, x, t0, n, piece;
-    int skip;             // tiles of step x before the run
-    long long left;       // tiles of the run from step x on
+    long long skip;       // of step x's cost and tiles, what lies before the run
+    long long left;       // cost and tiles of the run from there on
 };
+
+__device__ __forceinline__ void run_next(WRun &w)
+{
+    ++w.x;
+    w.skip = 0;
+    w.piece = 0;
+}
 
 template <int HD, int MODE>
 __device__ __forceinline__ bool run_step(const WParams &p, WRun &w)
@@ -169,21 +189,16 @@ __device__ __forceinline__ bool run_step(const WParams &p, WRun &w)
         }
         int t0, t1;
         stream_range(p, MODE, WShape<HD, MODE>::kStay, w.x, t0, t1);
-        w.t0 = t0 + w.skip;
-        w.n = static_cast<int>(min(static_cast<long long>(t1 - w.t0), w.left));
+        const long long size = t1 > t0 ? t1 - t0 + kStepCost : 0;
+        const long long end = min(size, w.skip + w.left);   // the run's share of the step: [skip, end)
+        const int first = static_cast<int>(max(w.skip - kStepCost, 0ll));
+        w.t0 = t0 + first;
+        w.n = static_cast<int>(max(end - kStepCost, 0ll)) - first;
+        w.left -= end - w.skip;
         if (w.n > 0) return true;
-        ++w.x;
-        w.skip = 0;
-        w.piece = 0;
+        run_next(w);
     }
     return false;
-}
-__device__ __forceinline__ void run_next(WRun &w)
-{
-    w.left -= w.n;
-    ++w.x;
-    w.skip = 0;
-    w.piece = 0;
 }
 
 // The run of CTA `cta`, found by one warp: tile number cta * run, then the staying step that
@@ -203,7 +218,7 @@ __device__ WRun find_run(const WParams &p, int cta)
     for (int x0 = 0; x0 < p.stay; x0 += 32) {
         int t0 = 0, t1 = 0;
         if (x0 + lane < p.stay) stream_range(p, MODE, WShape<HD, MODE>::kStay, x0 + lane, t0, t1);
-        const int mine = t1 - t0;
+        const int mine = t1 > t0 ? t1 - t0 + kStepCost : 0;
         int sum = mine;   // inclusive within the warp
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -216,8 +231,8 @@ __device__ WRun find_run(const WParams &p, int cta)
             const int l = __ffs(hit) - 1;
             const long long f = __shfl_sync(0xffffffffu, first, l);
             w.x = x0 + l;
-            w.skip = static_cast<int>(in_unit - f);
-            w.piece = cta - static_cast<int>((w.unit * p.unit_tiles + f) / p.run);
+            w.skip = in_unit - f;
+            w.piece = cta - static_cast<int>((w.unit * p.unit_tiles + f + kStepCost) / p.run);
             return w;
         }
         before += __shfl_sync(0xffffffffu, sum, 31);
@@ -226,8 +241,13 @@ __device__ WRun find_run(const WParams &p, int cta)
     return w;
 }
 
-// Pieces of staying step x of `unit` (the whole block asks for one step): the runs that its
-// tiles lie in.
+// Runs of length `run` that tiles [first, first + n) lie in.
+__device__ __forceinline__ int pieces_at(long long first, int n, long long run)
+{
+    return n > 0 ? static_cast<int>((first + n - 1) / run - first / run) + 1 : 0;
+}
+
+// Pieces of staying step x of `unit` (the whole block asks for one step).
 __device__ int step_pieces(const WParams &p, int mode, int kstay, int unit, int x)
 {
     __shared__ long long s_sum[32];
@@ -235,17 +255,17 @@ __device__ int step_pieces(const WParams &p, int mode, int kstay, int unit, int 
     for (int i = threadIdx.x; i < x; i += blockDim.x) {
         int t0, t1;
         stream_range(p, mode, kstay, i, t0, t1);
-        sum += t1 - t0;
+        if (t1 > t0) sum += t1 - t0 + kStepCost;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (threadIdx.x % 32 == 0) s_sum[threadIdx.x / 32] = sum;
     __syncthreads();
-    long long f = unit * p.unit_tiles;
+    long long f = unit * p.unit_tiles + kStepCost;
     for (int i = 0; i < static_cast<int>(blockDim.x / 32); ++i) f += s_sum[i];
     int t0, t1;
     stream_range(p, mode, kstay, x, t0, t1);
-    return t1 > t0 ? static_cast<int>((f + t1 - t0 - 1) / p.run - f / p.run) + 1 : 0;
+    return pieces_at(f, t1 - t0, p.run);
 }
 
 __device__ __forceinline__ const float *lse_of(const WParams &p, int unit, int row_tile)
@@ -268,8 +288,6 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     constexpr int ST = S::kStages, XS = S::kXStages, NX = S::kStay;
     constexpr int kProducer = kGroups * 4, kIssuer = kProducer + 1;
     constexpr bool kOne = MODE == kSumsOneRowTile, kRows = MODE == kStats || MODE == kStatsOneRowTile;
-    griddep_wait();
-    griddep_trigger();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -306,6 +324,9 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     tc_fence_after();
     const uint32_t tmem = bars->tmem_base;
     WRun w = find_run<HD, MODE>(p, blockIdx.x);
+    // everything above is the kernel's own: it may run while the kernels before this one finish
+    griddep_wait();
+    griddep_trigger();
 
     if (warp == kProducer) {
         // ================= TMA producer =================
@@ -328,8 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                 if (nx >= XS && !(ok = mbar_wait(smem_u32(&bars->x_empty[xs]), (nx / XS - 1) & 1, p.err, kErrWaitTmaEmpty)))
                     break;
                 const uint32_t xb = smem_u32(&bars->x_full[xs]);
-                mbar_arrive_expect_tx(xb, NX * (MODE == kSums ? S::kTileBytes : p.q_bytes) + (kOne ? kTile * 4 : 0));
-                if (kOne) bulk_load(smem_u32(smem + S::kOffLse) + nx % kLseRing * kTile * 4, lse_of(p, w.unit, 0), kTile * 4, xb);
+                mbar_arrive_expect_tx(xb, NX * (MODE == kSums ? S::kTileBytes : p.q_bytes));
 #pragma unroll
                 for (int i = 0; i < NX; ++i)
                     load(smem_u32(smem + xs * S::kXBytes + i * S::kTileBytes), xb, MODE != kSums, w.x * NX + i);
@@ -460,7 +480,8 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
             hi = static_cast<int>(min(max(last, 0ll), static_cast<long long>(used))) * p.group;
         };
 
-        int g0 = 0, steps = 0;   // streaming tiles and staying steps before this one
+        int g0 = 0, steps = 0;             // streaming tiles and staying steps before this one
+        int one_unit = -1, one_slot = 0;   // one row tile: the unit whose lse are in shared memory, and where
         for (; run_step<HD, MODE>(p, w); run_next(w), ++steps) {
             const int n = w.n;
             const long long unit = w.unit;
@@ -529,11 +550,50 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                     }
                     mbar_arrive(d_empty);
                 }
-                if (valid)
+                if (!ok) m = -INFINITY, l = 0.f;
+                if (S::kMeet) {
+                    float2 *box = reinterpret_cast<float2 *>(smem + S::kOffMeet) + (steps & 1) * kGroups * kTile;
+                    box[wg * kTile + r] = make_float2(m, l);
+                    named_bar_sync(1, kExpThreads);
+                    if (wg == 0) {
+                        for (int i = 1; i < kGroups; ++i) m = fmaxf(m, box[i * kTile + r].x);
+                        l = 0.f;
+                        for (int i = 0; i < kGroups; ++i) {
+                            const float2 v = box[i * kTile + r];
+                            if (v.x != -INFINITY) l += v.y * fast_exp2f(v.x - m);
+                        }
+                    }
+                }
+                if (valid && (!S::kMeet || wg == 0))
                     p.stat_parts[(unit * rows + static_cast<long long>(rt) * p.qp * p.group + r) * p.pieces +
-                                 w.piece * S::kWays + wg / NX] = ok ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+                                 w.piece * S::kResults + (S::kMeet ? 0 : wg / NX)] = make_float2(m, l);
             } else {
                 const int used = kOne ? (min(p.qp, p.seq_q) * p.group + 15) / 16 : kTile / 16;
+                float *ring = reinterpret_cast<float *>(smem + S::kOffLse);
+                if (kOne && one_unit != w.unit) {
+                    // the rows' -lse from their pieces, four lanes to a row
+                    one_unit = w.unit;
+                    one_slot ^= 1;
+                    int t0, t1;
+                    stream_range(p, kStatsOneRowTile, 1, 0, t0, t1);
+                    const int pieces = pieces_at(w.unit * p.stat_unit_tiles + kStepCost, t1 - t0, p.stat_run);
+                    const int row = threadIdx.x / 4, part = threadIdx.x % 4;
+                    const float2 *src = p.stat_parts + (unit * rows + row) * p.stat_pieces;
+                    float M = -INFINITY, L = 0.f;
+                    if (row < rows)
+                        for (int c = part; c < pieces; c += 4) M = fmaxf(M, src[c].x);
+                    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 1));
+                    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 2));
+                    if (row < rows)
+                        for (int c = part; c < pieces; c += 4) {
+                            const float2 v = src[c];
+                            if (v.x != -INFINITY) L += v.y * fast_exp2f(v.x - M);
+                        }
+                    L += __shfl_xor_sync(0xffffffffu, L, 1);
+                    L += __shfl_xor_sync(0xffffffffu, L, 2);
+                    if (part == 0) ring[one_slot * kTile + row] = M == -INFINITY ? -INFINITY : -(M + log2f(L));
+                    named_bar_sync(1, kExpThreads);   // the slot before is still read: two in turn
+                }
                 float sum = 0.f;
                 for (int t = first; t < n; t += kStep) {
                     // this thread's key, and the row tile
@@ -548,9 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                     float one = 0.f;
                     if (ok && __any_sync(0xffffffffu, hi > lo && key < p.seq_k)) {
                         tc_fence_after();
-                        const float *nl = reinterpret_cast<const float *>(smem + S::kOffLse) +
-                                          (kOne ? steps : g0 + t) % kLseRing * kTile;
-                        one = tile_sum(nl, used, whole, lo, hi);
+                        one = tile_sum(ring + (kOne ? one_slot : (g0 + t) % kLseRing) * kTile, used, whole, lo, hi);
                         tc_fence_before();
                     }
                     mbar_arrive(d_empty);
@@ -559,9 +617,15 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                 }
                 if (!kOne) {
                     const int key = (w.x * NX + stay) * kTile + r;
-                    if (key < p.seq_k)
-                        p.sum_parts[(static_cast<long long>(w.piece * S::kWays + wg / NX) * p.batch * p.n_kv_heads +
-                                     unit) * p.seq_k + key] = sum;
+                    if (S::kMeet) {
+                        float *box = reinterpret_cast<float *>(smem + S::kOffMeet) + (steps & 1) * kGroups * kTile;
+                        box[wg * kTile + r] = sum;
+                        named_bar_sync(1, kExpThreads);
+                        if (wg == 0) sum = (box[r] + box[kTile + r]) + (box[2 * kTile + r] + box[3 * kTile + r]);
+                    }
+                    if (key < p.seq_k && (!S::kMeet || wg == 0))
+                        p.sum_parts[(static_cast<long long>(w.piece * S::kResults + (S::kMeet ? 0 : wg / NX)) * p.batch *
+                                         p.n_kv_heads + unit) * p.seq_k + key] = sum;
                 }
             }
             g0 += n;
@@ -577,13 +641,13 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
 
 // -lse of the rows of a row tile from their pieces, `width` (a power of two, 2 to 32) lanes to
 // a row and 256 / width rows to a block: 128 entries a tile, -inf where no row is.
-__global__ void __launch_bounds__(256) weights_lse_kernel(const __grid_constant__ WParams p, int mode, int kstay, int width)
+__global__ void __launch_bounds__(256) weights_lse_kernel(const __grid_constant__ WParams p, int kstay, int results, int width)
 {
     griddep_wait();
     griddep_trigger();
     const int blocks = kTile * width / 256;   // of a tile
     const int unit = blockIdx.y, tile = blockIdx.x / blocks;
-    const int n = step_pieces(p, mode, kstay, unit, tile / kstay) * (4 / kstay);
+    const int n = step_pieces(p, kStats, kstay, unit, tile / kstay) * results;
     const int lane = threadIdx.x % width, in_tile = blockIdx.x % blocks * (256 / width) + threadIdx.x / width;
     const long long rows = static_cast<long long>(p.seq_q) * p.group;
     const long long row = static_cast<long long>(tile) * p.qp * p.group + in_tile;
@@ -605,13 +669,13 @@ __global__ void __launch_bounds__(256) weights_lse_kernel(const __grid_constant_
 }
 
 // weights_out = weights_in + the pieces of each key tile, in order (kstay 0: a copy).
-__global__ void __launch_bounds__(kTile) weights_add_kernel(const __grid_constant__ WParams p, int kstay)
+__global__ void __launch_bounds__(kTile) weights_add_kernel(const __grid_constant__ WParams p, int kstay, int results)
 {
     griddep_wait();
     griddep_trigger();
     const int unit = blockIdx.y;
     const int j = blockIdx.x * kTile + threadIdx.x;
-    const int n = kstay > 0 ? step_pieces(p, kSums, kstay, unit, blockIdx.x / kstay) * (4 / kstay) : 0;
+    const int n = kstay > 0 ? step_pieces(p, kSums, kstay, unit, blockIdx.x / kstay) * results : 0;
     if (j >= p.seq_k) return;
     const long long units = static_cast<long long>(p.batch) * p.n_kv_heads;
     float s = 0.f;
@@ -626,7 +690,7 @@ __global__ void __launch_bounds__(kTile) weights_add_kernel(const __grid_constan
 struct WPlan {
     int qp, row_tiles, key_tiles;
     int stat_kstay, stat_stay, stat_most, sum_kstay, sum_stay, sum_most;
-    int stat_pieces, sum_pieces;
+    int stat_pieces, sum_pieces, results;   // slots of a row / key; results of a piece (not one row tile)
     size_t lse, sums, total;   // the stats pieces at 0
 };
 
@@ -649,11 +713,12 @@ WPlan weights_plan(int batch, int seq_q, int seq_k, int n_heads, int n_kv_heads,
     w.stat_kstay = one ? 1 : two;
     w.stat_stay = up(w.row_tiles, w.stat_kstay);
     w.stat_most = most(w.stat_stay, w.key_tiles);
-    w.stat_pieces = (w.stat_most + 1) * (4 / w.stat_kstay);
+    w.results = two == 2 ? WShape<128, kStats>::kResults : WShape<256, kStats>::kResults;
+    w.stat_pieces = (w.stat_most + 1) * (one ? WShape<128, kStatsOneRowTile>::kResults : w.results);
     w.sum_kstay = one ? 1 : two;
     w.sum_stay = one ? 1 : up(w.key_tiles, two);
     w.sum_most = one ? up(148, units) : most(w.sum_stay, w.row_tiles);
-    w.sum_pieces = one ? 0 : (w.sum_most + 1) * (4 / w.sum_kstay);
+    w.sum_pieces = one ? 0 : (w.sum_most + 1) * w.results;
     const size_t rows = static_cast<size_t>(units) * seq_q * group;
     w.lse = al(rows * w.stat_pieces * 8);
     w.sums = w.lse + al(static_cast<size_t>(units) * w.row_tiles * kTile * 4);
@@ -705,7 +770,7 @@ int launch_pass(cudaStream_t st, WParams &p, int stay, int stream, int most, int
     for (int x = 0; x < stay; ++x) {
         int t0, t1;
         stream_range(p, MODE, S::kStay, x, t0, t1);
-        p.unit_tiles += t1 - t0;
+        if (t1 > t0) p.unit_tiles += t1 - t0 + kStepCost;
     }
     const long long all = p.unit_tiles * p.batch * p.n_kv_heads;
     const int sms = sm_count();
@@ -725,22 +790,28 @@ template <int HD>
 int launch_weights(cudaStream_t st, WParams &p, const WPlan &w)
 {
     const unsigned units = static_cast<unsigned>(p.batch) * p.n_kv_heads;
-    const bool one = w.row_tiles == 1;
-    int rc = one ? launch_pass<HD, kStatsOneRowTile>(st, p, w.stat_stay, w.key_tiles, w.stat_most, w.stat_pieces)
-                 : launch_pass<HD, kStats>(st, p, w.stat_stay, w.key_tiles, w.stat_most, w.stat_pieces);
+    if (w.row_tiles == 1) {
+        const int rc = launch_pass<HD, kStatsOneRowTile>(st, p, w.stat_stay, w.key_tiles, w.stat_most, w.stat_pieces);
+        if (rc != SMOL_B200_OK) return rc;
+        p.stat_unit_tiles = p.unit_tiles;
+        p.stat_run = p.run;
+        p.stat_pieces = w.stat_pieces;
+        return launch_pass<HD, kSumsOneRowTile>(st, p, 1, w.key_tiles, w.sum_most, 0);
+    }
+    int rc = launch_pass<HD, kStats>(st, p, w.stat_stay, w.key_tiles, w.stat_most, w.stat_pieces);
     if (rc != SMOL_B200_OK) return rc;
-    // about four pieces a lane: a step lies in at most key_tiles / run + 2 runs
-    long long pieces = (w.key_tiles / p.run + 2) * (4 / w.stat_kstay);
+    // about four results a lane: a step lies in at most key_tiles / run + 2 runs
+    long long pieces = (w.key_tiles / p.run + 2) * w.results;
     if (pieces > w.stat_pieces) pieces = w.stat_pieces;
     int width = 2;
     while (width < 32 && width * 4 < pieces) width *= 2;
     if (launch_kernel(weights_lse_kernel, dim3(static_cast<unsigned>(w.row_tiles) * (kTile * width / 256), units),
-                      dim3(256), 0, st, p, one ? kStatsOneRowTile : kStats, w.stat_kstay, width) != cudaSuccess)
+                      dim3(256), 0, st, p, w.stat_kstay, w.results, width) != cudaSuccess)
         return SMOL_B200_ERR_CUDA;
-    if (one) return launch_pass<HD, kSumsOneRowTile>(st, p, 1, w.key_tiles, w.sum_most, 0);
     rc = launch_pass<HD, kSums>(st, p, w.sum_stay, w.row_tiles, w.sum_most, w.sum_pieces);
     if (rc != SMOL_B200_OK) return rc;
-    return launch_kernel(weights_add_kernel, dim3(w.key_tiles, units), dim3(kTile), 0, st, p, w.sum_kstay) == cudaSuccess
+    return launch_kernel(weights_add_kernel, dim3(w.key_tiles, units), dim3(kTile), 0, st, p, w.sum_kstay, w.results) ==
+                   cudaSuccess
                ? SMOL_B200_OK
                : SMOL_B200_ERR_CUDA;
 }
@@ -825,8 +896,8 @@ int prefill_attention_weights(cudaStream_t st, const float *weights_in, float *w
                                           : launch_weights<256>(st, p, w);
         if (rc != SMOL_B200_OK) return rc;
     }
-    if (seq_q == 0 && launch_kernel(weights_add_kernel, dim3(w.key_tiles, batch * n_kv_heads), dim3(kTile), 0, st, p, 0) !=
-                          cudaSuccess)
+    if (seq_q == 0 && launch_kernel(weights_add_kernel, dim3(w.key_tiles, batch * n_kv_heads), dim3(kTile), 0, st, p, 0,
+                                    0) != cudaSuccess)
         return SMOL_B200_ERR_CUDA;
     return SMOL_B200_OK;
 }
