@@ -8,11 +8,14 @@
 // independent of one another and work in place, and no row is moved that need not be:
 // attention does not depend on the order of a head's rows.
 //
-// Select.  The B-th largest of the n 32-bit sort keys is found bit by bit, two bits a
-// round: keys stay in registers, a round counts those at or above three candidates.  Ties
-// at that key are taken in slot order.  One more ordered count gives holes and movers
-// their numbers.  A (sequence, KV head) is one CTA or, for long caches, one cluster whose
-// CTAs hold a segment of the slots each and exchange counts through shared memory.
+// Select.  The B-th largest of the n 32-bit sort keys is found by bracketing: keys stay in
+// registers, a round counts those at or above six candidates -- five around the rank
+// interpolated between the bracket's ends, one at its middle, so that it halves at worst.
+// It ends when exactly B keys lie at or above a candidate, or when one key value is left,
+// whose ties are taken in slot order.  One more ordered count gives holes and movers their
+// numbers.  (Two bits a round from the top took 16 rounds of 0.6 us, 1.2 us in a cluster.)
+// A (sequence, KV head) is one CTA or, for long caches, one cluster whose CTAs hold a
+// segment of the slots each and exchange counts through shared memory.
 //
 // Bytes: 8 per slot to read (weight, position), as many to write where the outputs are
 // other arrays, and K and V of the moved rows.
@@ -27,8 +30,8 @@ namespace {
 constexpr int kMaxThreads = 1024;
 constexpr int kMaxItems = 32;
 constexpr int kMaxCluster = 8;
-// Moves that the select kernel makes itself; with more possible a second kernel spreads them.
-constexpr int kFusedMoves = 64;
+// Moves whose slots are listed in shared memory; more go through the workspace.
+constexpr int kSmemMoves = 2048;
 
 struct EvictParams {
     uint16_t *k, *v;
@@ -43,11 +46,10 @@ struct EvictParams {
     int *kv_len_out;
     const int *seq_pos;
     int *lists;      // [n_seqs*n_kv_heads][2*cap]: holes, movers
-    int *counts;     // [n_seqs*n_kv_heads] moves
     int *lengths;    // [n_seqs] new lengths
     unsigned *err;
     int n_kv_heads, hd, max_kv_len, budget, sink, recent, cap;
-    int fused, write_len;   // this kernel makes the moves / writes kv_len_out
+    int smem_lists, write_len;   // lists in shared memory; this kernel writes kv_len_out
 };
 
 // Weight as an unsigned key of the same order: NaN lowest, -0 equal to 0.
@@ -65,21 +67,35 @@ __device__ __forceinline__ int slot_position(int recorded, int j, int n, int see
     return recorded >= 0 ? recorded : seen - n + j;
 }
 
-// Moves r = first, first + step, ... of (sequence b, head h), one per warp.
-__device__ __forceinline__ void move_rows(const EvictParams &p, long long row0, int h, const int *holes,
-                                          const int *movers, int m, int first, int step)
+// K and V of the moves of head h, 16 bytes a thread and four pieces in flight, by threads
+// first, first + step, ... of `step` (dst_src(r) gives the slots of move r).
+template <typename Slots>
+__device__ __forceinline__ void move_rows(const EvictParams &p, long long row0, int h, int m, int first, int step,
+                                          Slots &&dst_src)
 {
-    const int lane = threadIdx.x % 32;
     const int vecs = p.hd / 8;   // 16-byte pieces of one head's row
     const long long width = static_cast<long long>(p.n_kv_heads) * p.hd;
-    for (int r = first; r < m; r += step) {
-        const long long dst = (row0 + holes[r]) * width + static_cast<long long>(h) * p.hd;
-        const long long src = (row0 + movers[r]) * width + static_cast<long long>(h) * p.hd;
-        for (int i = lane; i < 2 * vecs; i += 32) {
-            uint16_t *pool = i < vecs ? p.k : p.v;
-            const int e = (i < vecs ? i : i - vecs) * 8;
-            *reinterpret_cast<uint4 *>(pool + dst + e) = *reinterpret_cast<const uint4 *>(pool + src + e);
+    const long long total = static_cast<long long>(m) * 2 * vecs;
+    constexpr int kLoad = 4;
+    for (long long i0 = first; i0 < total; i0 += static_cast<long long>(step) * kLoad) {
+        uint4 v[kLoad];
+        uint16_t *to[kLoad];
+#pragma unroll
+        for (int u = 0; u < kLoad; ++u) {
+            const long long i = i0 + static_cast<long long>(u) * step;
+            to[u] = nullptr;
+            if (i < total) {
+                const int r = static_cast<int>(i / (2 * vecs)), e = static_cast<int>(i - static_cast<long long>(r) * 2 * vecs);
+                uint16_t *pool = e < vecs ? p.k : p.v;
+                const long long col = static_cast<long long>(h) * p.hd + (e < vecs ? e : e - vecs) * 8;
+                const int2 ds = dst_src(r);
+                to[u] = pool + (row0 + ds.x) * width + col;
+                v[u] = *reinterpret_cast<const uint4 *>(pool + (row0 + ds.y) * width + col);
+            }
         }
+#pragma unroll
+        for (int u = 0; u < kLoad; ++u)
+            if (to[u]) *reinterpret_cast<uint4 *>(to[u]) = v[u];
     }
 }
 
@@ -88,10 +104,12 @@ __global__ void __launch_bounds__(kMaxThreads) evict_kernel(const __grid_constan
 {
     griddep_wait();
     griddep_trigger();
-    __shared__ int s_cnt[3][4];                          // counts of a round, three rounds in rotation
-    __shared__ int s_box[2][kMaxCluster][3];             // every CTA's counts, by round parity
-    __shared__ int s_scan[ITEMS * (kMaxThreads / 32)];   // flags per (item, warp), then their prefix
-    __shared__ int s_total, s_tot_box[kMaxCluster];
+    __shared__ uint32_t s_cnt[8][kMaxThreads / 32];      // every warp's results of a round
+    __shared__ uint32_t s_box[2][kMaxCluster][8];        // every CTA's, by round parity
+    __shared__ int s_scan[ITEMS][kMaxThreads / 32];      // flags per (item, warp), then those before within the item
+    __shared__ int s_item[ITEMS];                        // flags per item
+    __shared__ int s_tot_box[2][kMaxCluster];
+    __shared__ int s_holes[kSmemMoves], s_movers[kSmemMoves];
     const int C = static_cast<int>(gridDim.x), rank = blockIdx.x;
     const int h = blockIdx.y, b = blockIdx.z;
     const int T = blockDim.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32, W = T / 32;
@@ -111,7 +129,6 @@ __global__ void __launch_bounds__(kMaxThreads) evict_kernel(const __grid_constan
             p.lengths[b] = B;
             if (p.write_len) p.kv_len_out[b] = B;
         }
-        if (keep_all) p.counts[unit] = 0;
     }
     const float *w_in = p.weights_in + unit * p.stride;
     float *w_out = p.weights_out + unit * p.stride;
@@ -130,108 +147,170 @@ __global__ void __launch_bounds__(kMaxThreads) evict_kernel(const __grid_constan
         return;
     }
 
-    uint32_t key[ITEMS];
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const int j = j_first + i * T;
-        key[i] = 0u;
-        if (j < n) {
-            const int pos = slot_position(pos_in[j], j, n, seen);
-            key[i] = pos < p.sink || pos >= seen - p.recent ? 0xffffffffu : weight_key(w_in[j]);
-        }
-    }
-    if (tid < 12) s_cnt[tid / 4][tid % 4] = 0;
-    __syncthreads();
-
-    // t: the largest key with at least B keys at or above it, two bits a round
-    uint32_t t = 0;
-    int at_t = n, above = 0;   // keys >= t, keys >= the smallest rejected candidate above t
-    for (int round = 0; round < 16; ++round) {
-        const int shift = 30 - 2 * round;
-        const uint32_t c1 = t | (1u << shift), c2 = t | (2u << shift), c3 = t | (3u << shift);
-        int k1 = 0, k2 = 0, k3 = 0;
+    uint32_t key[ITEMS];   // 0 past the last slot: below every candidate
+    {
+        float w[ITEMS];
+        int q[ITEMS];
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            k1 += key[i] >= c1;
-            k2 += key[i] >= c2;
-            k3 += key[i] >= c3;
+            const int j = j_first + i * T;
+            w[i] = j < n ? w_in[j] : 0.f;
+            q[i] = j < n ? pos_in[j] : 0;
         }
-        k1 = __reduce_add_sync(0xffffffffu, k1);
-        k2 = __reduce_add_sync(0xffffffffu, k2);
-        k3 = __reduce_add_sync(0xffffffffu, k3);
-        int *cnt = s_cnt[round % 3];
-        if (lane < 3) atomicAdd(&cnt[lane], lane == 0 ? k1 : lane == 1 ? k2 : k3);
-        if (tid < 4) s_cnt[(round + 1) % 3][tid] = 0;   // last read two barriers ago
-        __syncthreads();
-        int n1 = cnt[0], n2 = cnt[1], n3 = cnt[2];
-        if (C > 1) {
-            if (tid < C * 3) {   // to every CTA of the cluster
-                const uint32_t dst = map_shared_rank(smem_u32(&s_box[round & 1][rank][tid % 3]), tid / 3);
-                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(cnt[tid % 3]) : "memory");
-            }
-            cluster_sync_all();
-            n1 = n2 = n3 = 0;
-            for (int r = 0; r < C; ++r) {
-                n1 += s_box[round & 1][r][0];
-                n2 += s_box[round & 1][r][1];
-                n3 += s_box[round & 1][r][2];
-            }
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int j = j_first + i * T;
+            const int pos = slot_position(q[i], j, n, seen);
+            key[i] = j >= n ? 0u : pos < p.sink || pos >= seen - p.recent ? 0xffffffffu : weight_key(w[i]);
         }
-        if (n3 >= B) t = c3, at_t = n3;
-        else if (n2 >= B) t = c2, at_t = n2, above = n3;
-        else if (n1 >= B) t = c1, at_t = n1, above = n2;
-        else above = n1;
-        if (at_t == B) break;   // exactly the keys >= t: no ties to choose from
     }
+    // Six sums (and, for `maxima`, two maxima) over all threads of the cluster.  A warp-wide
+    // reduction takes a scheduler some 35 cycles, so a warp's six counts go in two of them and
+    // one warp each adds up the warps' results.
+    int round = 0;
+    uint32_t res[8];
+    auto join = [&](const uint32_t (&c)[6], bool maxima, uint32_t m0, uint32_t m1) {
+        uint32_t sum[6];
+        if (ITEMS <= 16) {   // a warp's counts fit 10 bits: three to a reduction
+            const uint32_t a = __reduce_add_sync(0xffffffffu, c[0] | (c[1] << 10) | (c[2] << 20));
+            const uint32_t b = __reduce_add_sync(0xffffffffu, c[3] | (c[4] << 10) | (c[5] << 20));
+#pragma unroll
+            for (int k = 0; k < 3; ++k) sum[k] = (a >> (10 * k)) & 1023u, sum[3 + k] = (b >> (10 * k)) & 1023u;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 6; ++k) sum[k] = __reduce_add_sync(0xffffffffu, c[k]);
+        }
+        if (maxima) {
+            m0 = __reduce_max_sync(0xffffffffu, m0);
+            m1 = __reduce_max_sync(0xffffffffu, m1);
+        }
+        if (lane < 8) {
+            uint32_t mine = lane == 6 ? m0 : m1;
+#pragma unroll
+            for (int k = 0; k < 6; ++k)
+                if (lane == k) mine = sum[k];
+            s_cnt[lane][warp] = mine;
+        }
+        __syncthreads();
+        uint32_t (*box)[8] = s_box[round & 1];
+        for (int k = warp; k < (maxima ? 8 : 6); k += W) {
+            const uint32_t v = lane < W ? s_cnt[k][lane] : 0;
+            const uint32_t all = k < 6 ? __reduce_add_sync(0xffffffffu, v) : __reduce_max_sync(0xffffffffu, v);
+            if (C == 1) {
+                if (lane == 0) box[0][k] = all;
+            } else if (lane < C) {   // to every CTA of the cluster
+                const uint32_t dst = map_shared_rank(smem_u32(&box[rank][k]), lane);
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(all) : "memory");
+            }
+        }
+        if (C > 1) cluster_sync_all();
+        else __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) res[k] = box[0][k];
+        for (int r = 1; r < C; ++r) {
+#pragma unroll
+            for (int k = 0; k < 6; ++k) res[k] += box[r][k];
+            res[6] = max(res[6], box[r][6]);
+            res[7] = max(res[7], box[r][7]);
+        }
+        ++round;
+    };
+    // The bracket [lo, hi) with count(>= lo) = at_lo >= B > at_hi = count(>= hi): at first the
+    // smallest key and just above the largest unprotected one.
+    uint32_t lo = 0xffffffffu, hi = 0xffffffffu;
+    int at_lo = B, at_hi = 0;
+    {
+        uint32_t c[6] = {0, 0, 0, 0, 0, 0}, top = 0, bottom = 0;   // bottom: largest complement
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const bool in = j_first + i * T < n;
+            c[0] += key[i] == 0xffffffffu;
+            if (in && key[i] != 0xffffffffu) top = max(top, key[i]), bottom = max(bottom, ~key[i]);
+        }
+        join(c, true, top, bottom);
+        const int safe = static_cast<int>(res[0]);
+        if (safe < B) lo = ~res[7], hi = res[6] + 1, at_lo = n, at_hi = safe;
+        // safe >= B: exactly the protected ones (at most `budget` of them)
+        else at_lo = safe;
+    }
+    auto narrow = [&](uint32_t c, int k) {
+        if (k >= B) {
+            if (c > lo) lo = c, at_lo = k;
+        } else if (c < hi) {
+            hi = c, at_hi = k;
+        }
+    };
+    while (at_lo != B && hi - lo > 1) {
+        const uint32_t size = hi - lo;
+        const float at = __fdividef(static_cast<float>(at_lo - B) + 0.5f, static_cast<float>(at_lo - at_hi));
+        const uint32_t d = size / 8 + 1, e = size / 64 + 1;
+        const uint32_t x = lo + min(static_cast<uint32_t>(at * static_cast<float>(size)), size - 1);
+        uint32_t cand[6] = {x > lo + d ? x - d : lo + 1, x > lo + e ? x - e : lo + 1, x, hi - x > e ? x + e : hi - 1,
+                            hi - x > d ? x + d : hi - 1, lo + size / 2};
+        uint32_t c[6] = {0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 6; ++k) cand[k] = max(cand[k], lo + 1);   // inside (lo, hi)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int k = 0; k < 6; ++k) c[k] += key[i] >= cand[k];
+        join(c, false, 0, 0);
+#pragma unroll
+        for (int k = 0; k < 6; ++k) narrow(cand[k], static_cast<int>(res[k]));
+    }
+    const uint32_t t = lo;
+    const int at_t = at_lo, above = at_hi;   // keys >= t; keys above t where ties decide
 
-    // Ordered counts: flags of (CTA, item, thread) order = slot order.  Leaves in s_scan the
-    // number of flags before each (item, warp) of the cluster; returns their total.
+    // Ordered counts: flags in (CTA, item, thread) order = slot order.  Afterwards before_me()
+    // gives the flags in front of one of this thread's items; returns their total.
+    int scans = 0;
+    int item_first[ITEMS];   // flags before this CTA's item i
     auto ordered = [&](uint32_t flags) -> int {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const uint32_t bal = __ballot_sync(0xffffffffu, (flags >> i) & 1u);
-            if (lane == 0) s_scan[i * W + warp] = __popc(bal);
+            if (lane == 0) s_scan[i][warp] = __popc(bal);
         }
         __syncthreads();
-        if (warp == 0) {
-            int run = 0;
-            for (int e0 = 0; e0 < ITEMS * W; e0 += 32) {
-                const int e = e0 + lane;
-                const int v = e < ITEMS * W ? s_scan[e] : 0;
-                int x = v;
+        for (int i = warp; i < ITEMS; i += W) {   // one warp an item: prefix over its W warps
+            const int v = lane < W ? s_scan[i][lane] : 0;
+            int x = v;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int y = __shfl_up_sync(0xffffffffu, x, o);
-                    if (lane >= o) x += y;
-                }
-                if (e < ITEMS * W) s_scan[e] = run + x - v;
-                run += __shfl_sync(0xffffffffu, x, 31);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
             }
-            if (lane == 0) s_total = run;
+            if (lane < W) s_scan[i][lane] = x - v;
+            if (lane == 31) s_item[i] = x;
         }
         __syncthreads();
-        int total = s_total;
+        int total = 0;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            item_first[i] = total;
+            total += s_item[i];
+        }
         if (C > 1) {
+            const int box = scans++ & 1;   // at most two scans, a box each
             if (tid < C) {
-                const uint32_t dst = map_shared_rank(smem_u32(&s_tot_box[rank]), tid);
+                const uint32_t dst = map_shared_rank(smem_u32(&s_tot_box[box][rank]), tid);
                 asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(total) : "memory");
             }
             cluster_sync_all();
             int before = 0;
             total = 0;
             for (int r = 0; r < C; ++r) {
-                if (r < rank) before += s_tot_box[r];
-                total += s_tot_box[r];
+                if (r < rank) before += s_tot_box[box][r];
+                total += s_tot_box[box][r];
             }
-            cluster_sync_all();   // every CTA has read its box before the next count writes it
-            for (int e = tid; e < ITEMS * W; e += T) s_scan[e] += before;
-            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) item_first[i] += before;
         }
         return total;
     };
     auto before_me = [&](uint32_t flags, int i) -> int {   // flags before this thread's item i
         const uint32_t bal = __ballot_sync(0xffffffffu, (flags >> i) & 1u);
-        return s_scan[i * W + warp] + __popc(bal & ((1u << lane) - 1u));
+        return item_first[i] + s_scan[i][warp] + __popc(bal & ((1u << lane) - 1u));
     };
 
     uint32_t kept = 0, ties = 0;
@@ -260,17 +339,22 @@ __global__ void __launch_bounds__(kMaxThreads) evict_kernel(const __grid_constan
         if (j < n && (j < B ? !k : k)) moved |= 1u << i;
     }
     const int m = ordered(moved) / 2;   // as many movers as holes
-    int *holes = p.lists + unit * 2 * p.cap, *movers = holes + p.cap;
+    // The lists: short ones in every CTA's shared memory, long ones in the workspace.
+    int *holes = p.smem_lists ? s_holes : p.lists + unit * 2 * p.cap;
+    int *movers = p.smem_lists ? s_movers : holes + p.cap;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int j = j_first + i * T;
         const int k = before_me(moved, i);
         if ((moved >> i) & 1u) {
-            if (j < B) holes[k] = j;
-            else movers[k - m] = j;
+            int *at = j < B ? holes + k : movers + (k - m);
+            if (!p.smem_lists || C == 1) *at = j;
+            else
+                for (int r = 0; r < C; ++r)
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_shared_rank(smem_u32(at), r)), "r"(j)
+                                 : "memory");
         }
     }
-    if (rank == 0 && tid == 0) p.counts[unit] = m;
     // slots that stay
 #pragma unroll 4
     for (int i = 0; i < ITEMS; ++i) {
@@ -281,17 +365,16 @@ __global__ void __launch_bounds__(kMaxThreads) evict_kernel(const __grid_constan
             if (pos_in != pos_out || q < 0) pos_out[j] = slot_position(q, j, n, seen);
         }
     }
-    __threadfence();
+    if (!p.smem_lists) __threadfence();
     __syncthreads();
     if (C > 1) cluster_sync_all();   // the lists are complete
     for (int r = rank * T + tid; r < m; r += C * T) {
-        const int src = movers[r], dst = holes[r];
+        const int dst = holes[r], src = movers[r];
         w_out[dst] = w_in[src];
         pos_out[dst] = slot_position(pos_in[src], src, n, seen);
     }
-    if (p.fused) move_rows(p, row0, h, holes, movers, m, rank * W + warp, C * W);
     __syncthreads();
-    if (C > 1) cluster_sync_all();   // every mover has been read
+    if (C > 1) cluster_sync_all();   // every mover's weight and position has been read
 #pragma unroll 4
     for (int i = 0; i < ITEMS; ++i) {
         const int j = j_first + i * T;
@@ -300,21 +383,7 @@ __global__ void __launch_bounds__(kMaxThreads) evict_kernel(const __grid_constan
             pos_out[j] = -1;
         }
     }
-}
-
-constexpr int kMoveThreads = 256;
-
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p)
-{
-    griddep_wait();
-    griddep_trigger();
-    const int h = blockIdx.y, b = blockIdx.z;
-    const long long unit = static_cast<long long>(b) * p.n_kv_heads + h;
-    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) p.kv_len_out[b] = p.lengths[b];
-    const int m = p.fused ? 0 : p.counts[unit];
-    const int *holes = p.lists + unit * 2 * p.cap;
-    const int W = kMoveThreads / 32;
-    move_rows(p, p.seq_row0[b], h, holes, holes + p.cap, m, blockIdx.x * W + threadIdx.x / 32, gridDim.x * W);
+    move_rows(p, row0, h, m, rank * T + tid, C * T, [&](int r) { return make_int2(holes[r], movers[r]); });
 }
 
 // kv_len_out is kv_len_in: written once every CTA has read it
@@ -327,7 +396,7 @@ __global__ void evict_length_kernel(int *kv_len_out, const int *lengths, int n_s
 }
 
 struct EvictLayout {
-    size_t counts, lengths, total;
+    size_t lengths, total;
     int cap;
 };
 
@@ -337,8 +406,7 @@ EvictLayout evict_layout(int n_seqs, int max_kv_len, int n_kv_heads)
     EvictLayout L;
     const size_t units = static_cast<size_t>(n_seqs) * n_kv_heads;
     L.cap = max_kv_len / 2 + 1;   // min(B, n - B) moves at most
-    L.counts = al(units * 2 * L.cap * 4);
-    L.lengths = L.counts + al(units * 4);
+    L.lengths = al(units * 2 * L.cap * 4);
     L.total = L.lengths + al(static_cast<size_t>(n_seqs) * 4);
     return L;
 }
@@ -404,7 +472,6 @@ int cache_evict(cudaStream_t st, uint16_t *k_pool, uint16_t *v_pool, int64_t poo
     p.kv_len_out = kv_len_out;
     p.seq_pos = seq_pos;
     p.lists = reinterpret_cast<int *>(base);
-    p.counts = reinterpret_cast<int *>(base + L.counts);
     p.lengths = reinterpret_cast<int *>(base + L.lengths);
     p.err = device_error_word();
     if (!p.err) return SMOL_B200_ERR_CUDA;
@@ -416,17 +483,18 @@ int cache_evict(cudaStream_t st, uint16_t *k_pool, uint16_t *v_pool, int64_t poo
     p.recent = recent;
     p.cap = L.cap;
     const int most = budget < max_kv_len - budget ? budget : max_kv_len - budget;   // moves of one head
-    p.fused = most <= kFusedMoves;
-    p.write_len = p.fused && kv_len_out != kv_len_in;
-    // Slots per CTA: one CTA per (sequence, KV head) while there are enough of them, else a
-    // cluster; never more than kMaxItems per thread.
+    p.smem_lists = most <= kSmemMoves;
+    p.write_len = kv_len_out != kv_len_in;
+    // One CTA of up to 1024 threads (which fill an SM's registers) per (sequence, KV head), or a
+    // cluster: for more slots than it can hold, and while the CTAs still run at once and have
+    // more than two slots a thread.
     const long long units = static_cast<long long>(n_seqs) * n_kv_heads;
     int C = 1;
     while (C < kMaxCluster && (max_kv_len > C * kMaxItems * kMaxThreads ||
-                               (units * C < 148 && max_kv_len > C * 2 * kMaxThreads)))
+                               (units * C * 2 <= 148 && max_kv_len > C * 2 * kMaxThreads)))
         C *= 2;
     const int per = (max_kv_len + C - 1) / C;
-    int threads = per >= 4 * kMaxThreads ? kMaxThreads : (per / 4 + 31) / 32 * 32;
+    int threads = per >= 4 * kMaxThreads ? kMaxThreads : ((per + 3) / 4 + 31) / 32 * 32;
     if (threads < 128) threads = 128;
     const int items = per > 0 ? (per + threads - 1) / threads : 1;
     PdlScope pdl(g_api_pdl);
@@ -439,14 +507,7 @@ int cache_evict(cudaStream_t st, uint16_t *k_pool, uint16_t *v_pool, int64_t poo
         cudaGetLastError();
         return SMOL_B200_ERR_CUDA;
     }
-    if (!p.fused) {
-        const int per_cta = kMoveThreads / 32 * 4;   // four moves a warp
-        int x = (most + per_cta - 1) / per_cta;
-        if (x > 256) x = 256;
-        if (launch_kernel(evict_move_kernel, dim3(x, n_kv_heads, n_seqs), dim3(kMoveThreads), 0, st, p) !=
-            cudaSuccess)
-            return SMOL_B200_ERR_CUDA;
-    } else if (!p.write_len) {
+    if (!p.write_len) {
         if (launch_kernel(evict_length_kernel, dim3((n_seqs + 255) / 256), dim3(256), 0, st, kv_len_out,
                           static_cast<const int *>(p.lengths), n_seqs) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
