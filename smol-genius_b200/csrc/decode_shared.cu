@@ -25,16 +25,16 @@
 #include <mutex>
 
 #include "b200_common.cuh"
+#include "fast_math.cuh"
 #include "runtime.h"
 
 namespace smolb200 {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSms = 148;
 
 struct SharedParams {
-    CUtensorMap tk, tv;             // [pool_rows, kv_dim], boxes of 64 columns
+    CUtensorMap tk, tv;             // [pool_rows, kv_dim], boxes of 64 columns x 64 rows (PrefixShape's kBoxRows)
     const void *q;                  // [n_seqs, n_heads*hd] fp32 or bf16
     const int64_t *prefix_row0;
     const int *prefix_len, *prefix_seq0;
@@ -52,19 +52,14 @@ struct SharedParams {
     int n_seqs, n_heads, n_kv_heads, group, n_qgroups;
     int n_prefixes, max_prefix_len, max_prefix_seqs;
     int prefix_chunk, prefix_slots; // keys of one prefix part; parts of the longest prefix
+    int prefix_qtiles;              // query tiles of the largest group
+    int prefix_items;               // query tiles x parts x KV heads x prefixes
     int chunk, max_chunks;          // the same for own rows
     int slots;                      // prefix_slots + max_chunks
     int max_kv_len, score_rows, score_cols;
     int window;
     float scale, softcap;
 };
-
-__device__ __forceinline__ float fast_exp2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // x0, x1 as TERMS packed bf16 pairs whose sum is x to 8*TERMS bits.
 template <int TERMS>
@@ -114,8 +109,9 @@ __device__ __forceinline__ void own_range(const SharedParams &p, int b, int &ks,
 // ===========================================================================
 // prefix
 // ===========================================================================
-// CTA = (query tile, KV head and chunk of keys, prefix): softmax warpgroups of one packed
-// row per thread (thread = TMEM lane), a TMA producer warp and a tcgen05 issuer warp.
+// Item = (query tile, part of the keys, KV head, prefix); persistent CTAs take items in turn:
+// softmax warpgroups of one packed row per thread (thread = TMEM lane), a TMA producer warp
+// that runs ahead into the next item, and a tcgen05 issuer warp.
 //   S = Q K^T  (QT bf16 terms of Q, fp32 in TMEM, two buffers)
 //   P = 2^(S*scale*log2e - m) as PT fp16 terms over S's columns
 //   O += P V
@@ -132,6 +128,7 @@ struct PrefixShape {
     // Key tile: 128; 64 / 32 where the query terms of head dim 256 (64 KB each) leave less room.
     static constexpr int BN = HD == 256 ? (QT == 3 ? 32 : 64) : 128;
     static constexpr int kStages = HD == 256 && QT == 3 ? 1 : 2;
+    static constexpr int kBoxRows = BN < 64 ? BN : 64;   // of a TMA copy: 64 fits the split kernel too
     static constexpr int kSub = HD / 64;
     static constexpr int kQSubBytes = kBM * 128;
     static constexpr int kQTermBytes = kSub * kQSubBytes;
@@ -150,13 +147,110 @@ struct PrefixShape {
     static constexpr int kTmO = 2 * BN;                 // O of warpgroup w at kTmO + w * HD
     static constexpr int kTmCols = 512;
     static_assert(kTmO + kGroups * HD <= kTmCols, "TMEM");
+    // once an item's products are complete its Q makes room for the warpgroups' (m, l) and
+    // then for 2 KB of staged output per warp
+    static_assert(kGroups * 4 * 2048 <= kQTermBytes, "staging");
 };
 
 struct PrefixBars {
     uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], o_final, mma_done;
     uint32_t tmem_base;
-    int lo_min;
 };
+
+// Query tiles and parts of prefix g.
+__device__ __forceinline__ int prefix_tiles(const SharedParams &p, int s0, int s1)
+{
+    return s1 > s0 ? ((s1 - s0) * p.group + kBM - 1) / kBM : 0;
+}
+__device__ __forceinline__ int prefix_parts_of(const SharedParams &p, int plen)
+{
+    return (plen + p.prefix_chunk - 1) / p.prefix_chunk;
+}
+
+// One item's geometry, found by each warp for itself.
+struct PrefixItem {
+    int qt, kvh, c, g;
+    int s0, s1, plen;        // sequences and length of the prefix
+    int key_lo, key_hi;      // keys of the part
+    int n_tiles;
+};
+
+// Up to 32 prefixes: lane g knows prefix g, and items are numbered over the query tiles and
+// parts that exist, so that CTAs get equal counts of them.  More: over those of the largest
+// group and longest prefix.
+struct PrefixTable {
+    int s0, s1, plen;
+    int items;               // of prefixes 0 .. lane
+    int all;
+};
+
+__device__ __forceinline__ PrefixTable prefix_table(const SharedParams &p, bool flag)
+{
+    PrefixTable t;
+    t.s0 = t.s1 = t.plen = 0;
+    t.items = 0;
+    t.all = p.prefix_items;
+    if (p.n_prefixes > 32) return t;
+    const int lane = threadIdx.x % 32;
+    if (lane < p.n_prefixes) {
+        prefix_range(p, lane, t.s0, t.s1, t.plen, flag);
+        t.items = prefix_tiles(p, t.s0, t.s1) * prefix_parts_of(p, t.plen) * p.n_kv_heads;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, t.items, o);
+        if (lane >= o) t.items += y;
+    }
+    t.all = __shfl_sync(0xffffffffu, t.items, 31);
+    return t;
+}
+
+template <int BN>
+__device__ __forceinline__ PrefixItem prefix_item(const SharedParams &p, const PrefixTable &t, int k, bool flag)
+{
+    PrefixItem it;
+    int qtiles = p.prefix_qtiles, parts = p.prefix_slots;
+    if (p.n_prefixes <= 32) {
+        it.g = __popc(__ballot_sync(0xffffffffu, t.items <= k));
+        const int before = __shfl_sync(0xffffffffu, t.items, it.g > 0 ? it.g - 1 : 0);
+        if (it.g > 0) k -= before;
+        it.s0 = __shfl_sync(0xffffffffu, t.s0, it.g);
+        it.s1 = __shfl_sync(0xffffffffu, t.s1, it.g);
+        it.plen = __shfl_sync(0xffffffffu, t.plen, it.g);
+        qtiles = prefix_tiles(p, it.s0, it.s1);
+        parts = prefix_parts_of(p, it.plen);
+    }
+    // query tiles fastest: those that share keys run at the same time
+    it.qt = k % qtiles;
+    k /= qtiles;
+    it.c = k % parts;
+    k /= parts;
+    it.kvh = k % p.n_kv_heads;
+    if (p.n_prefixes > 32) {
+        it.g = k / p.n_kv_heads;
+        prefix_range(p, it.g, it.s0, it.s1, it.plen, flag && it.qt == 0 && it.c == 0 && it.kvh == 0);
+    }
+    it.n_tiles = 0;
+    it.key_lo = it.key_hi = 0;
+    const int b0 = it.s0 + it.qt * kBM / p.group;   // sequences of the tile: [b0, b1)
+    if (b0 >= it.s1) return it;
+    // parts count from the first key any row of the tile sees
+    int lo = 0;
+    if (p.window > 0) {
+        const int b1 = min(it.s1, it.s0 + (it.qt * kBM + kBM - 1) / p.group + 1);
+        lo = it.plen;
+        for (int b = b0 + static_cast<int>(threadIdx.x % 32); b < b1; b += 32) {
+            int ks, n;
+            own_range(p, b, ks, n);
+            lo = min(lo, max(0, it.plen + n - p.window));
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo);
+    }
+    it.key_lo = lo + it.c * p.prefix_chunk;
+    it.key_hi = min(it.plen, it.key_lo + p.prefix_chunk);
+    if (it.key_hi > it.key_lo) it.n_tiles = (it.key_hi - it.key_lo + BN - 1) / BN;
+    return it;
+}
 
 template <int HD, int QT, int PT>
 __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kernel(const __grid_constant__ SharedParams p)
@@ -165,32 +259,11 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
     constexpr int BN = S::BN, ST = S::kStages, NG = S::kGroups;
     constexpr int kProducer = NG * 4, kIssuer = kProducer + 1;
     static_assert(sizeof(PrefixBars) <= 256, "barriers");
-    griddep_wait();
-    griddep_trigger();
-    const int qt = blockIdx.x;
-    const int kvh = blockIdx.y / p.prefix_slots, c = blockIdx.y % p.prefix_slots;
-    const int g = blockIdx.z;
-    int s0, s1, plen;
-    prefix_range(p, g, s0, s1, plen, threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0);
-    if (s1 <= s0 || qt * kBM >= (s1 - s0) * p.group) return;   // no rows in this tile
-
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     PrefixBars *bars = reinterpret_cast<PrefixBars *>(smem + S::kOffBar);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-
-    // this softmax thread's packed row and its first visible prefix key
-    const int pr = qt * kBM + static_cast<int>(threadIdx.x) % kBM;
-    const int b = s0 + pr / p.group, head = kvh * p.group + pr % p.group;
-    const bool row_valid = warp < kProducer && b < s1;
-    int lo = 0;
-    if (row_valid && p.window > 0) {
-        int ks, n;
-        own_range(p, b, ks, n);
-        lo = max(0, plen + n - p.window);
-    }
     if (threadIdx.x == 0) {
-        bars->lo_min = plen;
         mbar_init(smem_u32(&bars->q_full), S::kSoftmax);
         for (int s = 0; s < 2; ++s) {
             mbar_init(smem_u32(&bars->k_full[s]), 1);
@@ -205,20 +278,10 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
         mbar_init(smem_u32(&bars->mma_done), 1);
         fence_mbar_init();
     }
-    __syncthreads();
-    if (row_valid && lo < plen) atomicMin(&bars->lo_min, lo);
-    __syncthreads();
-    // keys of this part: the chunks count from the first key any row of the tile sees
-    const int key_lo = bars->lo_min + c * p.prefix_chunk;
-    const int key_hi = min(plen, key_lo + p.prefix_chunk);
-    const int n_tiles = key_hi > key_lo ? (key_hi - key_lo + BN - 1) / BN : 0;
-    const long long slot = (static_cast<long long>(b) * p.n_heads + head) * p.slots + c;
-    if (n_tiles == 0) {
-        if (row_valid && threadIdx.x < kBM) p.part_ml[slot] = make_float2(-INFINITY, 0.f);
-        return;
-    }
-    const long long row_base = p.prefix_row0[g] + key_lo;
-
+    // TMEM only after the wait: a CTA that held it while an earlier kernel's CTA on the same SM
+    // still had to allocate would wait for that kernel for good
+    griddep_wait();
+    griddep_trigger();
     if (warp == kIssuer) {
         tmem_alloc(smem_u32(&bars->tmem_base), S::kTmCols);
         tmem_relinquish();
@@ -230,46 +293,72 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
     uint8_t *sK = smem + S::kOffK;
     uint8_t *sV = smem + S::kOffV;
 
+    const PrefixTable table = prefix_table(p, blockIdx.x == 0 && warp == 0);
+    // Items with key tiles are numbered n_items = 0, 1, ... and their tiles g = 0, 1, ... over the
+    // whole CTA; every barrier's phase follows from these numbers.
     if (warp == kProducer) {
-        // ================= TMA producer =================
+        // ================= TMA producer (one lane issues; the geometry takes the warp) =================
         if (lane == 0) {
             tma_prefetch_desc(&p.tk);
             tma_prefetch_desc(&p.tv);
-            int nk = 0, nv = 0;   // K and V tiles issued
-            auto load = [&](bool is_v, int j) -> bool {
-                const int st = j % ST;
+        }
+        int nk = 0, nv = 0;   // K and V tiles issued
+        int v_kvh = 0, v_row = 0;   // V tile nv, owed until K tile nv + 1 is issued
+        bool ok = true;
+        auto load = [&](bool is_v, int n, int kvh, int row) -> bool {
+            const int st = n % ST;
+            bool good = true;
+            if (lane == 0) {
                 const uint32_t full = smem_u32(is_v ? &bars->v_full[st] : &bars->k_full[st]);
                 const uint32_t empty = smem_u32(is_v ? &bars->v_empty[st] : &bars->k_empty[st]);
-                if (j >= ST && !mbar_wait(empty, (j / ST - 1) & 1, p.err, kErrWaitTmaEmpty)) return false;
-                mbar_arrive_expect_tx(full, S::kKvBytes);
-                uint8_t *dst = (is_v ? sV : sK) + st * S::kKvBytes;
+                good = n < ST || mbar_wait(empty, (n / ST - 1) & 1, p.err, kErrWaitTmaEmpty);
+                if (good) {
+                    mbar_arrive_expect_tx(full, S::kKvBytes);
+                    uint8_t *dst = (is_v ? sV : sK) + st * S::kKvBytes;
 #pragma unroll
-                for (int sub = 0; sub < S::kSub; ++sub)
-                    tma_load_2d(smem_u32(dst + sub * S::kKvSubBytes), is_v ? &p.tv : &p.tk, full, kvh * HD + sub * 64,
-                                static_cast<int>(row_base + j * BN));
-                return true;
-            };
-            bool ok = true;
-            for (int j = 0; j < n_tiles && ok; ++j) {   // K runs one tile ahead of V
-                if ((ok = load(false, j))) ++nk;
-                if (ok && j >= 1 && (ok = load(true, j - 1))) ++nv;
+                    for (int sub = 0; sub < S::kSub; ++sub)
+#pragma unroll
+                        for (int r = 0; r < BN; r += S::kBoxRows)
+                            tma_load_2d(smem_u32(dst + sub * S::kKvSubBytes + r * 128), is_v ? &p.tv : &p.tk, full,
+                                        kvh * HD + sub * 64, row + r);
+                }
             }
-            if (ok && load(true, n_tiles - 1)) ++nv;
+            return __shfl_sync(0xffffffffu, good, 0);
+        };
+        for (int k = blockIdx.x; k < table.all && ok; k += gridDim.x) {
+            const PrefixItem it = prefix_item<BN>(p, table, k, lane == 0);
+            if (it.n_tiles == 0) continue;
+            const int row0 = static_cast<int>(p.prefix_row0[it.g] + it.key_lo);
+            for (int j = 0; j < it.n_tiles && ok; ++j) {   // K runs one tile ahead of V
+                if (!(ok = load(false, nk, it.kvh, row0 + j * BN))) break;
+                ++nk;
+                if (nv < nk - 1) {
+                    if (!(ok = load(true, nv, v_kvh, v_row))) break;
+                    ++nv;
+                }
+                v_kvh = it.kvh;
+                v_row = row0 + j * BN;
+            }
+        }
+        if (ok && nv < nk && load(true, nv, v_kvh, v_row)) ++nv;
+        if (lane == 0) {
             for (int j = max(0, nk - ST); j < nk; ++j)
                 if (!mbar_wait(smem_u32(&bars->k_full[j % ST]), (j / ST) & 1, p.err, kErrDrain)) break;
             for (int j = max(0, nv - ST); j < nv; ++j)
                 if (!mbar_wait(smem_u32(&bars->v_full[j % ST]), (j / ST) & 1, p.err, kErrDrain)) break;
         }
+        __syncwarp();
     } else if (warp == kIssuer) {
         // ================= tcgen05 issuer (converged warp, one elected lane issues) =================
         constexpr uint32_t idesc_s = umma_idesc_f16(kBM, BN, true, false);
         constexpr uint32_t idesc_pv = umma_idesc_f16(kBM, HD, false, true);
         const uint32_t q_addr = smem_u32(smem);
+        int n_items = 0, g0 = 0;
+        // P V of tile j of the item whose first tile has number g0
         auto issue_pv = [&](int j) -> bool {
-            const int st = j % ST, sb = j & 1;
-            // the softmax threads waited for V(j) themselves before they arrived here
-            if (!mbar_wait_warp(smem_u32(&bars->p_full[sb]), (j >> 1) & 1, p.err, kErrWaitSoftmax)) return false;
-            if (!mbar_wait_warp(smem_u32(&bars->v_full[st]), (j / ST) & 1, p.err, kErrWaitTmaFull)) return false;
+            const int g = g0 + j, st = g % ST, sb = g & 1;
+            if (!mbar_wait_warp(smem_u32(&bars->p_full[sb]), (g >> 1) & 1, p.err, kErrWaitSoftmax)) return false;
+            if (!mbar_wait_warp(smem_u32(&bars->v_full[st]), (g / ST) & 1, p.err, kErrWaitTmaFull)) return false;
             tc_fence_after();
             const uint32_t v_addr = smem_u32(sV + st * S::kKvBytes);
 #pragma unroll
@@ -278,264 +367,318 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
                 for (int kk = 0; kk < BN / 16; ++kk) {
                     const uint64_t bd = umma_sdesc_sw128(v_addr + kk * 16 * 128, S::kKvSubBytes, 1024);
                     // columns of P: see the softmax (32-key groups: 16 of values, 16 of remainders)
-                    umma_ts_elect(tmem + S::kTmO + (j % NG) * HD, tmem + sb * BN + (kk >> 1) * 32 + t * 16 + (kk & 1) * 8, bd,
+                    umma_ts_elect(tmem + S::kTmO + (g % NG) * HD, tmem + sb * BN + (kk >> 1) * 32 + t * 16 + (kk & 1) * 8, bd,
                                   idesc_pv, (j >= NG || t < PT - 1 || kk > 0) ? 1u : 0u);
                 }
-            umma_commit_elect(smem_u32(&bars->o_done[j % NG]));
+            umma_commit_elect(smem_u32(&bars->o_done[g % NG]));
             umma_commit_elect(smem_u32(&bars->v_empty[st]));
             return true;
         };
-        bool ok = mbar_wait_warp(smem_u32(&bars->q_full), 0, p.err, kErrWaitSoftmax);
-        // Two warpgroups: P V of tile j - 2, whose P lies in the buffer of S(j), goes before
-        // S(j).  One: S(j) goes first, so that it runs during the softmax of tile j - 1.
-        for (int j = 0; j < n_tiles && ok; ++j) {
-            const int st = j % ST;
-            if (NG == 2 && j >= 2 && !(ok = issue_pv(j - 2))) break;
-            if (!(ok = mbar_wait_warp(smem_u32(&bars->k_full[st]), (j / ST) & 1, p.err, kErrWaitTmaFull))) break;
-            tc_fence_after();
-            const uint32_t k_addr = smem_u32(sK + st * S::kKvBytes);
-            const uint32_t s_col = tmem + (j & 1) * BN;
+        bool ok = true;
+        for (int k = blockIdx.x; k < table.all && ok; k += gridDim.x) {
+            const PrefixItem it = prefix_item<BN>(p, table, k, false);
+            if (it.n_tiles == 0) continue;
+            // Q is written after the item before was read out, so its O may be overwritten too
+            ok = mbar_wait_warp(smem_u32(&bars->q_full), n_items & 1, p.err, kErrWaitSoftmax);
+            // Two warpgroups: P V of tile j - 2, whose P lies in the buffer of S(j), goes before
+            // S(j).  One: S(j) goes first, so that it runs during the softmax of tile j - 1.
+            for (int j = 0; j < it.n_tiles && ok; ++j) {
+                const int g = g0 + j, st = g % ST;
+                if (NG == 2 && j >= 2 && !(ok = issue_pv(j - 2))) break;
+                if (!(ok = mbar_wait_warp(smem_u32(&bars->k_full[st]), (g / ST) & 1, p.err, kErrWaitTmaFull))) break;
+                tc_fence_after();
+                const uint32_t k_addr = smem_u32(sK + st * S::kKvBytes);
+                const uint32_t s_col = tmem + (g & 1) * BN;
 #pragma unroll
-            for (int t = QT - 1; t >= 0; --t)
+                for (int t = QT - 1; t >= 0; --t)
 #pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk) {
-                    const uint32_t off = (kk & 3) * 32;
-                    const uint64_t ad =
-                        umma_sdesc_sw128(q_addr + t * S::kQTermBytes + (kk >> 2) * S::kQSubBytes + off, 16, 1024);
-                    const uint64_t bd = umma_sdesc_sw128(k_addr + (kk >> 2) * S::kKvSubBytes + off, 16, 1024);
-                    umma_ss_elect(s_col, ad, bd, idesc_s, (t < QT - 1 || kk > 0) ? 1u : 0u);
-                }
-            umma_commit_elect(smem_u32(&bars->s_full[j & 1]));
-            umma_commit_elect(smem_u32(&bars->k_empty[st]));
-            if (NG == 1 && j >= 1) ok = issue_pv(j - 1);
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint32_t off = (kk & 3) * 32;
+                        const uint64_t ad =
+                            umma_sdesc_sw128(q_addr + t * S::kQTermBytes + (kk >> 2) * S::kQSubBytes + off, 16, 1024);
+                        const uint64_t bd = umma_sdesc_sw128(k_addr + (kk >> 2) * S::kKvSubBytes + off, 16, 1024);
+                        umma_ss_elect(s_col, ad, bd, idesc_s, (t < QT - 1 || kk > 0) ? 1u : 0u);
+                    }
+                umma_commit_elect(smem_u32(&bars->s_full[g & 1]));
+                umma_commit_elect(smem_u32(&bars->k_empty[st]));
+                if (NG == 1 && j >= 1) ok = issue_pv(j - 1);
+            }
+            if (ok && NG == 2 && it.n_tiles >= 2) ok = issue_pv(it.n_tiles - 2);
+            if (ok) ok = issue_pv(it.n_tiles - 1);
+            if (ok) umma_commit_elect(smem_u32(&bars->o_final));
+            g0 += it.n_tiles;
+            ++n_items;
         }
-        if (ok && NG == 2 && n_tiles >= 2) ok = issue_pv(n_tiles - 2);
-        if (ok && issue_pv(n_tiles - 1)) umma_commit_elect(smem_u32(&bars->o_final));
         // every MMA must be complete before TMEM is released
         umma_commit_elect(smem_u32(&bars->mma_done));
         mbar_wait_warp(smem_u32(&bars->mma_done), 0, p.err, kErrDrain);
     } else {
         // ================= softmax =================
-        // This warp's query rows as QT bf16 terms in the 128B-swizzled K-major layout, kLoad
-        // 8-element pieces in flight per lane (one at a time took 11 us of an 18 us call at
-        // 512 prefix keys).  Rows past the last sequence stay unwritten: a row of Q only
-        // reaches its own row of S and O, and those rows are neither used nor stored.
-        constexpr int kVecs = HD / 8, kLoad = 4, kRows = 32 / NG;   // rows loaded by a warp
-        const int lr = warp * kRows;
-        if (s0 + (qt * kBM + lr) / p.group < s1) {
-            for (int i0 = lane; i0 < kRows * kVecs; i0 += 32 * kLoad) {
-                uint4 raw[kLoad][2];
-#pragma unroll
-                for (int n = 0; n < kLoad; ++n) {
-                    const int i = i0 + 32 * n;
-                    const int rr = qt * kBM + lr + i / kVecs;
-                    const int rb = s0 + rr / p.group, rh = kvh * p.group + rr % p.group;
-                    const long long off = (static_cast<long long>(rb) * p.n_heads + rh) * HD + (i % kVecs) * 8;
-                    if (rb < s1) {
-                        if (p.q_is_bf16) {
-                            raw[n][0] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + off));
-                        } else {
-                            const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const float *>(p.q) + off);
-                            raw[n][0] = __ldg(src);
-                            raw[n][1] = __ldg(src + 1);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < kLoad; ++n) {
-                    const int i = i0 + 32 * n;
-                    const int r = lr + i / kVecs, e = (i % kVecs) * 8;
-                    if (s0 + (qt * kBM + r) / p.group >= s1) continue;
-                    const uint32_t at = (e / 64) * S::kQSubBytes + sw128_offset(r, (e % 64) / 8);
-                    const uint32_t u[8] = {raw[n][0].x, raw[n][0].y, raw[n][0].z, raw[n][0].w,
-                                           raw[n][1].x, raw[n][1].y, raw[n][1].z, raw[n][1].w};
-                    uint32_t t[4][QT];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (p.q_is_bf16) {
-                            t[k][0] = u[k];
-#pragma unroll
-                            for (int q = 1; q < QT; ++q) t[k][q] = 0u;
-                        } else {
-                            split_bf16<QT>(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]), t[k]);
-                        }
-                    }
-#pragma unroll
-                    for (int q = 0; q < QT; ++q)
-                        *reinterpret_cast<uint4 *>(smem + q * S::kQTermBytes + at) =
-                            make_uint4(t[0][q], t[1][q], t[2][q], t[3][q]);
-                }
-            }
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(smem_u32(&bars->q_full));
-        const int wg = warp / 4;
-        const bool warp_live = s0 + (qt * kBM + (warp % 4) * 32) / p.group < s1;
+        const int wg = warp / 4, tid = threadIdx.x % kBM;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
-        const uint32_t o_col = lane_base + S::kTmO + wg * HD;
         const float cap = p.softcap, inv_cap = cap > 0.f ? 1.f / cap : 0.f;
         const float mul = cap > 0.f ? 1.f : p.scale * kLog2e;
-        float m = -INFINITY, l = 0.f;
-        bool ok = true;
-        for (int j = wg; j < n_tiles; j += NG) {
-            const int sb = j & 1;
-            ok = mbar_wait_warp(smem_u32(&bars->s_full[sb]), (j >> 1) & 1, p.err, kErrWaitMma);
-            if (!ok) break;
-            if (!warp_live && key_hi - (key_lo + j * BN) >= BN) {   // no row here, no V rows to clear
-                mbar_arrive(smem_u32(&bars->p_full[sb]));
+        int n_items = 0, g0 = 0;
+        bool ok = true;   // false after a wait that ran out (the device error word is set)
+        for (int k = blockIdx.x; k < table.all; k += gridDim.x) {
+            const PrefixItem it = prefix_item<BN>(p, table, k, false);
+            // this thread's packed row
+            const int pr = it.qt * kBM + tid;
+            const int b = it.s0 + pr / p.group;
+            const bool row_valid = b < it.s1;
+            const long long slot =
+                (static_cast<long long>(b) * p.n_heads + it.kvh * p.group + pr % p.group) * p.slots + it.c;
+            if (it.n_tiles == 0) {
+                if (row_valid && wg == 0) p.part_ml[slot] = make_float2(-INFINITY, 0.f);
                 continue;
             }
-            tc_fence_after();
-            const uint32_t s_col = lane_base + sb * BN;
-            const int key0 = key_lo + j * BN;
-            const bool whole = __all_sync(0xffffffffu, row_valid && key0 >= lo && key0 + BN <= key_hi);
-            // The row's keys in groups of 32 columns, once for the maximum and once for the
-            // exponentials: S is read twice, but the code stays small (fully unrolled over the
-            // tile it was fetched from memory for every short call).
-            float mx = -INFINITY;
+            int lo = 0;   // the row's first visible prefix key
+            if (row_valid && p.window > 0) {
+                int ks, n;
+                own_range(p, b, ks, n);
+                lo = max(0, it.plen + n - p.window);
+            }
+            // This warp's share of the query rows as QT bf16 terms in the 128B-swizzled K-major
+            // layout, kLoad 8-element pieces in flight per lane (one at a time took 11 us of an
+            // 18 us call at 512 prefix keys).  Rows past the last sequence stay as they are: a row
+            // of Q only reaches its own row of S and O, and those are neither used nor stored.
+            if (n_items > 0) named_bar_sync(1, S::kSoftmax);   // the last item's staging has been read
+            constexpr int kVecs = HD / 8, kLoad = QT == 1 ? 8 : 4, kRows = 32 / NG;   // rows loaded by a warp
+            const int lr = warp * kRows;
+            if (it.s0 + (it.qt * kBM + lr) / p.group < it.s1) {
 #pragma unroll 1
-            for (int q = 0; q < BN / 32; ++q) {
-                uint32_t rr[32];
-                tmem_ld32(s_col + q * 32, rr);
-                tmem_ld_wait();
-                if (!whole) {
+                for (int i0 = lane; i0 < kRows * kVecs; i0 += 32 * kLoad) {
+                    uint4 raw[kLoad][QT == 1 ? 1 : 2];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int key = key0 + q * 32 + i;
-                        if (!row_valid || key < lo || key >= key_hi) rr[i] = 0xff800000u;   // -inf
+                    for (int n = 0; n < kLoad; ++n) {
+                        const int i = i0 + 32 * n;
+                        const int rr = it.qt * kBM + lr + i / kVecs;
+                        const int rb = it.s0 + rr / p.group, rh = it.kvh * p.group + rr % p.group;
+                        const long long off = (static_cast<long long>(rb) * p.n_heads + rh) * HD + (i % kVecs) * 8;
+                        if (i < kRows * kVecs && rb < it.s1) {
+                            if constexpr (QT == 1) {
+                                raw[n][0] =
+                                    __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + off));
+                            } else {
+                                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const float *>(p.q) + off);
+                                raw[n][0] = __ldg(src);
+                                raw[n][1] = __ldg(src + 1);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < kLoad; ++n) {
+                        const int i = i0 + 32 * n;
+                        const int r = lr + i / kVecs, e = (i % kVecs) * 8;
+                        if (i >= kRows * kVecs || it.s0 + (it.qt * kBM + r) / p.group >= it.s1) continue;
+                        uint8_t *at = smem + (e / 64) * S::kQSubBytes + sw128_offset(r, (e % 64) / 8);
+                        if constexpr (QT == 1) {
+                            *reinterpret_cast<uint4 *>(at) = raw[n][0];
+                        } else {
+                            const uint32_t u[8] = {raw[n][0].x, raw[n][0].y, raw[n][0].z, raw[n][0].w,
+                                                   raw[n][1].x, raw[n][1].y, raw[n][1].z, raw[n][1].w};
+                            uint32_t t[4][QT];
+#pragma unroll
+                            for (int i2 = 0; i2 < 4; ++i2)
+                                split_bf16<QT>(__uint_as_float(u[2 * i2]), __uint_as_float(u[2 * i2 + 1]), t[i2]);
+#pragma unroll
+                            for (int q = 0; q < QT; ++q)
+                                *reinterpret_cast<uint4 *>(at + q * S::kQTermBytes) =
+                                    make_uint4(t[0][q], t[1][q], t[2][q], t[3][q]);
+                        }
                     }
                 }
-                float pm[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) pm[i] = fmaxf(__uint_as_float(rr[2 * i]), __uint_as_float(rr[2 * i + 1]));
-#pragma unroll
-                for (int i = 8; i < 32; i += 8)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        pm[k] = fmaxf(pm[k], fmaxf(__uint_as_float(rr[i + 2 * k]), __uint_as_float(rr[i + 2 * k + 1])));
-                mx = fmaxf(mx, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])));
             }
-            if (cap > 0.f) {   // the cap is monotonic: the maximum's capped score is the capped maximum
-                if (mx != -INFINITY) mx = cap * tanhf(mx * p.scale * inv_cap) * kLog2e;
-            } else {
-                mx *= mul;
-            }
-            // The reference m of a row is the first maximum it meets; it moves only when a
-            // maximum passes it by more than 2^8 (P stays below 256 in fp16), so O is rescaled
-            // rarely.  NaN scores keep m and reach P.
-            const bool fresh = m == -INFINITY;
-            const bool move = mx > m + kMoveLog2 || (fresh && mx != -INFINITY);
-            if (__any_sync(0xffffffffu, move && !fresh)) {
-                const float f = move && !fresh ? fast_exp2(m - mx) : 1.f;
-                l *= f;
-                // not the first tile; O holds the earlier ones' P V: scale it once they are complete
-                ok = mbar_wait_warp(smem_u32(&bars->o_done[wg]), (j / NG - 1) & 1, p.err, kErrWaitMma);
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll 1
-                for (int q = 0; q < HD / 32; ++q) {
-                    uint32_t ro[32];
-                    tmem_ld32(o_col + q * 32, ro);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) ro[i] = __float_as_uint(__uint_as_float(ro[i]) * f);
-                    tmem_st32(o_col + q * 32, ro);
-                }
-            }
-            if (move) m = mx;
-            const float negm = m != -INFINITY ? -m : 0.f;
-            // P over S, in place by groups: columns 32q .. 32q+15 take the fp16 pairs of the
-            // group's 32 keys, 32q+16 .. 32q+31 what their rounding left (PT == 2).
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-            for (int q = 0; q < BN / 32; ++q) {
-                uint32_t rr[32];
-                tmem_ld32(s_col + q * 32, rr);
-                tmem_ld_wait();
-                if (cap > 0.f) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        rr[i] = __float_as_uint(cap * tanhf(__uint_as_float(rr[i]) * p.scale * inv_cap) * kLog2e);
-                }
-                if (!whole) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int key = key0 + q * 32 + i;
-                        if (!row_valid || key < lo || key >= key_hi) rr[i] = 0xff800000u;
-                    }
-                }
-                uint32_t w[32];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float e0 = fast_exp2(fmaf(__uint_as_float(rr[2 * i]), mul, negm));
-                    const float e1 = fast_exp2(fmaf(__uint_as_float(rr[2 * i + 1]), mul, negm));
-                    acc[i & 3] += e0 + e1;
-                    if (PT == 2) split_f16(e0, e1, w[i], w[16 + i]);
-                    else w[i] = pack_f16x2(e0, e1), w[16 + i] = 0u;
-                }
-                tmem_st32(s_col + q * 32, w);
-            }
-            l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
-            // Rows of the V tile past the part's last key may hold anything (another
-            // sequence's rows, unwritten memory): 0 * NaN would reach O, so they are zeroed.
-            const int nv = key_hi - key0;
-            if (nv < BN) {
-                ok = mbar_wait_warp(smem_u32(&bars->v_full[j % ST]), (j / ST) & 1, p.err, kErrWaitTmaFull);
-                if (!ok) break;
-                uint8_t *vt = sV + (j % ST) * S::kKvBytes;
-                for (int i = threadIdx.x % kBM; i < (BN - nv) * 8 * S::kSub; i += kBM) {
-                    const int sub = i / ((BN - nv) * 8), k = i % ((BN - nv) * 8);
-                    *reinterpret_cast<uint4 *>(vt + sub * S::kKvSubBytes + nv * 128 + k * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async_smem();
-            }
-            tmem_st_wait();
+            fence_proxy_async_smem();
             tc_fence_before();
-            mbar_arrive(smem_u32(&bars->p_full[sb]));
-        }
-        // o_done may be two phases behind here (a parity wait could not tell), hence o_final
-        if (ok) ok = mbar_wait_warp(smem_u32(&bars->o_final), 0, p.err, kErrWaitMma);
-        // after a wait that ran out the part counts as empty (the device error word is set)
-        if (!ok) m = -INFINITY, l = 0.f;
-        float M = m, f[2] = {1.f, 0.f};   // the row's reference, and each warpgroup's factor to it
-        const int half = threadIdx.x % kBM;
-        if (NG == 2) {
-            float2 *ml = reinterpret_cast<float2 *>(sK);   // the K tiles are no longer needed
-            ml[wg * kBM + half] = make_float2(m, l);
-            named_bar_sync(1, S::kSoftmax);
-            const float2 a = ml[half], d = ml[kBM + half];
-            M = fmaxf(a.x, d.x);
-            f[0] = a.x == -INFINITY ? 0.f : fast_exp2(a.x - M);
-            f[1] = d.x == -INFINITY ? 0.f : fast_exp2(d.x - M);
-            l = f[0] * a.y + f[1] * d.y;
-        }
-        if (__any_sync(0xffffffffu, row_valid && M != -INFINITY)) {
-            tc_fence_after();
-            float *dst = p.part_o + slot * HD;
-#pragma unroll 1
-            for (int c0 = wg * (HD / NG); c0 < (wg + 1) * (HD / NG); c0 += 32) {
-                uint32_t r0[32], r1[32];
-                tmem_ld32(lane_base + S::kTmO + c0, r0);
-                if (NG == 2 && n_tiles > 1) tmem_ld32(lane_base + S::kTmO + HD + c0, r1);
-                tmem_ld_wait();
-                if (NG == 2) {
+            mbar_arrive(smem_u32(&bars->q_full));
+            const bool warp_live = it.s0 + (it.qt * kBM + (warp % 4) * 32) / p.group < it.s1;
+            float m = -INFINITY, l = 0.f;
+            // this warpgroup's tiles: numbers g with g % NG == wg; the first of the item is the
+            // wg'th or, where the item starts on an odd number, the other
+            for (int j = NG == 2 ? (g0 + wg) & 1 : 0; j < it.n_tiles; j += NG) {
+                const int g = g0 + j, sb = g & 1;
+                if (ok) ok = mbar_wait_warp(smem_u32(&bars->s_full[sb]), (g >> 1) & 1, p.err, kErrWaitMma);
+                if (!ok) break;
+                const int key0 = it.key_lo + j * BN;
+                const int nv = it.key_hi - key0;   // valid keys of the tile (may be more)
+                if (!warp_live && nv >= BN) {      // no row here, no V rows to clear
+                    mbar_arrive(smem_u32(&bars->p_full[sb]));
+                    continue;
+                }
+                tc_fence_after();
+                const uint32_t s_col = lane_base + sb * BN, o_col = lane_base + S::kTmO + (g % NG) * HD;
+                const bool whole = __all_sync(0xffffffffu, row_valid && key0 >= lo && nv >= BN);
+                // The row's keys in groups of 32 columns, once for the maximum and once for the
+                // exponentials: S is read twice, but the code stays small (fully unrolled over the
+                // tile it was fetched from memory for every short call).
+                auto hide = [&](int q, uint32_t (&rr)[32]) {
+                    if (!whole) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        float x = f[0] != 0.f ? f[0] * __uint_as_float(r0[i]) : 0.f;
-                        if (n_tiles > 1 && f[1] != 0.f) x += f[1] * __uint_as_float(r1[i]);
-                        r0[i] = __float_as_uint(x);
+                        for (int i = 0; i < 32; ++i) {
+                            const int key = key0 + q * 32 + i;
+                            if (!row_valid || key < lo || key >= it.key_hi) rr[i] = 0xff800000u;   // -inf
+                        }
+                    }
+                };
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int q = 0; q < BN / 32; ++q) {
+                    uint32_t rr[32];
+                    tmem_ld32(s_col + q * 32, rr);
+                    tmem_ld_wait();
+                    hide(q, rr);
+                    float pm[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        pm[i] = fmaxf(__uint_as_float(rr[2 * i]), __uint_as_float(rr[2 * i + 1]));
+#pragma unroll
+                    for (int i = 8; i < 32; i += 8)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            pm[u] =
+                                fmaxf(pm[u], fmaxf(__uint_as_float(rr[i + 2 * u]), __uint_as_float(rr[i + 2 * u + 1])));
+                    mx = fmaxf(mx, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])));
+                }
+                if (cap > 0.f) {   // the cap is monotonic: the maximum's capped score is the capped maximum
+                    if (mx != -INFINITY) mx = cap * tanhf(mx * p.scale * inv_cap) * kLog2e;
+                } else {
+                    mx *= mul;
+                }
+                // The reference m of a row is the first maximum it meets; it moves only when a
+                // maximum passes it by more than 2^8 (P stays below 256 in fp16), so O is rescaled
+                // rarely.  NaN scores keep m and reach P.
+                const bool fresh = m == -INFINITY;
+                const bool move = mx > m + kMoveLog2 || (fresh && mx != -INFINITY);
+                if (j >= NG && __any_sync(0xffffffffu, move && !fresh)) {
+                    const float f = move && !fresh ? fast_exp2f(m - mx) : 1.f;
+                    l *= f;
+                    // O holds the earlier tiles' P V: scale it once they are complete
+                    ok = mbar_wait_warp(smem_u32(&bars->o_done[wg]), (g / NG - 1) & 1, p.err, kErrWaitMma);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int q = 0; q < HD / 32; ++q) {
+                        uint32_t ro[32];
+                        tmem_ld32(o_col + q * 32, ro);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) ro[i] = __float_as_uint(__uint_as_float(ro[i]) * f);
+                        tmem_st32(o_col + q * 32, ro);
                     }
                 }
-                if (row_valid) {
+                if (move) m = mx;
+                const float negm = m != -INFINITY ? -m : 0.f;
+                // P over S, in place by groups: columns 32q .. 32q+15 take the fp16 pairs of the
+                // group's 32 keys, 32q+16 .. 32q+31 what their rounding left (PT == 2).
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+                for (int q = 0; q < BN / 32; ++q) {
+                    uint32_t rr[32];
+                    tmem_ld32(s_col + q * 32, rr);
+                    tmem_ld_wait();
+                    if (cap > 0.f) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4 *>(dst + c0 + i) = make_uint4(r0[i], r0[i + 1], r0[i + 2], r0[i + 3]);
+                        for (int i = 0; i < 32; ++i)
+                            rr[i] = __float_as_uint(cap * tanhf(__uint_as_float(rr[i]) * p.scale * inv_cap) * kLog2e);
+                    }
+                    hide(q, rr);
+                    uint32_t w[32];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float e0 = fast_exp2f(fmaf(__uint_as_float(rr[2 * i]), mul, negm));
+                        const float e1 = fast_exp2f(fmaf(__uint_as_float(rr[2 * i + 1]), mul, negm));
+                        acc[i & 3] += e0 + e1;
+                        if (PT == 2) split_f16(e0, e1, w[i], w[16 + i]);
+                        else w[i] = pack_f16x2(e0, e1), w[16 + i] = 0u;
+                    }
+                    tmem_st32(s_col + q * 32, w);
+                }
+                l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+                // Rows of the V tile past the part's last key may hold anything (another
+                // sequence's rows, unwritten memory): 0 * NaN would reach O, so they are zeroed.
+                if (nv < BN) {
+                    ok = mbar_wait_warp(smem_u32(&bars->v_full[g % ST]), (g / ST) & 1, p.err, kErrWaitTmaFull);
+                    if (!ok) break;
+                    uint8_t *vt = sV + (g % ST) * S::kKvBytes;
+                    for (int i = tid; i < (BN - nv) * 8 * S::kSub; i += kBM) {
+                        const int sub = i / ((BN - nv) * 8), u = i % ((BN - nv) * 8);
+                        *reinterpret_cast<uint4 *>(vt + sub * S::kKvSubBytes + nv * 128 + u * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(smem_u32(&bars->p_full[sb]));
+            }
+            // o_done may be two phases behind here (a parity wait could not tell), hence o_final
+            if (ok) ok = mbar_wait_warp(smem_u32(&bars->o_final), n_items & 1, p.err, kErrWaitMma);
+            if (!ok) m = -INFINITY, l = 0.f;   // the part counts as empty
+            tc_fence_after();
+            float M = m, f[2] = {1.f, 0.f};   // the row's reference, and each warpgroup's factor to it
+            bool have[2] = {true, false};     // whether a warpgroup had tiles
+            if (NG == 2) {
+                float2 *ml = reinterpret_cast<float2 *>(smem);   // Q is no longer needed
+                ml[wg * kBM + tid] = make_float2(m, l);
+                named_bar_sync(1, S::kSoftmax);
+                const float2 a = ml[tid], d = ml[kBM + tid];
+                M = fmaxf(a.x, d.x);
+                f[0] = a.x == -INFINITY ? 0.f : fast_exp2f(a.x - M);
+                f[1] = d.x == -INFINITY ? 0.f : fast_exp2f(d.x - M);
+                l = f[0] * a.y + f[1] * d.y;
+                have[0] = it.n_tiles > 1 || (g0 & 1) == 0;
+                have[1] = it.n_tiles > 1 || (g0 & 1) == 1;
+                named_bar_sync(1, S::kSoftmax);   // read, before the staging below writes there
+            }
+            if (row_valid && wg == 0) p.part_ml[slot] = make_float2(M, l);
+            if (ok && warp_live) {
+                // O by blocks of 16 columns through shared memory, so that eight rows' 64 bytes go
+                // out at a time (stores of 16 bytes from 32 rows each took 3 us of a part)
+                uint8_t *stage = smem + warp * 2048;
+                long long off[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {   // rows written by this lane: 8 i + lane / 4
+                    const int rr = it.qt * kBM + (warp % 4) * 32 + 8 * i + lane / 4;
+                    const int rb = it.s0 + rr / p.group;
+                    off[i] = rb < it.s1 ? ((static_cast<long long>(rb) * p.n_heads + it.kvh * p.group + rr % p.group) *
+                                               p.slots + it.c) * HD + lane % 4 * 4
+                                        : -1;
+                }
+#pragma unroll 1
+                for (int c0 = wg * (HD / NG); c0 < (wg + 1) * (HD / NG); c0 += 16) {
+                    uint32_t r0[16], r1[16];
+                    tmem_ld16(lane_base + S::kTmO + c0, r0);
+                    if (NG == 2) tmem_ld16(lane_base + S::kTmO + HD + c0, r1);
+                    tmem_wait16(r0);
+                    if (NG == 2) tmem_wait16(r1);
+                    if (NG == 2) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float x = have[0] && f[0] != 0.f ? f[0] * __uint_as_float(r0[i]) : 0.f;
+                            if (have[1] && f[1] != 0.f) x += f[1] * __uint_as_float(r1[i]);
+                            r0[i] = __float_as_uint(x);
+                        }
+                    }
+                    __syncwarp();   // the block before has been read
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        *reinterpret_cast<uint4 *>(stage + lane * 64 + ((u ^ (lane >> 1)) & 3) * 16) =
+                            make_uint4(r0[4 * u], r0[4 * u + 1], r0[4 * u + 2], r0[4 * u + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = 8 * i + lane / 4;
+                        const uint4 v = *reinterpret_cast<const uint4 *>(stage + row * 64 + (((lane % 4) ^ (row >> 1)) & 3) * 16);
+                        if (off[i] >= 0) *reinterpret_cast<uint4 *>(p.part_o + off[i] + c0) = v;
+                    }
                 }
             }
+            tc_fence_before();
+            g0 += it.n_tiles;
+            ++n_items;
         }
-        if (row_valid && wg == 0) p.part_ml[slot] = make_float2(M, l);
-        tc_fence_before();
     }
+    tc_fence_before();
     __syncthreads();
     if (warp == kIssuer) {
         tc_fence_after();
@@ -574,26 +717,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
     using S = SplitShape<HD>;
     constexpr int KSTEPS = HD / 16;
     // After a prefix kernel, whose CTAs have all passed their own wait when this grid starts,
-    // the inputs are complete and nothing here depends on it: the two run side by side, and
-    // this grid only may not end before it (the merge waits for this grid alone).
-    if (p.prefix_slots == 0) griddep_wait();
-    griddep_trigger();
-    const int b = blockIdx.z;
-    const int kvh = blockIdx.y / p.n_qgroups, qg = blockIdx.y % p.n_qgroups;
-    const int c = blockIdx.x;
-    int ks, n;
-    own_range(p, b, ks, n);
-    const int key0 = ks + c * p.chunk;
-    if (key0 >= n) {
-        if (p.prefix_slots > 0) griddep_wait();
-        return;
-    }
-    const int nkeys = min(p.chunk, n - key0);
-    const int ntiles = (nkeys + kKeysPerTile - 1) / kKeysPerTile;
-    const int h_first = kvh * p.group + qg * 8;
-    const int nh = min(8, p.group - qg * 8);
-    const long long row_base = p.seq_row0[b] + key0;
-
+    // the inputs are complete and nothing here depends on it: the two run side by side.  This
+    // grid may not end before it, as the merge waits for this grid alone: the last CTA waits
+    // (if every CTA did, finished ones would hold their SMs until the prefix kernel's end).
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float *qs = reinterpret_cast<float *>(smem + S::kStages * S::kStageBytes);
@@ -608,6 +734,26 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
         fence_mbar_init();
     }
     __syncthreads();
+    if (p.prefix_slots == 0) griddep_wait();
+    griddep_trigger();
+    const bool last_cta =
+        p.prefix_slots > 0 && blockIdx.x + 1 == gridDim.x && blockIdx.y + 1 == gridDim.y && blockIdx.z + 1 == gridDim.z;
+    const int b = blockIdx.z;
+    const int kvh = blockIdx.y / p.n_qgroups, qg = blockIdx.y % p.n_qgroups;
+    const int c = blockIdx.x;
+    const long long seq_row0 = p.seq_row0[b];
+    int ks, n;
+    own_range(p, b, ks, n);
+    const int key0 = ks + c * p.chunk;
+    if (key0 >= n) {
+        if (last_cta) griddep_wait();
+        return;
+    }
+    const int nkeys = min(p.chunk, n - key0);
+    const int ntiles = (nkeys + kKeysPerTile - 1) / kKeysPerTile;
+    const int h_first = kvh * p.group + qg * 8;
+    const int nh = min(8, p.group - qg * 8);
+    const long long row_base = seq_row0 + key0;
 
     if (warp == kConsumerWarps) {
         if (lane == 0) {
@@ -725,11 +871,11 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
             const float mn0 = fmaxf(m_run[0], mb0), mn1 = fmaxf(m_run[1], mb1);
             // a row whose scores are all -inf so far keeps exponentials of exactly 0
             const float n0 = mn0 == -INFINITY ? 0.f : -mn0, n1 = mn1 == -INFINITY ? 0.f : -mn1;
-            const float corr0 = fast_exp2(m_run[0] + n0), corr1 = fast_exp2(m_run[1] + n1);
+            const float corr0 = fast_exp2f(m_run[0] + n0), corr1 = fast_exp2f(m_run[1] + n1);
             m_run[0] = mn0;
             m_run[1] = mn1;
-            const float p0 = fast_exp2(x[0] + n0), p1 = fast_exp2(x[1] + n1);
-            const float p2 = fast_exp2(x[2] + n0), p3 = fast_exp2(x[3] + n1);
+            const float p0 = fast_exp2f(x[0] + n0), p1 = fast_exp2f(x[1] + n1);
+            const float p2 = fast_exp2f(x[2] + n0), p3 = fast_exp2f(x[3] + n1);
             l_run[0] = l_run[0] * corr0 + (p0 + p2);
             l_run[1] = l_run[1] * corr1 + (p1 + p3);
 #pragma unroll
@@ -818,7 +964,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
 #pragma unroll
         for (int w = 0; w < kConsumerWarps; ++w) {
             const float mw = red[(w * 8 + h) * kRowF];
-            const float f = mw == -INFINITY ? 0.f : fast_exp2(mw - M);
+            const float f = mw == -INFINITY ? 0.f : fast_exp2f(mw - M);
             if (f != 0.f) acc += f * red[(w * 8 + h) * kRowF + 2 + d];
             sum += f * red[(w * 8 + h) * kRowF + 1];
         }
@@ -827,126 +973,157 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
         p.part_o[slot * HD + d] = acc;
         if (d == 0) p.part_ml[slot] = make_float2(M, sum);
     }
-    if (p.prefix_slots > 0) griddep_wait();
+    if (last_cta) griddep_wait();
 }
 
 // ===========================================================================
 // merge
 // ===========================================================================
-// CTA = (part of the work of one KV head, KV head, sequence).  The first out_blocks CTAs
-// join 128 outputs of one query head each: warp w takes every 8th part (512 contiguous
-// bytes), then the warps meet in shared memory.  The others, with weights, add the
-// probabilities of kMergeKeys own keys each.  Every warp finds the M and L it needs
-// itself: the (m, l) pairs of a head are few and the warps of a CTA share them in L1.
+// Blocks below out_blocks join outputs: kMergeOuts of a query head by `ways` warps that take
+// the parts in turn (512 contiguous bytes each) and meet in shared memory.  The others, with
+// weights, add the probabilities of kMergeKeys own keys of a KV head each.  A warp finds the
+// M and L it needs itself from the (m, l) of the head's parts.
 constexpr int kMergeThreads = 256;
+constexpr int kMergeWarps = kMergeThreads / 32;
 constexpr int kMergeKeys = 1024;
 constexpr int kMergeOuts = 128;
 
-// M and 1/L of a head whose parts [first, last) have the pairs ml (the whole warp).
-__device__ __forceinline__ void head_sum(const float2 *ml, int first, int last, float &M, float &inv)
+// The slots of sequence b that hold parts: [0, np) of its prefix and [own0, own1) of its own
+// rows (the whole warp).
+struct Parts {
+    int np, own0, own1;
+    __device__ __forceinline__ bool has(int slot) const { return slot < np || (slot >= own0 && slot < own1); }
+};
+__device__ __forceinline__ Parts parts_of(const SharedParams &p, int b, int own_keys)
+{
+    Parts t;
+    t.np = 0;
+    for (int g0 = 0; g0 < p.n_prefixes; g0 += 32) {
+        const int g = g0 + static_cast<int>(threadIdx.x % 32);
+        int mine = 0;
+        if (g < p.n_prefixes) {
+            int s0, s1, len;
+            prefix_range(p, g, s0, s1, len, false);
+            if (b >= s0 && b < s1) mine = prefix_parts_of(p, len);
+        }
+        t.np = max(t.np, __reduce_max_sync(0xffffffffu, mine));
+        if (t.np > 0) break;
+    }
+    t.own0 = p.prefix_slots;
+    t.own1 = p.prefix_slots + (own_keys > 0 ? (own_keys + p.chunk - 1) / p.chunk : 0);
+    return t;
+}
+
+// M and 1/L of a head whose pairs are ml (the whole warp); v: pair `lane`, loaded ahead.
+__device__ __forceinline__ void head_sum(const SharedParams &p, const float2 *ml, float2 v, const Parts &t, float &M,
+                                         float &inv)
 {
     const int lane = threadIdx.x % 32;
     M = -INFINITY;
-    for (int c = first + lane; c < last; c += 32) M = fmaxf(M, ml[c].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     float L = 0.f;
-    for (int c = first + lane; c < last; c += 32) {
-        const float2 v = ml[c];
-        if (v.x != -INFINITY) L += fast_exp2(v.x - M) * v.y;
-    }
+    for (int s0 = 0; s0 < t.own1 || s0 < t.np; s0 += 32) {   // one pass: the sum moves with the maximum
+        if (s0 > 0) v = t.has(s0 + lane) ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
+        if (!t.has(s0 + lane)) v = make_float2(-INFINITY, 0.f);
+        float mx = v.x;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        if (mx == -INFINITY) continue;
+        const float top = fmaxf(M, mx);
+        float s = v.x == -INFINITY ? 0.f : fast_exp2f(v.x - top) * v.y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        L = (M == -INFINITY ? 0.f : L * fast_exp2f(M - top)) + s;
+        M = top;
+    }
     inv = L != 0.f ? 1.f / L : 0.f;   // NaN stays NaN
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ SharedParams p)
+__global__ void __launch_bounds__(kMergeThreads, 4) merge_kernel(const __grid_constant__ SharedParams p, int ways, int out_blocks)
 {
     griddep_wait();
     griddep_trigger();
-    const int b = blockIdx.z, kvh = blockIdx.y;
-    int ks, n;
-    own_range(p, b, ks, n);
-    const int out_blocks = (p.group * HD + kMergeOuts - 1) / kMergeOuts;
-    const int j0 = (static_cast<int>(blockIdx.x) - out_blocks) * kMergeKeys;
-    if (j0 >= 0 && j0 >= n) return;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0 && (p.kv_len[b] > p.max_kv_len || p.kv_len[b] < 0))
-        atomicOr(p.err, kErrBadArgs);
-    // whether the sequence has a prefix (its parts were then all written)
-    bool has_prefix = false;
-    for (int g = lane; g < p.n_prefixes; g += 32) {
-        int s0, s1, len;
-        prefix_range(p, g, s0, s1, len, false);
-        has_prefix |= b >= s0 && b < s1;
-    }
-    has_prefix = __any_sync(0xffffffffu, has_prefix);
-    const int first = has_prefix ? 0 : p.prefix_slots;
-    const int last = p.prefix_slots + (n > ks ? (n - ks + p.chunk - 1) / p.chunk : 0);
-    const long long row0 = static_cast<long long>(b) * p.n_heads + kvh * p.group;
-
-    if (j0 < 0) {
-        // four outputs per lane; head dim 64: two heads per CTA
+    if (static_cast<int>(blockIdx.x) < out_blocks) {
+        // unit u: 128 outputs from element 128 u of the output on (head dim 64: of two heads)
         __shared__ float4 red[kMergeThreads];
-        const int e = blockIdx.x * kMergeOuts + lane * 4;
-        constexpr int kHeads = HD < kMergeOuts ? kMergeOuts / HD : 1;   // heads in this CTA
-        const int h0 = blockIdx.x * kMergeOuts / HD;
-        float M = -INFINITY, inv = 0.f;
+        const long long u = static_cast<long long>(blockIdx.x) * (kMergeWarps / ways) + warp / ways;
+        const long long row_elems = static_cast<long long>(p.n_heads) * HD;
+        const long long e = u * kMergeOuts + lane * 4;      // this lane's first output
+        const bool live = e < row_elems * p.n_seqs;
+        const int way = warp % ways;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        float inv = 0.f;
+        constexpr int kHeads = HD < kMergeOuts ? kMergeOuts / HD : 1;   // heads of a unit
+        const long long head0 = u * kMergeOuts / HD;                   // its first (sequence, head)
 #pragma unroll
         for (int i = 0; i < kHeads; ++i) {
-            if (h0 + i >= p.group) break;
-            float Mi, invi;
-            head_sum(p.part_ml + (row0 + h0 + i) * p.slots, first, last, Mi, invi);
-            if (e / HD == h0 + i) M = Mi, inv = invi;
-        }
-        const bool live = e / HD < p.group;
-        const float2 *ml = p.part_ml + (row0 + e / HD) * p.slots;
-        const float *src = p.part_o + (row0 + e / HD) * p.slots * HD + e % HD;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        constexpr int kLoad = 4, kWarps = kMergeThreads / 32;   // parts in flight, parts side by side
-        for (int c0 = first + warp; live && c0 < last; c0 += kLoad * kWarps) {
-            float f[kLoad];
-            float4 v[kLoad];
+            const long long hs = head0 + i;
+            if (hs >= static_cast<long long>(p.n_seqs) * p.n_heads) break;
+            const int b = static_cast<int>(hs / p.n_heads);
+            const float2 *ml = p.part_ml + hs * p.slots;
+            // in flight while the sequence's parts are found (a slot without one is not used)
+            const float2 ahead = lane < p.slots ? ml[lane] : make_float2(-INFINITY, 0.f);
+            int ks, n;
+            own_range(p, b, ks, n);
+            if (lane == 0 && way == 0 && hs % p.n_heads == 0 && p.kv_len[b] != n) atomicOr(p.err, kErrBadArgs);
+            const Parts t = parts_of(p, b, n - ks);
+            float M, my_inv;
+            head_sum(p, ml, ahead, t, M, my_inv);
+            if (e / HD != hs) continue;   // (a half-warp at head dim 64)
+            inv = my_inv;
+            const float *src = p.part_o + hs * p.slots * HD + e % HD;
+            constexpr int kLoad = 4;   // parts in flight
+            for (int c0 = way; c0 < t.own1 || c0 < t.np; c0 += kLoad * ways) {
+                float f[kLoad];
+                float4 v[kLoad];
 #pragma unroll
-            for (int i = 0; i < kLoad; ++i) {
-                const int c = c0 + i * kWarps;
-                f[i] = c < last ? ml[c].x : -INFINITY;
+                for (int k = 0; k < kLoad; ++k) f[k] = t.has(c0 + k * ways) ? ml[c0 + k * ways].x : -INFINITY;
+#pragma unroll
+                for (int k = 0; k < kLoad; ++k) {   // an empty part has no output written
+                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (f[k] != -INFINITY)
+                        v[k] = *reinterpret_cast<const float4 *>(src + static_cast<long long>(c0 + k * ways) * HD);
+                    f[k] = f[k] != -INFINITY ? fast_exp2f(f[k] - M) : 0.f;
+                }
+#pragma unroll
+                for (int k = 0; k < kLoad; ++k)
+                    a.x += f[k] * v[k].x, a.y += f[k] * v[k].y, a.z += f[k] * v[k].z, a.w += f[k] * v[k].w;
             }
-#pragma unroll
-            for (int i = 0; i < kLoad; ++i) {   // an empty part has no output written
-                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (f[i] != -INFINITY)
-                    v[i] = *reinterpret_cast<const float4 *>(src + static_cast<long long>(c0 + i * kWarps) * HD);
-                f[i] = f[i] != -INFINITY ? fast_exp2(f[i] - M) : 0.f;
+        }
+        if (ways > 1) {
+            red[threadIdx.x] = a;
+            __syncthreads();
+            if (way != 0) return;
+            for (int w = 1; w < ways; ++w) {
+                const float4 v = red[threadIdx.x + 32 * w];
+                a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
             }
-#pragma unroll
-            for (int i = 0; i < kLoad; ++i)
-                a.x += f[i] * v[i].x, a.y += f[i] * v[i].y, a.z += f[i] * v[i].z, a.w += f[i] * v[i].w;
         }
-        red[threadIdx.x] = a;
-        __syncthreads();
-        if (warp != 0 || !live) return;
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) {
-            const float4 v = red[w * 32 + lane];
-            a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
-        }
+        if (!live) return;
         a.x *= inv, a.y *= inv, a.z *= inv, a.w *= inv;
-        const long long at = row0 * HD + e;
         if (p.out_is_bf16)
-            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) =
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + e) =
                 make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
         else
-            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = a;
+            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + e) = a;
         return;
     }
+    const int key_blocks = (p.max_kv_len + kMergeKeys - 1) / kMergeKeys;
+    const long long wb = blockIdx.x - out_blocks;
+    const int j0 = static_cast<int>(wb % key_blocks) * kMergeKeys;
+    const long long own = wb / key_blocks;   // (sequence, KV head)
+    const int b = static_cast<int>(own / p.n_kv_heads), kvh = static_cast<int>(own % p.n_kv_heads);
+    const long long row0 = static_cast<long long>(b) * p.n_heads + kvh * p.group;
+    const float2 *ml = p.part_ml + (row0 + warp) * p.slots;   // of the first eight heads
+    const float2 ahead = warp < p.group && lane < p.slots ? ml[lane] : make_float2(-INFINITY, 0.f);
+    int ks, n;
+    own_range(p, b, ks, n);
+    if (j0 >= n) return;
+    const Parts t = parts_of(p, b, n - ks);
     __shared__ float s_M[8], s_inv[8];
     constexpr int kPer = kMergeKeys / kMergeThreads;
-    float w[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) w[i] = 0.f;
-    const long long own = static_cast<long long>(b) * p.n_kv_heads + kvh;
+    float w[kPer], w_in[kPer];
     auto load_pair = [&](const float *sc, int h, float2 (&x)[kPer]) {   // score_cols is even: 8-byte loads
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -955,10 +1132,10 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
                                     : make_float2(-INFINITY, -INFINITY);
         }
     };
-    float w_in[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int j = j0 + i * kMergeThreads + static_cast<int>(threadIdx.x);
+        w[i] = 0.f;
         w_in[i] = p.weights_in && j < n ? p.weights_in[own * p.weights_stride + j] : 0.f;
     }
     for (int h0 = 0; h0 < p.group; h0 += 8) {
@@ -967,8 +1144,9 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
         float2 x[kPer];
         load_pair(sc, 0, x);   // in flight while the sums are found
         if (warp < nh) {
+            const float2 *mine = ml + static_cast<long long>(h0) * p.slots;
             float M, inv;
-            head_sum(p.part_ml + (row0 + h0 + warp) * p.slots, first, last, M, inv);
+            head_sum(p, mine, h0 == 0 ? ahead : lane < p.slots ? mine[lane] : make_float2(-INFINITY, 0.f), t, M, inv);
             if (lane == 0) s_M[warp] = M, s_inv[warp] = inv;
         }
         __syncthreads();
@@ -976,8 +1154,8 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
             if (h > 0) load_pair(sc, h, x);
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                if (x[i].x != -INFINITY) w[i] += fast_exp2(x[i].x - s_M[h]) * s_inv[h];
-                if (h + 1 < nh && x[i].y != -INFINITY) w[i] += fast_exp2(x[i].y - s_M[h + 1]) * s_inv[h + 1];
+                if (x[i].x != -INFINITY) w[i] += fast_exp2f(x[i].x - s_M[h]) * s_inv[h];
+                if (h + 1 < nh && x[i].y != -INFINITY) w[i] += fast_exp2f(x[i].y - s_M[h + 1]) * s_inv[h + 1];
             }
         }
         __syncthreads();
@@ -1030,6 +1208,26 @@ int prefix_parts(int n_prefixes, int max_prefix_len, int max_prefix_seqs, int n_
     return parts < least ? least : parts < most ? parts : most;
 }
 
+// CTAs of the prefix kernel: every SM, or half of them where the own rows have enough to do
+// beside it -- the split kernel keeps HBM busy from the other half while the prefix kernel,
+// bound by its products and exponentials, works (64 sequences on 8192 shared and 100 to 1024
+// own keys: 52.9 us with all SMs, 48.3 with half; four prefixes, 200 sequences: 233 and 207).
+// SMOL_PREFIX_CTAS in the environment overrides it (measurement knob).
+const int g_prefix_ctas = [] {
+    const char *e = getenv("SMOL_PREFIX_CTAS");
+    return e ? atoi(e) : 0;
+}();
+int prefix_ctas(const SharedParams &p, int hd)
+{
+    if (g_prefix_ctas > 0 && g_prefix_ctas <= kSms) return g_prefix_ctas;
+    // bytes of own rows if half of the bound is used, against those a prefix kernel on all
+    // SMs reads in the same time: about 20 us per 512 KB part
+    const double own_us = 0.5 * p.n_seqs * p.max_kv_len * 4.0 * p.n_kv_heads * hd / 6.3e6;
+    const double part_us = 5.0 + p.prefix_chunk * 4.0 * hd / 512e3 * 15.0;
+    const double prefix_us = static_cast<double>(p.prefix_items) / kSms * part_us;
+    return own_us > 0.5 * prefix_us ? kSms / 2 : kSms;
+}
+
 struct SharedLayout {
     size_t part_ml, scores, total;   // part_o at 0
 };
@@ -1075,30 +1273,41 @@ template <int HD, int QT, int PT>
 int launch_shared(cudaStream_t st, SharedParams &p, const uint16_t *k_pool, const uint16_t *v_pool, int64_t pool_rows)
 {
     const int kv_dim = p.n_kv_heads * HD;
+    auto maps = [&](int rows) {
+        return make_tmap_2d(&p.tk, k_pool, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv_dim, pool_rows, 64, rows) &&
+               make_tmap_2d(&p.tv, v_pool, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kv_dim, pool_rows, 64, rows);
+    };
+    int box_rows = 0;   // of the maps in p
     if (p.prefix_slots > 0) {
         using S = PrefixShape<HD, QT>;
-        if (!make_tmap_2d(&p.tk, k_pool, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv_dim, pool_rows, 64, S::BN) ||
-            !make_tmap_2d(&p.tv, v_pool, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kv_dim, pool_rows, 64, S::BN) ||
+        if (!maps(box_rows = S::kBoxRows) ||
             !allow_smem(reinterpret_cast<const void *>(prefix_kernel<HD, QT, PT>), S::kSmemBytes))
             return SMOL_B200_ERR_CUDA;
-        const dim3 grid(div_up(static_cast<long long>(p.max_prefix_seqs) * p.group, kBM),
-                        p.n_kv_heads * p.prefix_slots, p.n_prefixes);
+        const int at_most = prefix_ctas(p, HD);
+        const dim3 grid(static_cast<unsigned>(p.prefix_items < at_most ? p.prefix_items : at_most));
         if (launch_kernel(prefix_kernel<HD, QT, PT>, grid, dim3(S::kThreads), S::kSmemBytes, st, p) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
     }
     if (p.max_kv_len > 0) {
         using S = SplitShape<HD>;
-        if (!make_tmap_2d(&p.tk, k_pool, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv_dim, pool_rows, 64, kKeysPerTile) ||
-            !make_tmap_2d(&p.tv, v_pool, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kv_dim, pool_rows, 64, kKeysPerTile) ||
+        if ((box_rows != kKeysPerTile && !maps(kKeysPerTile)) ||
             !allow_smem(reinterpret_cast<const void *>(split_kernel<HD, QT, PT>), S::kSmemBytes))
             return SMOL_B200_ERR_CUDA;
         const dim3 grid(p.max_chunks, p.n_kv_heads * p.n_qgroups, p.n_seqs);
         if (launch_kernel(split_kernel<HD, QT, PT>, grid, dim3(kSplitThreads), S::kSmemBytes, st, p) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
     }
-    const int blocks = div_up(p.group * HD, kMergeOuts) + (p.scores ? div_up(p.max_kv_len, kMergeKeys) : 0);
-    if (launch_kernel(merge_kernel<HD>, dim3(blocks, p.n_kv_heads, p.n_seqs), dim3(kMergeThreads), 0, st, p) !=
-        cudaSuccess)
+    // Warps per 128 outputs: one where that fills the GPU with warps, up to eight (and a part
+    // each) where a row's parts would otherwise be read one after another.
+    const long long units = (static_cast<long long>(p.n_seqs) * p.n_heads * HD + kMergeOuts - 1) / kMergeOuts;
+    int ways = 1;
+    while (ways < kMergeWarps && units * ways < kSms * kMergeWarps && 2 * ways < p.slots) ways *= 2;
+    const long long out_blocks = (units * ways + kMergeWarps - 1) / kMergeWarps;
+    const long long key_blocks =
+        p.scores ? static_cast<long long>(div_up(p.max_kv_len, kMergeKeys)) * p.n_seqs * p.n_kv_heads : 0;
+    if (out_blocks + key_blocks > 0x7fffffffLL) return SMOL_B200_ERR_ARGS;
+    if (launch_kernel(merge_kernel<HD>, dim3(static_cast<unsigned>(out_blocks + key_blocks)), dim3(kMergeThreads), 0, st, p,
+                      ways, static_cast<int>(out_blocks)) != cudaSuccess)
         return SMOL_B200_ERR_CUDA;
     return SMOL_B200_OK;
 }
@@ -1165,7 +1374,10 @@ int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const v
     p.max_chunks = max_kv_len > 0 ? div_up(max_kv_len, p.chunk) : 0;
     p.prefix_slots = prefix_parts(n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads);
     if (p.prefix_slots > 0) p.prefix_chunk = (div_up(max_prefix_len, p.prefix_slots) + 63) / 64 * 64;
-    if (static_cast<long long>(n_kv_heads) * p.prefix_slots > 65535) return SMOL_B200_ERR_ARGS;
+    p.prefix_qtiles = div_up(static_cast<long long>(max_prefix_seqs) * p.group, kBM);
+    const long long items = static_cast<long long>(p.prefix_qtiles) * p.prefix_slots * n_kv_heads * n_prefixes;
+    if (items > 0x7fffff00LL) return SMOL_B200_ERR_ARGS;
+    p.prefix_items = static_cast<int>(items);
     p.slots = p.prefix_slots + p.max_chunks;
     if (p.slots < 1) p.slots = 1;
     const size_t need = decode_shared_workspace_bytes(n_seqs, max_kv_len, n_prefixes, max_prefix_len, max_prefix_seqs,

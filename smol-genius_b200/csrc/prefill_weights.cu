@@ -315,6 +315,12 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
             *reinterpret_cast<uint4 *>(smem + i * 16) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
     }
+    WRun w = find_run<HD, MODE>(p, blockIdx.x);
+    // Everything above is the kernel's own and may run while the kernels before this one finish.
+    // TMEM only after the wait: a CTA that held it while an earlier kernel's CTA on the same SM
+    // still had to allocate would wait for that kernel for good.
+    griddep_wait();
+    griddep_trigger();
     if (warp == kIssuer) {
         tmem_alloc(smem_u32(&bars->tmem_base), 512);
         tmem_relinquish();
@@ -323,10 +329,6 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = bars->tmem_base;
-    WRun w = find_run<HD, MODE>(p, blockIdx.x);
-    // everything above is the kernel's own: it may run while the kernels before this one finish
-    griddep_wait();
-    griddep_trigger();
 
     if (warp == kProducer) {
         // ================= TMA producer =================

@@ -183,6 +183,14 @@ def _ptr(x) -> int | None:
     return x.data_ptr()
 
 
+def _torch_stream(torch) -> int:
+    """Handle of torch's current stream; without building a Stream object (3 us a call) where torch allows it."""
+    try:
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    except AttributeError:
+        return torch.cuda.current_stream().cuda_stream
+
+
 def _stream(stream) -> int | None:
     """The CUDA stream handle to launch on.  None means torch's current stream when
     torch has initialised CUDA in this process (so calls inside `torch.cuda.stream(s)`
@@ -191,7 +199,7 @@ def _stream(stream) -> int | None:
     if stream is None:
         torch = sys.modules.get("torch")
         if torch is not None and torch.cuda.is_initialized():
-            return torch.cuda.current_stream().cuda_stream or None
+            return _torch_stream(torch) or None
         return None
     if isinstance(stream, int):
         return stream
@@ -552,6 +560,11 @@ def layer_norm(out, x, w, b, rows, hidden, eps, out_bf16=False, stream=None):
 # ---------------------------------------------------------------------------
 # Part 6: shared prefixes, attention weights, eviction
 # ---------------------------------------------------------------------------
+def _dev(t) -> int | None:
+    """Address of a tensor (None -> NULL); what _ptr does, for tensors alone."""
+    return None if t is None else t.data_ptr()
+
+
 def decode_shared_workspace_bytes(n_seqs, max_kv_len, n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads,
                                   head_dim) -> int:
     return lib().smol_b200_decode_shared_workspace_bytes(n_seqs, max_kv_len, n_prefixes, max_prefix_len,
@@ -566,12 +579,13 @@ def decode_attention_shared(out, q, k_pool, v_pool, pool_rows, prefix_row0, pref
     [n_prefixes], prefix_seq0 int32 [n_prefixes + 1]; weights fp32 [n_seqs, n_kv_heads, weights_stride] or None."""
     import torch
     rc = lib().smol_b200_decode_attention_shared(
-        _stream(stream), _ptr(out), int(out.dtype == torch.bfloat16), _ptr(q), int(q.dtype == torch.bfloat16),
-        _ptr(k_pool), _ptr(v_pool), pool_rows, _ptr(prefix_row0), _ptr(prefix_len), _ptr(prefix_seq0), n_prefixes,
-        max_prefix_len, max_prefix_seqs, _ptr(seq_row0), _ptr(kv_len), n_seqs, max_kv_len, n_heads, n_kv_heads,
-        head_dim, scale, window, softcap, _ptr(weights_in), _ptr(weights_out), weights_stride, _ptr(workspace),
-        workspace.numel() * workspace.element_size())
-    check(rc, "smol_b200_decode_attention_shared")
+        _stream(stream), _dev(out), out.dtype == torch.bfloat16, _dev(q), q.dtype == torch.bfloat16,
+        _dev(k_pool), _dev(v_pool), pool_rows, _dev(prefix_row0), _dev(prefix_len), _dev(prefix_seq0), n_prefixes,
+        max_prefix_len, max_prefix_seqs, _dev(seq_row0), _dev(kv_len), n_seqs, max_kv_len, n_heads, n_kv_heads,
+        head_dim, scale, window, softcap, _dev(weights_in), _dev(weights_out), weights_stride, _dev(workspace),
+        workspace.nbytes)
+    if rc:
+        check(rc, "smol_b200_decode_attention_shared")
 
 
 def decode_weights_workspace_bytes(n_seqs, max_kv_len, n_heads, n_kv_heads, head_dim) -> int:
@@ -585,10 +599,10 @@ def decode_attention_weights(out, q, k_pool, v_pool, pool_rows, seq_row0, kv_len
     head) to weights_in (None: zero), into weights_out (may be weights_in)."""
     import torch
     rc = lib().smol_b200_decode_attention_weights(
-        _stream(stream), _ptr(out), int(out.dtype == torch.bfloat16), _ptr(q), int(q.dtype == torch.bfloat16),
-        _ptr(k_pool), _ptr(v_pool), pool_rows, _ptr(seq_row0), _ptr(kv_len), n_seqs, max_kv_len, n_heads, n_kv_heads,
-        head_dim, scale, window, softcap, _ptr(weights_in), _ptr(weights_out), weights_stride, _ptr(workspace),
-        workspace.numel() * workspace.element_size())
+        _stream(stream), _dev(out), out.dtype == torch.bfloat16, _dev(q), q.dtype == torch.bfloat16,
+        _dev(k_pool), _dev(v_pool), pool_rows, _dev(seq_row0), _dev(kv_len), n_seqs, max_kv_len, n_heads, n_kv_heads,
+        head_dim, scale, window, softcap, _dev(weights_in), _dev(weights_out), weights_stride, _dev(workspace),
+        workspace.nbytes)
     check(rc, "smol_b200_decode_attention_weights")
 
 
@@ -606,9 +620,9 @@ def prefill_attention_weights(weights_in, weights_out, weights_stride, q, k, bat
         strides = ((qw, seq_q * qw), (kw, seq_k * kw))
     (qrs, qbs), (krs, kbs) = strides
     rc = lib().smol_b200_prefill_attention_weights(
-        _stream(stream), _ptr(weights_in), _ptr(weights_out), weights_stride, _ptr(q), qrs, qbs, _ptr(k), krs, kbs,
+        _stream(stream), _dev(weights_in), _dev(weights_out), weights_stride, _dev(q), qrs, qbs, _dev(k), krs, kbs,
         batch, seq_q, seq_k, n_heads, n_kv_heads, head_dim, scale, mask_kind, q_offset, prefix_len, window, softcap,
-        _ptr(workspace), workspace.numel() * workspace.element_size())
+        _dev(workspace), workspace.nbytes)
     check(rc, "smol_b200_prefill_attention_weights")
 
 
@@ -621,8 +635,8 @@ def cache_evict(k_pool, v_pool, pool_rows, seq_row0, weights_in, weights_out, po
                 workspace, stream=None):
     """Weights fp32 and positions int32 [n_seqs, n_kv_heads, stride]; each output may be its input."""
     rc = lib().smol_b200_cache_evict(
-        _stream(stream), _ptr(k_pool), _ptr(v_pool), pool_rows, _ptr(seq_row0), _ptr(weights_in), _ptr(weights_out),
-        _ptr(positions_in), _ptr(positions_out), stride, _ptr(kv_len_in), _ptr(kv_len_out), _ptr(seq_pos), n_seqs,
-        max_kv_len, n_kv_heads, head_dim, budget, sink, recent, _ptr(workspace),
-        workspace.numel() * workspace.element_size())
+        _stream(stream), _dev(k_pool), _dev(v_pool), pool_rows, _dev(seq_row0), _dev(weights_in), _dev(weights_out),
+        _dev(positions_in), _dev(positions_out), stride, _dev(kv_len_in), _dev(kv_len_out), _dev(seq_pos), n_seqs,
+        max_kv_len, n_kv_heads, head_dim, budget, sink, recent, _dev(workspace),
+        workspace.nbytes)
     check(rc, "smol_b200_cache_evict")
