@@ -10,7 +10,10 @@
 //          a single row tile the roles of the two operands in the products change: the
 //          rows stay in shared memory, key tiles stream and each is complete by itself.
 // The probabilities themselves are never stored.  Bound: two exponentials per visible
-// (row, key) pair at 16 per clock and SM; a tile's products take half as long.
+// (row, key) pair at 16 per clock and SM, 60 us for 4096 causal rows of 16/8 heads of 128,
+// which take 106; a pass's products alone take 800 clocks a 128 x 128 tile, its exponentials
+// 1000, one waits for the other for 1100 to 1360.  (256-column products, two buffers of S in
+// turn: 120 us.)
 //
 // One persistent CTA per SM.  The visible tiles of all staying tiles, laid end to end, are cut
 // into one contiguous run per CTA, so that causal work spreads evenly (whole items of up to
@@ -141,12 +144,10 @@ __host__ __device__ __forceinline__ void stream_range(const WParams &p, int mode
 }
 
 // acc += 2^(v*mul + off) for 16 columns.  MUFU takes 16 cycles of a scheduler for a pair, the
-// FMA pipe 4 for its product and sum and 16 more for a polynomial: kPoly of every 8 pairs go
-// there.
-#ifndef SMOL_WEIGHTS_POLY
-#define SMOL_WEIGHTS_POLY 2
-#endif
-constexpr int kPoly = SMOL_WEIGHTS_POLY;
+// FMA pipe 4 for its product and sum and 16 more for a polynomial.  kPoly of every 8 pairs go
+// there: 111.5 us with 0, 106.3 with 1, 106.5 with 2, 108.8 with 3 (4096 causal rows, 16/8 heads
+// of 128).
+constexpr int kPoly = 1;
 template <typename Off>
 __device__ __forceinline__ void add_exp2(const uint32_t (&v)[16], f32x2 mul2, Off &&off, f32x2 &acc0, f32x2 &acc1)
 {
@@ -159,10 +160,16 @@ __device__ __forceinline__ void add_exp2(const uint32_t (&v)[16], f32x2 mul2, Of
     }
 }
 
-// Changing the staying tiles costs about as much as kStepCost streaming tiles (1.7 us against
-// 1.45 us a tile, head dim 128), so a step counts that many more, in front of its own, when
-// the runs are cut.
-constexpr int kStepCost = 1;
+// A staying step costs its CTA time beside its tiles: loads that nothing hides, and for causal
+// rows the tiles on the mask's border.  When the runs are cut it counts as this many streaming
+// tiles more, in front of its own (fits of the time of each CTA's run, in clocks: stats 2194 a
+// tile and 4590 a step, sums 2725 and 786, head dim 128; one row tile: stats 412 and 4638, sums
+// 890 and 4369).  4096 causal rows, 16/8 heads: 110.7 us with 1 for all, 106.0 so; 32 rows
+// against 16384 keys: 22.2 and 19.4.
+__host__ __device__ constexpr int step_cost(int mode)
+{
+    return mode == kStats ? 2 : mode == kSums ? 1 : mode == kStatsOneRowTile ? 8 : 5;
+}
 
 // One CTA's run, staying step by staying step: step x of unit (b, kvh) against streaming tiles
 // [t0, t0 + n), as piece `piece` of that step.
@@ -189,11 +196,11 @@ __device__ __forceinline__ bool run_step(const WParams &p, WRun &w)
         }
         int t0, t1;
         stream_range(p, MODE, WShape<HD, MODE>::kStay, w.x, t0, t1);
-        const long long size = t1 > t0 ? t1 - t0 + kStepCost : 0;
+        const long long size = t1 > t0 ? t1 - t0 + step_cost(MODE) : 0;
         const long long end = min(size, w.skip + w.left);   // the run's share of the step: [skip, end)
-        const int first = static_cast<int>(max(w.skip - kStepCost, 0ll));
+        const int first = static_cast<int>(max(w.skip - step_cost(MODE), 0ll));
         w.t0 = t0 + first;
-        w.n = static_cast<int>(max(end - kStepCost, 0ll)) - first;
+        w.n = static_cast<int>(max(end - step_cost(MODE), 0ll)) - first;
         w.left -= end - w.skip;
         if (w.n > 0) return true;
         run_next(w);
@@ -218,7 +225,7 @@ __device__ WRun find_run(const WParams &p, int cta)
     for (int x0 = 0; x0 < p.stay; x0 += 32) {
         int t0 = 0, t1 = 0;
         if (x0 + lane < p.stay) stream_range(p, MODE, WShape<HD, MODE>::kStay, x0 + lane, t0, t1);
-        const int mine = t1 > t0 ? t1 - t0 + kStepCost : 0;
+        const int mine = t1 > t0 ? t1 - t0 + step_cost(MODE) : 0;
         int sum = mine;   // inclusive within the warp
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -232,7 +239,7 @@ __device__ WRun find_run(const WParams &p, int cta)
             const long long f = __shfl_sync(0xffffffffu, first, l);
             w.x = x0 + l;
             w.skip = in_unit - f;
-            w.piece = cta - static_cast<int>((w.unit * p.unit_tiles + f + kStepCost) / p.run);
+            w.piece = cta - static_cast<int>((w.unit * p.unit_tiles + f + step_cost(MODE)) / p.run);
             return w;
         }
         before += __shfl_sync(0xffffffffu, sum, 31);
@@ -255,13 +262,13 @@ __device__ int step_pieces(const WParams &p, int mode, int kstay, int unit, int 
     for (int i = threadIdx.x; i < x; i += blockDim.x) {
         int t0, t1;
         stream_range(p, mode, kstay, i, t0, t1);
-        if (t1 > t0) sum += t1 - t0 + kStepCost;
+        if (t1 > t0) sum += t1 - t0 + step_cost(mode);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (threadIdx.x % 32 == 0) s_sum[threadIdx.x / 32] = sum;
     __syncthreads();
-    long long f = unit * p.unit_tiles + kStepCost;
+    long long f = unit * p.unit_tiles + step_cost(mode);
     for (int i = 0; i < static_cast<int>(blockDim.x / 32); ++i) f += s_sum[i];
     int t0, t1;
     stream_range(p, mode, kstay, x, t0, t1);
@@ -578,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                     one_slot ^= 1;
                     int t0, t1;
                     stream_range(p, kStatsOneRowTile, 1, 0, t0, t1);
-                    const int pieces = pieces_at(w.unit * p.stat_unit_tiles + kStepCost, t1 - t0, p.stat_run);
+                    const int pieces = pieces_at(w.unit * p.stat_unit_tiles + step_cost(kStatsOneRowTile), t1 - t0, p.stat_run);
                     const int row = threadIdx.x / 4, part = threadIdx.x % 4;
                     const float2 *src = p.stat_parts + (unit * rows + row) * p.stat_pieces;
                     float M = -INFINITY, L = 0.f;
@@ -772,7 +779,7 @@ int launch_pass(cudaStream_t st, WParams &p, int stay, int stream, int most, int
     for (int x = 0; x < stay; ++x) {
         int t0, t1;
         stream_range(p, MODE, S::kStay, x, t0, t1);
-        if (t1 > t0) p.unit_tiles += t1 - t0 + kStepCost;
+        if (t1 > t0) p.unit_tiles += t1 - t0 + step_cost(MODE);
     }
     const long long all = p.unit_tiles * p.batch * p.n_kv_heads;
     const int sms = sm_count();
