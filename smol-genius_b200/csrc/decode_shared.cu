@@ -7,7 +7,8 @@
 // kernels do one step:
 //   prefix  the rows of a shared prefix against the query heads of ALL its sequences, on
 //           tcgen05: a 128-row tile holds (sequence, head of the KV group) pairs, so a
-//           prefix row is read once per tile instead of once per sequence;
+//           prefix row is read once per tile instead of once per sequence (kFewRows packed
+//           rows at most: left to the split kernel);
 //   split   every sequence's own rows (mma.sync over a TMA ring, keys as the M dimension);
 //           with weights it also keeps the scores of the own keys;
 //   merge   combines the parts of a row and, with weights, adds
@@ -52,8 +53,9 @@ struct SharedParams {
     int n_seqs, n_heads, n_kv_heads, group, n_qgroups;
     int n_prefixes, max_prefix_len, max_prefix_seqs;
     int prefix_chunk, prefix_slots; // keys of one prefix part; parts of the longest prefix
-    int prefix_qtiles;              // query tiles of the largest group
-    int prefix_items;               // query tiles x parts x KV heads x prefixes
+    int prefix_qtiles;              // query tiles of the largest group (few rows: of 8 rows)
+    int prefix_items;               // query tiles x parts x KV heads x prefixes; 0: few rows
+    int prefix_units;               // few rows: query tiles x prefixes, taken by the split kernel
     int chunk, max_chunks;          // the same for own rows
     int slots;                      // prefix_slots + max_chunks
     int max_kv_len, score_rows, score_cols;
@@ -687,9 +689,10 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
 }
 
 // ===========================================================================
-// split: a sequence's own rows
+// split: a sequence's own rows, and prefixes of few packed rows
 // ===========================================================================
-// CTA = (chunk of keys, KV head and up to 8 of its query heads, sequence).  Warp 4 streams
+// CTA = (chunk of keys, KV head and up to 8 of its query heads, sequence), or the same of a
+// prefix, where the 8 columns run over its sequences' heads.  Warp 4 streams
 // 64-key tiles of K and V through a TMA ring; warps 0-3 take 16 keys of each tile:
 //   S^T(16 keys x 8 heads) = K . Q^T,  O^T(hd x 8 heads) += V^T . P^T   (mma.sync)
 // so one tile in shared memory serves every query head of the KV head.
@@ -734,25 +737,63 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
         fence_mbar_init();
     }
     __syncthreads();
-    if (p.prefix_slots == 0) griddep_wait();
+    if (p.prefix_items == 0) griddep_wait();
     griddep_trigger();
     const bool last_cta =
-        p.prefix_slots > 0 && blockIdx.x + 1 == gridDim.x && blockIdx.y + 1 == gridDim.y && blockIdx.z + 1 == gridDim.z;
-    const int b = blockIdx.z;
-    const int kvh = blockIdx.y / p.n_qgroups, qg = blockIdx.y % p.n_qgroups;
+        p.prefix_items > 0 && blockIdx.x + 1 == gridDim.x && blockIdx.y + 1 == gridDim.y && blockIdx.z + 1 == gridDim.z;
     const int c = blockIdx.x;
-    const long long seq_row0 = p.seq_row0[b];
-    int ks, n;
-    own_range(p, b, ks, n);
-    const int key0 = ks + c * p.chunk;
-    if (key0 >= n) {
+    const bool of_prefix = static_cast<int>(blockIdx.z) < p.prefix_units;
+    int b, kvh, h_first, nh, key0, n, plen = 0;   // nh head columns; row_of() says whose
+    long long seq_row0;
+    if (of_prefix) {
+        const int u = blockIdx.z / p.prefix_qtiles, t = blockIdx.z % p.prefix_qtiles;
+        int s1;
+        prefix_range(p, u, b, s1, plen, blockIdx.x + blockIdx.y + t + threadIdx.x == 0);
+        kvh = blockIdx.y;
+        h_first = t * 8;
+        nh = kvh < p.n_kv_heads && c * p.prefix_chunk < plen ? min(8, (s1 - b) * p.group - h_first) : 0;
+        seq_row0 = p.prefix_row0[u];
+    } else {
+        b = blockIdx.z - p.prefix_units;
+        kvh = blockIdx.y / p.n_qgroups;
+        const int qg = blockIdx.y % p.n_qgroups;
+        h_first = kvh * p.group + qg * 8;
+        nh = min(8, p.group - qg * 8);
+        seq_row0 = p.seq_row0[b];
+    }
+    // (sequence, query head) of column i; the columns of a prefix run over its sequences' heads
+    auto row_of = [&](int i) -> long long {
+        const int r = h_first + i;
+        return of_prefix ? static_cast<long long>(b + r / p.group) * p.n_heads + kvh * p.group + r % p.group
+                         : static_cast<long long>(b) * p.n_heads + r;
+    };
+    auto first_key = [&](int i) -> int {   // of the prefix that the sequence of column i sees
+        int ks, own;
+        own_range(p, b + (h_first + i) / p.group, ks, own);
+        return max(0, plen + own - p.window);
+    };
+    if (of_prefix) {   // parts count from the first key any column sees
+        int lo = 0;
+        if (p.window > 0) {
+            lo = plen;
+            for (int i = 0; i < nh; ++i) lo = min(lo, first_key(i));
+        }
+        key0 = lo + c * p.prefix_chunk;
+        n = min(plen, key0 + p.prefix_chunk);
+        if (key0 >= n && static_cast<int>(threadIdx.x) < nh)
+            p.part_ml[row_of(threadIdx.x) * p.slots + c] = make_float2(-INFINITY, 0.f);
+    } else {
+        int ks;
+        own_range(p, b, ks, n);
+        key0 = ks + c * p.chunk;
+        n = min(n, key0 + p.chunk);
+    }
+    if (key0 >= n || nh <= 0) {
         if (last_cta) griddep_wait();
         return;
     }
-    const int nkeys = min(p.chunk, n - key0);
+    const int nkeys = n - key0;
     const int ntiles = (nkeys + kKeysPerTile - 1) / kKeysPerTile;
-    const int h_first = kvh * p.group + qg * 8;
-    const int nh = min(8, p.group - qg * 8);
     const long long row_base = seq_row0 + key0;
 
     if (warp == kConsumerWarps) {
@@ -783,12 +824,12 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
     }
     const int g = lane >> 2, tq = lane & 3;   // key row / head column of a fragment
     {   // the CTA's query rows as fp32, one padded row per head
-        const long long off = (static_cast<long long>(b) * p.n_heads + h_first) * HD;
         for (int v = threadIdx.x; v < nh * HD / 8; v += kConsumerWarps * 32) {
             const int e = v * 8;
             float *dst = qs + (e / HD) * S::kQRowFloats + e % HD;
+            const long long off = row_of(e / HD) * HD + e % HD;
             if (p.q_is_bf16) {
-                const uint4 w = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + off + e));
+                const uint4 w = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + off));
                 const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -796,7 +837,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
                     dst[2 * k + 1] = bf16hi_f32(u[k]);
                 }
             } else {
-                const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + off + e);
+                const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + off);
                 reinterpret_cast<float4 *>(dst)[0] = __ldg(src);
                 reinterpret_cast<float4 *>(dst)[1] = __ldg(src + 1);
             }
@@ -818,9 +859,14 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
     const float cap = p.softcap, inv_cap = cap > 0.f ? 1.f / cap : 0.f;
     const float scale2 = p.scale * kLog2e;
     float *sc_out = nullptr;   // scores of the two heads of this lane, key 0 of the chunk
-    if (p.scores && 2 * tq < nh)
+    if (p.scores && !of_prefix && 2 * tq < nh)
         sc_out = p.scores + ((static_cast<long long>(b) * p.n_kv_heads + kvh) * p.score_rows + key0) * p.score_cols +
-                 qg * 8 + 2 * tq;
+                 h_first - kvh * p.group + 2 * tq;
+    int hidden[2] = {0, 0};   // keys of the chunk before the first that the window shows these heads
+    if (of_prefix && p.window > 0)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (2 * tq + i < nh) hidden[i] = first_key(2 * tq + i) - key0;
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
     float o[KSTEPS][4];
 #pragma unroll
@@ -852,7 +898,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
             for (int i = 0; i < 4; ++i) {
                 const float raw = QT > 1 ? acc[i] + low[i] : acc[i];
                 x[i] = cap > 0.f ? cap * tanhf(raw * p.scale * inv_cap) * kLog2e : raw * scale2;
-                if (g + (i >> 1) * 8 >= nv) x[i] = -INFINITY;
+                const int at = g + (i >> 1) * 8;   // key of the block
+                if (at >= nv || kb + at < hidden[i & 1]) x[i] = -INFINITY;
             }
             if (sc_out) {
                 if (g < nv)
@@ -968,8 +1015,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
             if (f != 0.f) acc += f * red[(w * 8 + h) * kRowF + 2 + d];
             sum += f * red[(w * 8 + h) * kRowF + 1];
         }
-        const long long slot =
-            (static_cast<long long>(b) * p.n_heads + h_first + h) * p.slots + p.prefix_slots + c;
+        const long long slot = row_of(h) * p.slots + (of_prefix ? 0 : p.prefix_slots) + c;
         p.part_o[slot * HD + d] = acc;
         if (d == 0) p.part_ml[slot] = make_float2(M, sum);
     }
@@ -1173,25 +1219,27 @@ __global__ void __launch_bounds__(kMergeThreads, 4) merge_kernel(const __grid_co
 // ===========================================================================
 int div_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
-// Keys per part of the own rows: about 8 CTAs per SM, multiples of 64 keys, at most 2048.
-int own_chunk(long long units, int max_kv_len)
+// Keys per part for about `per_sm` CTAs per SM, multiples of 64 keys, at most 2048.
+int part_keys(long long units, int max_len, int per_sm)
 {
-    long long c = (units * (max_kv_len > 0 ? max_kv_len : 1) + kSms * 8 - 1) / (kSms * 8);
+    long long c = (units * (max_len > 0 ? max_len : 1) + kSms * per_sm - 1) / (kSms * per_sm);
     c = (c + kKeysPerTile - 1) / kKeysPerTile * kKeysPerTile;
     return static_cast<int>(c < kKeysPerTile ? kKeysPerTile : c > 2048 ? 2048 : c);
 }
 
-// Most parts own_chunk() makes for any length up to max_kv_len: ceil(L/64) while the
-// chunk is 64, at most ceil(1184/units) while it grows with the length, ceil(L/2048) after.
-int own_slots(long long units, int max_kv_len)
+// Most parts part_keys() makes for any length up to max_len: ceil(L/64) while a part is 64 keys,
+// at most ceil(148 per_sm / units) while it grows with the length, ceil(L/2048) after.
+int most_parts(long long units, int max_len, int per_sm)
 {
-    const int len = max_kv_len > 0 ? max_kv_len : 1;
+    const int len = max_len > 0 ? max_len : 1;
     int small = div_up(len, kKeysPerTile);
-    const int by_work = div_up(kSms * 8, units);
+    const int by_work = div_up(kSms * per_sm, units);
     if (small > by_work) small = by_work;
     const int big = div_up(len, 2048);
     return small > big ? small : big;
 }
+constexpr int kOwnPerSm = 8;   // own rows, whose lengths differ
+constexpr int kFewPerSm = 2;   // a prefix in the split kernel: one wave (4096 keys, 8 rows: 15.7 us; with 4: 23.6)
 
 // Parts of a prefix: one CTA per SM over the query tiles and KV heads of all prefixes, no
 // part under 128 keys, and none over kMaxPart: the tensor core truncates when it adds to an
@@ -1206,6 +1254,25 @@ int prefix_parts(int n_prefixes, int max_prefix_len, int max_prefix_seqs, int n_
     if (parts < 1) parts = 1;
     const int most = div_up(max_prefix_len, 128), least = div_up(max_prefix_len, kMaxPart);
     return parts < least ? least : parts < most ? parts : most;
+}
+
+// Packed rows (sequences x group) of a prefix up to which the split kernel takes it too, 8 rows
+// at a time: a CTA of the prefix kernel takes as long for one row of its 128-row tile as for all.
+// us with the prefix kernel / with the split kernel, 8 KV heads of 128, fp32:
+//   rows                  4            8           16           32
+//   512 shared keys   15.3 /  8.1  15.8 /  9.8  16.2 / 11.1  15.1 / 16.6
+//   4096              18.1 / 12.8  18.6 / 15.7  20.8 / 16.6  21.2 / 22.7
+//   32768             63.1 / 31.4  63.6 / 34.5  66.5 / 41.9  54.7 / 67.4
+//   8 times 4096      62.3 / 27.2  64.2 / 32.5  66.8 / 44.3  72.7 / 74.2
+constexpr int kFewRows = 16;
+bool few_rows(int n_seqs, int n_prefixes, int max_prefix_len, int max_prefix_seqs, int n_heads, int n_kv_heads)
+{
+    const long long rows = static_cast<long long>(max_prefix_seqs) * (n_heads / n_kv_heads);
+    return n_prefixes > 0 && max_prefix_len > 0 && rows > 0 && rows <= kFewRows && n_seqs + n_prefixes * ((rows + 7) / 8) <= 65535;
+}
+long long few_units(int n_prefixes, int max_prefix_seqs, int n_heads, int n_kv_heads)
+{
+    return static_cast<long long>(n_prefixes) * n_kv_heads * ((max_prefix_seqs * (n_heads / n_kv_heads) + 7) / 8);
 }
 
 // CTAs of the prefix kernel: every SM, or half of them where the own rows have enough to do
@@ -1278,7 +1345,7 @@ int launch_shared(cudaStream_t st, SharedParams &p, const uint16_t *k_pool, cons
                make_tmap_2d(&p.tv, v_pool, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kv_dim, pool_rows, 64, rows);
     };
     int box_rows = 0;   // of the maps in p
-    if (p.prefix_slots > 0) {
+    if (p.prefix_items > 0) {
         using S = PrefixShape<HD, QT>;
         if (!maps(box_rows = S::kBoxRows) ||
             !allow_smem(reinterpret_cast<const void *>(prefix_kernel<HD, QT, PT>), S::kSmemBytes))
@@ -1288,12 +1355,13 @@ int launch_shared(cudaStream_t st, SharedParams &p, const uint16_t *k_pool, cons
         if (launch_kernel(prefix_kernel<HD, QT, PT>, grid, dim3(S::kThreads), S::kSmemBytes, st, p) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
     }
-    if (p.max_kv_len > 0) {
+    if (p.max_kv_len > 0 || p.prefix_units > 0) {
         using S = SplitShape<HD>;
         if ((box_rows != kKeysPerTile && !maps(kKeysPerTile)) ||
             !allow_smem(reinterpret_cast<const void *>(split_kernel<HD, QT, PT>), S::kSmemBytes))
             return SMOL_B200_ERR_CUDA;
-        const dim3 grid(p.max_chunks, p.n_kv_heads * p.n_qgroups, p.n_seqs);
+        const int parts = p.prefix_units > 0 && p.prefix_slots > p.max_chunks ? p.prefix_slots : p.max_chunks;
+        const dim3 grid(parts, p.n_kv_heads * p.n_qgroups, p.prefix_units + p.n_seqs);
         if (launch_kernel(split_kernel<HD, QT, PT>, grid, dim3(kSplitThreads), S::kSmemBytes, st, p) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
     }
@@ -1337,8 +1405,11 @@ size_t decode_shared_workspace_bytes(int n_seqs, int max_kv_len, int n_prefixes,
                                      int max_prefix_seqs, int n_heads, int n_kv_heads, int head_dim, bool weights)
 {
     if (!sizes_ok(n_seqs, max_kv_len, n_heads, n_kv_heads, head_dim)) return 0;
-    const int slots = own_slots(own_units(n_seqs, n_heads, n_kv_heads), max_kv_len) +
-                      prefix_parts(n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads);
+    const int slots =
+        most_parts(own_units(n_seqs, n_heads, n_kv_heads), max_kv_len, kOwnPerSm) +
+        (few_rows(n_seqs, n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads)
+             ? most_parts(few_units(n_prefixes, max_prefix_seqs, n_heads, n_kv_heads), max_prefix_len, kFewPerSm)
+             : prefix_parts(n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads));
     return shared_layout(n_seqs, max_kv_len, slots, n_heads, n_kv_heads, head_dim, weights).total;
 }
 
@@ -1370,14 +1441,21 @@ int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const v
     if (n_kv_heads * ((n_heads / n_kv_heads + 7) / 8) > 65535) return SMOL_B200_ERR_ARGS;
     p.group = n_heads / n_kv_heads;
     p.n_qgroups = (p.group + 7) / 8;
-    p.chunk = own_chunk(units, max_kv_len);
+    p.chunk = part_keys(units, max_kv_len, kOwnPerSm);
     p.max_chunks = max_kv_len > 0 ? div_up(max_kv_len, p.chunk) : 0;
-    p.prefix_slots = prefix_parts(n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads);
-    if (p.prefix_slots > 0) p.prefix_chunk = (div_up(max_prefix_len, p.prefix_slots) + 63) / 64 * 64;
-    p.prefix_qtiles = div_up(static_cast<long long>(max_prefix_seqs) * p.group, kBM);
-    const long long items = static_cast<long long>(p.prefix_qtiles) * p.prefix_slots * n_kv_heads * n_prefixes;
-    if (items > 0x7fffff00LL) return SMOL_B200_ERR_ARGS;
-    p.prefix_items = static_cast<int>(items);
+    if (few_rows(n_seqs, n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads)) {
+        p.prefix_chunk = part_keys(few_units(n_prefixes, max_prefix_seqs, n_heads, n_kv_heads), max_prefix_len, kFewPerSm);
+        p.prefix_slots = div_up(max_prefix_len, p.prefix_chunk);
+        p.prefix_qtiles = (max_prefix_seqs * p.group + 7) / 8;
+        p.prefix_units = n_prefixes * p.prefix_qtiles;
+    } else {
+        p.prefix_slots = prefix_parts(n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads);
+        if (p.prefix_slots > 0) p.prefix_chunk = (div_up(max_prefix_len, p.prefix_slots) + 63) / 64 * 64;
+        p.prefix_qtiles = div_up(static_cast<long long>(max_prefix_seqs) * p.group, kBM);
+        const long long items = static_cast<long long>(p.prefix_qtiles) * p.prefix_slots * n_kv_heads * n_prefixes;
+        if (items > 0x7fffff00LL) return SMOL_B200_ERR_ARGS;
+        p.prefix_items = static_cast<int>(items);
+    }
     p.slots = p.prefix_slots + p.max_chunks;
     if (p.slots < 1) p.slots = 1;
     const size_t need = decode_shared_workspace_bytes(n_seqs, max_kv_len, n_prefixes, max_prefix_len, max_prefix_seqs,

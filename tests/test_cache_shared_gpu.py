@@ -309,3 +309,140 @@ def test_pool_rows_past_32_bit_offsets(cuda):
     c.pfirst, c.first = [x + off for x in c.pfirst], [x + off for x in c.first]
     c.check(c.run())
     no_error()
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+@pytest.mark.parametrize("more", [0, 1, 9])
+@pytest.mark.parametrize("window", [0, 1, 100, 420])
+def test_packed_rows_around_sixteen(cuda, hq, hkv, hd, more, window):
+    # sequences x group of up to 16 rows, just above, and well above; a second prefix has a
+    # single sequence, and the last sequence none
+    seqs = max(1, 16 * hkv // hq) + more
+    lens = [(i * 37) % 150 for i in range(seqs)] + [30, 12]
+    for bf16 in (False, True):
+        c = Case(cuda, lens, plens=[400, 129], cut=[0, seqs, seqs + 1], hq=hq, hkv=hkv, hd=hd, q_bf16=bf16,
+                 out_bf16=bf16, window=window, cap=20.0 * more, seed=16)
+        c.check(c.run())
+    no_error()
+
+
+@pytest.mark.parametrize("per", [1, 3, 10])
+@pytest.mark.parametrize("prefixes", [32, 33, 70])
+def test_many_prefixes(cuda, prefixes, per):
+    # lengths from none up, groups of `per` sequences and some of none
+    cut = [0]
+    for i in range(prefixes):
+        cut.append(cut[-1] + (per if i % 5 != 3 else 0))
+    c = Case(cuda, [i % 7 for i in range(cut[-1] + 1)], plens=[i * 29 % 200 for i in range(prefixes)], cut=cut, hq=4,
+             hkv=2, hd=64, seed=17)
+    c.check(c.run())
+    no_error()
+
+
+@pytest.mark.parametrize("big,cap", [(1.0, 50.0), (20.0, 30.0), (12.0, 0.0)])
+def test_large_scores_of_many_sequences(cuda, big, cap):
+    c = Case(cuda, [i * 13 % 90 for i in range(20)], plens=[1300], cut=[0, 20], cap=cap, big=big, seed=18)
+    c.check(c.run())
+    no_error()
+
+
+def test_rising_scores_of_many_sequences(cuda):
+    c = Case(cuda, [5] * 70, plens=[900], cut=[0, 70], hq=2, hkv=1, hd=64, seed=19)
+    q = c.q.view(70, 2, 64)
+    q[:] = q[0, 0].sign()
+    f = torch.linspace(-8.0, 4.0, 900, device=cuda).view(900, 1)
+    c.k[c.pfirst[0]:c.pfirst[0] + 900] = (q[0, 0].view(1, 64) * f).to(torch.bfloat16)
+    c.check(c.run())
+    no_error()
+
+
+@pytest.mark.parametrize("seqs", [4, 30])
+def test_prefixes_beyond_the_announced_are_flagged(cuda, seqs):
+    c = Case(cuda, [3 + i % 4 for i in range(seqs)], plens=[200, 90], cut=[0, seqs - 1, seqs], seed=20)
+    n, maxl = seqs, max(c.lens)
+    ws = torch.empty(smol_b200.decode_shared_workspace_bytes(n, maxl, 2, 128, seqs - 1, 16, 8, 128), dtype=torch.uint8,
+                     device=cuda)
+
+    def run(plens, cut, most):
+        smol_b200.decode_attention_shared(c.out, c.q, c.k, c.v, c.rows, c.i64(c.pfirst), c.i32(plens), c.i32(cut), 2, 128,
+                                          most, c.i64(c.first), c.i32(c.lens), n, maxl, 16, 8, 128, c.scale, ws,
+                                          weights_in=c.win, weights_out=c.wout, weights_stride=c.stride)
+        torch.cuda.synchronize()
+        flagged = smol_b200.device_error() & (1 << 5)
+        smol_b200.clear_error()
+        return flagged
+
+    assert run([200, 90], c.cut, seqs - 1)       # longer than announced: its first rows count
+    c.plens = [128, 90]
+    c.check(c.wout)
+    assert not run([128, 90], c.cut, seqs - 1)
+    c.check(c.wout)
+    assert run([128, 90], [0, seqs - 1, seqs + 5], seqs - 1)   # past the last sequence
+    c.check(c.wout)
+    assert run([128, -4], c.cut, seqs - 1)       # counts as empty
+    c.plens = [128, 0]
+    c.check(c.wout)
+    assert run([128, 0], c.cut, seqs - 2)        # more sequences than announced: the rest has no prefix
+    c.cut = [0, seqs - 2, seqs - 2]
+    c.check(c.wout)
+
+
+@pytest.mark.parametrize("seqs", [3, 21])
+def test_captured_step_follows_the_device_prefixes(cuda, seqs):
+    c = Case(cuda, [40 + i % 9 for i in range(seqs)], plens=[700, 300], cut=[0, seqs - 1, seqs], seed=21)
+    plens, cut, lens = c.i32(c.plens), c.i32(c.cut), c.i32(c.lens)
+    pfirst, first = c.i64(c.pfirst), c.i64(c.first)
+    maxl = max(c.lens)
+    ws = torch.empty(smol_b200.decode_shared_workspace_bytes(seqs, maxl, 2, 700, seqs, 16, 8, 128), dtype=torch.uint8,
+                     device=cuda)
+
+    def step():
+        smol_b200.decode_attention_shared(c.out, c.q, c.k, c.v, c.rows, pfirst, plens, cut, 2, 700, seqs, first, lens,
+                                          seqs, maxl, 16, 8, 128, c.scale, ws, weights_in=c.win, weights_out=c.wout,
+                                          weights_stride=c.stride)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        step()
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        for _ in range(3):   # launches of one step after those of another, on one workspace
+            step()
+    for p, k in (([700, 300], [0, seqs - 1, seqs]), ([0, 1], [0, 1, seqs]), ([130, 300], [0, seqs, seqs]),
+                 ([699, 2], [1, 2, 2])):
+        plens.copy_(c.i32(p))
+        cut.copy_(c.i32(k))
+        c.plens, c.cut = p, k
+        c.wout.fill_(-3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(c.wout)
+    no_error()
+
+
+def test_two_streams_with_their_own_workspaces(cuda):
+    cases = [Case(cuda, [100 + 13 * i for i in range(n)], plens=[900], cut=[0, n], seed=22 + n) for n in (5, 40)]
+    alone = []
+    for c in cases:
+        w = c.run()
+        alone.append((c.out.clone(), w.clone()))
+        c.check(w)
+    streams = [torch.cuda.Stream() for _ in cases]
+    args = []
+    for c in cases:
+        n = len(c.lens)
+        ws = torch.empty(smol_b200.decode_shared_workspace_bytes(n, max(c.lens), 1, 900, n, 16, 8, 128),
+                         dtype=torch.uint8, device=cuda)
+        args.append((c.out, c.q, c.k, c.v, c.rows, c.i64(c.pfirst), c.i32(c.plens), c.i32(c.cut), 1, 900, n,
+                     c.i64(c.first), c.i32(c.lens), n, max(c.lens), 16, 8, 128, c.scale, ws))
+        c.out.zero_()
+        c.wout.fill_(-3.0)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, a, s in zip(cases, args, streams):
+            with torch.cuda.stream(s):
+                smol_b200.decode_attention_shared(*a, weights_in=c.win, weights_out=c.wout, weights_stride=c.stride)
+    torch.cuda.synchronize()
+    for c, (o, w) in zip(cases, alone):
+        assert torch.equal(c.out, o) and torch.equal(c.wout, w)
+    no_error()
