@@ -101,11 +101,15 @@ __device__ __forceinline__ void prefix_range(const SharedParams &p, int g, int &
     if (bad && flag) atomicOr(p.err, kErrBadArgs);
 }
 
-// Own keys [ks, n) of sequence b that are visible; n is clipped to max_kv_len.
+// Own keys [ks, n) that a sequence of kv_len rows sees; n is clipped to max_kv_len.
+__device__ __forceinline__ void own_keys(const SharedParams &p, int kv_len, int &ks, int &n)
+{
+    n = min(max(kv_len, 0), p.max_kv_len);
+    ks = (p.window > 0 && n > p.window) ? n - p.window : 0;
+}
 __device__ __forceinline__ void own_range(const SharedParams &p, int b, int &ks, int &n)
 {
-    n = min(max(p.kv_len[b], 0), p.max_kv_len);
-    ks = (p.window > 0 && n > p.window) ? n - p.window : 0;
+    own_keys(p, p.kv_len[b], ks, n);
 }
 
 // ===========================================================================
@@ -1034,13 +1038,14 @@ constexpr int kMergeWarps = kMergeThreads / 32;
 constexpr int kMergeKeys = 1024;
 constexpr int kMergeOuts = 128;
 
-// The slots of sequence b that hold parts: [0, np) of its prefix and [own0, own1) of its own
-// rows (the whole warp).
+// The slots of a sequence that hold parts: [0, np) of its prefix and [own0, own1) of its own rows.
 struct Parts {
     int np, own0, own1;
     __device__ __forceinline__ bool has(int slot) const { return slot < np || (slot >= own0 && slot < own1); }
 };
-__device__ __forceinline__ Parts parts_of(const SharedParams &p, int b, int own_keys)
+// Of sequence b, whose length the caller has loaded; also its visible own keys [ks, n) (the
+// whole warp).
+__device__ __forceinline__ Parts parts_of(const SharedParams &p, int b, int kv_len, int &ks, int &n)
 {
     Parts t;
     t.np = 0;
@@ -1055,8 +1060,9 @@ __device__ __forceinline__ Parts parts_of(const SharedParams &p, int b, int own_
         t.np = max(t.np, __reduce_max_sync(0xffffffffu, mine));
         if (t.np > 0) break;
     }
+    own_keys(p, kv_len, ks, n);
     t.own0 = p.prefix_slots;
-    t.own1 = p.prefix_slots + (own_keys > 0 ? (own_keys + p.chunk - 1) / p.chunk : 0);
+    t.own1 = p.prefix_slots + (n > ks ? (n - ks + p.chunk - 1) / p.chunk : 0);
     return t;
 }
 
@@ -1102,39 +1108,50 @@ __global__ void __launch_bounds__(kMergeThreads, 4) merge_kernel(const __grid_co
         float inv = 0.f;
         constexpr int kHeads = HD < kMergeOuts ? kMergeOuts / HD : 1;   // heads of a unit
         const long long head0 = u * kMergeOuts / HD;                   // its first (sequence, head)
+        constexpr int kLoad = 4;                                       // parts in flight
+        // Everything the first parts need is loaded at once: what a slot without a part holds is
+        // not used.
+        const long long mine = live ? e / HD : 0;   // this lane's (sequence, head)
+        const float2 *my_ml = p.part_ml + mine * p.slots;
+        const float *src = p.part_o + mine * p.slots * HD + e % HD;
+        float r[kLoad];
+        float4 v[kLoad];
+        auto load_parts = [&](int c0, auto &&wanted) {
+#pragma unroll
+            for (int k = 0; k < kLoad; ++k) {
+                const int c = c0 + k * ways;
+                r[k] = -INFINITY;
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (live && wanted(c)) {
+                    r[k] = my_ml[c].x;
+                    v[k] = *reinterpret_cast<const float4 *>(src + static_cast<long long>(c) * HD);
+                }
+            }
+        };
+        load_parts(way, [&](int c) { return c < p.slots; });
 #pragma unroll
         for (int i = 0; i < kHeads; ++i) {
             const long long hs = head0 + i;
             if (hs >= static_cast<long long>(p.n_seqs) * p.n_heads) break;
             const int b = static_cast<int>(hs / p.n_heads);
             const float2 *ml = p.part_ml + hs * p.slots;
-            // in flight while the sequence's parts are found (a slot without one is not used)
             const float2 ahead = lane < p.slots ? ml[lane] : make_float2(-INFINITY, 0.f);
+            const int kv_len = p.kv_len[b];
             int ks, n;
-            own_range(p, b, ks, n);
-            if (lane == 0 && way == 0 && hs % p.n_heads == 0 && p.kv_len[b] != n) atomicOr(p.err, kErrBadArgs);
-            const Parts t = parts_of(p, b, n - ks);
+            const Parts t = parts_of(p, b, kv_len, ks, n);
+            if (lane == 0 && way == 0 && hs % p.n_heads == 0 && kv_len != n) atomicOr(p.err, kErrBadArgs);
             float M, my_inv;
             head_sum(p, ml, ahead, t, M, my_inv);
             if (e / HD != hs) continue;   // (a half-warp at head dim 64)
             inv = my_inv;
-            const float *src = p.part_o + hs * p.slots * HD + e % HD;
-            constexpr int kLoad = 4;   // parts in flight
             for (int c0 = way; c0 < t.own1 || c0 < t.np; c0 += kLoad * ways) {
-                float f[kLoad];
-                float4 v[kLoad];
-#pragma unroll
-                for (int k = 0; k < kLoad; ++k) f[k] = t.has(c0 + k * ways) ? ml[c0 + k * ways].x : -INFINITY;
-#pragma unroll
-                for (int k = 0; k < kLoad; ++k) {   // an empty part has no output written
-                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (f[k] != -INFINITY)
-                        v[k] = *reinterpret_cast<const float4 *>(src + static_cast<long long>(c0 + k * ways) * HD);
-                    f[k] = f[k] != -INFINITY ? fast_exp2f(f[k] - M) : 0.f;
-                }
+                if (c0 != way) load_parts(c0, [&](int c) { return t.has(c); });
 #pragma unroll
                 for (int k = 0; k < kLoad; ++k)
-                    a.x += f[k] * v[k].x, a.y += f[k] * v[k].y, a.z += f[k] * v[k].z, a.w += f[k] * v[k].w;
+                    if (t.has(c0 + k * ways) && r[k] != -INFINITY) {   // an empty part has no output written
+                        const float f = fast_exp2f(r[k] - M);
+                        a.x += f * v[k].x, a.y += f * v[k].y, a.z += f * v[k].z, a.w += f * v[k].w;
+                    }
             }
         }
         if (ways > 1) {
@@ -1163,10 +1180,10 @@ __global__ void __launch_bounds__(kMergeThreads, 4) merge_kernel(const __grid_co
     const long long row0 = static_cast<long long>(b) * p.n_heads + kvh * p.group;
     const float2 *ml = p.part_ml + (row0 + warp) * p.slots;   // of the first eight heads
     const float2 ahead = warp < p.group && lane < p.slots ? ml[lane] : make_float2(-INFINITY, 0.f);
+    const int kv_len = p.kv_len[b];
     int ks, n;
-    own_range(p, b, ks, n);
+    const Parts t = parts_of(p, b, kv_len, ks, n);
     if (j0 >= n) return;
-    const Parts t = parts_of(p, b, n - ks);
     __shared__ float s_M[8], s_inv[8];
     constexpr int kPer = kMergeKeys / kMergeThreads;
     float w[kPer], w_in[kPer];
