@@ -1236,26 +1236,32 @@ __global__ void __launch_bounds__(kMergeThreads, 4) merge_kernel(const __grid_co
 // ===========================================================================
 int div_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
-// Keys per part for about `per_sm` CTAs per SM, multiples of 64 keys, at most 2048.
+// Keys per part for about `per_sm` CTAs per SM, multiples of 64 keys, at most kMostKeys: more
+// parts cost their joining, longer ones leave SMs without work where lengths differ (16 sequences
+// of 2000 to 8192 keys, 8 KV heads of 128: 65.2 us with 1024, 69.7 with 2048).
+constexpr int kMostKeys = 1024;
 int part_keys(long long units, int max_len, int per_sm)
 {
     long long c = (units * (max_len > 0 ? max_len : 1) + kSms * per_sm - 1) / (kSms * per_sm);
     c = (c + kKeysPerTile - 1) / kKeysPerTile * kKeysPerTile;
-    return static_cast<int>(c < kKeysPerTile ? kKeysPerTile : c > 2048 ? 2048 : c);
+    return static_cast<int>(c < kKeysPerTile ? kKeysPerTile : c > kMostKeys ? kMostKeys : c);
 }
 
 // Most parts part_keys() makes for any length up to max_len: ceil(L/64) while a part is 64 keys,
-// at most ceil(148 per_sm / units) while it grows with the length, ceil(L/2048) after.
+// at most ceil(148 per_sm / units) while it grows with the length, ceil(L / kMostKeys) after.
 int most_parts(long long units, int max_len, int per_sm)
 {
     const int len = max_len > 0 ? max_len : 1;
     int small = div_up(len, kKeysPerTile);
     const int by_work = div_up(kSms * per_sm, units);
     if (small > by_work) small = by_work;
-    const int big = div_up(len, 2048);
+    const int big = div_up(len, kMostKeys);
     return small > big ? small : big;
 }
-constexpr int kOwnPerSm = 8;   // own rows, whose lengths differ
+// Own rows, whose lengths differ (us with 8 / 3 / 2: 4 sequences of 2000 to 8192 keys, 8 KV heads
+// of 128 19.4 / 14.6 / 15.9; 64 of 300 to 1000, one KV head of 256 31.7 / 18.4 / 20.1; 16 of 300 to
+// 1000, 12 KV heads of 64 13.3 / 12.2 / 12.9).
+constexpr int kOwnPerSm = 3;
 constexpr int kFewPerSm = 2;   // a prefix in the split kernel: one wave (4096 keys, 8 rows: 15.7 us; with 4: 23.6)
 
 // Parts of a prefix: one CTA per SM over the query tiles and KV heads of all prefixes, no
