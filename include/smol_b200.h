@@ -531,12 +531,12 @@ SMOL_B200_API int smol_b200_layer_norm(void *stream, void *out, int out_bf16, co
  * prefix_seq0[g] <= b < prefix_seq0[g+1] (device, n_prefixes + 1 ascending entries) attend
  * pool rows [prefix_row0[g], prefix_row0[g] + prefix_len[g]) followed by their own rows
  * [seq_row0[b], seq_row0[b] + kv_len[b]); a sequence outside every range has no prefix.
- * Prefix rows are read once for all the sequences that share them.  kv_len[b] and
+ * Prefix rows are read for many of the sequences that share them at once.  kv_len[b] and
  * prefix_len[g] may be 0; a sequence without any visible row gives zeros.  window > 0
  * limits a sequence to the last `window` of its prefix and own rows together; softcap > 0
  * caps scores as in Part 3.  max_kv_len, max_prefix_len and max_prefix_seqs (sequences of
  * one prefix) bound the device values: what exceeds them is left out and flagged in the
- * device error word.
+ * device error word.  The two lengths go up to 2^29.
  * q: [n_seqs, n_heads*head_dim] fp32 or bf16 (q_is_bf16); out: the same shape, fp32 or
  * bf16 (out_is_bf16); both and the pools 16-byte aligned.  fp32 queries enter with 24 bits,
  * and an fp32 output is computed to fp32 accuracy from the cached values; a bf16 output is

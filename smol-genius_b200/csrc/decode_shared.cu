@@ -19,8 +19,6 @@
 // two left the scores 4e-6 off), bf16 queries as they are.  The probabilities multiply V
 // as fp16: one term (2^-12) where the output is rounded to bf16 (2^-9) anyway, the value
 // and its remainder (2^-23) where the output is fp32.
-#include <stdio.h>
-#include <stdlib.h>
 #include <string.h>
 
 #include <mutex>
@@ -1234,6 +1232,7 @@ __global__ void __launch_bounds__(kMergeThreads, 4) merge_kernel(const __grid_co
 // ===========================================================================
 // host
 // ===========================================================================
+constexpr int kMostLen = 1 << 29;   // of max_kv_len and max_prefix_len: sums of lengths and parts stay within an int
 int div_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
 // Keys per part for about `per_sm` CTAs per SM, multiples of 64 keys, at most kMostKeys: more
@@ -1302,16 +1301,10 @@ long long few_units(int n_prefixes, int max_prefix_seqs, int n_heads, int n_kv_h
 // beside it -- the split kernel keeps HBM busy from the other half while the prefix kernel,
 // bound by its products and exponentials, works (64 sequences on 8192 shared and 100 to 1024
 // own keys: 52.9 us with all SMs, 48.3 with half; four prefixes, 200 sequences: 233 and 207).
-// SMOL_PREFIX_CTAS in the environment overrides it (measurement knob).
-const int g_prefix_ctas = [] {
-    const char *e = getenv("SMOL_PREFIX_CTAS");
-    return e ? atoi(e) : 0;
-}();
 int prefix_ctas(const SharedParams &p, int hd)
 {
-    if (g_prefix_ctas > 0 && g_prefix_ctas <= kSms) return g_prefix_ctas;
-    // bytes of own rows if half of the bound is used, against those a prefix kernel on all
-    // SMs reads in the same time: about 20 us per 512 KB part
+    // own rows at HBM's rate, half of the bound in use, against items of 5 us and 15 more for
+    // every 512 KB they read
     const double own_us = 0.5 * p.n_seqs * p.max_kv_len * 4.0 * p.n_kv_heads * hd / 6.3e6;
     const double part_us = 5.0 + p.prefix_chunk * 4.0 * hd / 512e3 * 15.0;
     const double prefix_us = static_cast<double>(p.prefix_items) / kSms * part_us;
@@ -1367,6 +1360,15 @@ int launch_shared(cudaStream_t st, SharedParams &p, const uint16_t *k_pool, cons
         return make_tmap_2d(&p.tk, k_pool, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kv_dim, pool_rows, 64, rows) &&
                make_tmap_2d(&p.tv, v_pool, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kv_dim, pool_rows, 64, rows);
     };
+    // Warps per 128 outputs: one where that fills the GPU with warps, up to eight (and a part
+    // each) where a row's parts would otherwise be read one after another.
+    const long long units = (static_cast<long long>(p.n_seqs) * p.n_heads * HD + kMergeOuts - 1) / kMergeOuts;
+    int ways = 1;
+    while (ways < kMergeWarps && units * ways < kSms * kMergeWarps && 2 * ways < p.slots) ways *= 2;
+    const long long out_blocks = (units * ways + kMergeWarps - 1) / kMergeWarps;
+    const long long key_blocks =
+        p.scores ? static_cast<long long>(div_up(p.max_kv_len, kMergeKeys)) * p.n_seqs * p.n_kv_heads : 0;
+    if (out_blocks + key_blocks > 0x7fffffffLL) return SMOL_B200_ERR_ARGS;
     int box_rows = 0;   // of the maps in p
     if (p.prefix_items > 0) {
         using S = PrefixShape<HD, QT>;
@@ -1388,15 +1390,6 @@ int launch_shared(cudaStream_t st, SharedParams &p, const uint16_t *k_pool, cons
         if (launch_kernel(split_kernel<HD, QT, PT>, grid, dim3(kSplitThreads), S::kSmemBytes, st, p) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
     }
-    // Warps per 128 outputs: one where that fills the GPU with warps, up to eight (and a part
-    // each) where a row's parts would otherwise be read one after another.
-    const long long units = (static_cast<long long>(p.n_seqs) * p.n_heads * HD + kMergeOuts - 1) / kMergeOuts;
-    int ways = 1;
-    while (ways < kMergeWarps && units * ways < kSms * kMergeWarps && 2 * ways < p.slots) ways *= 2;
-    const long long out_blocks = (units * ways + kMergeWarps - 1) / kMergeWarps;
-    const long long key_blocks =
-        p.scores ? static_cast<long long>(div_up(p.max_kv_len, kMergeKeys)) * p.n_seqs * p.n_kv_heads : 0;
-    if (out_blocks + key_blocks > 0x7fffffffLL) return SMOL_B200_ERR_ARGS;
     if (launch_kernel(merge_kernel<HD>, dim3(static_cast<unsigned>(out_blocks + key_blocks)), dim3(kMergeThreads), 0, st, p,
                       ways, static_cast<int>(out_blocks)) != cudaSuccess)
         return SMOL_B200_ERR_CUDA;
@@ -1447,7 +1440,7 @@ int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const v
     if (n_seqs <= 0) return SMOL_B200_OK;
     if (!sizes_ok(n_seqs, max_kv_len, n_heads, n_kv_heads, head_dim) || !out || !q || !k_pool || !v_pool ||
         !seq_row0 || !kv_len || pool_rows <= 0 || pool_rows >= (1ll << 31) || n_prefixes < 0 || n_prefixes > 65535 ||
-        max_prefix_len < 0 || max_prefix_seqs < 0 || max_prefix_seqs > n_seqs)
+        max_prefix_len < 0 || max_prefix_len > kMostLen || max_kv_len > kMostLen || max_prefix_seqs < 0 || max_prefix_seqs > n_seqs)
         return SMOL_B200_ERR_ARGS;
     if (n_prefixes > 0 && (!prefix_row0 || !prefix_len || !prefix_seq0)) return SMOL_B200_ERR_ARGS;
     if ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool) | reinterpret_cast<uintptr_t>(q) |

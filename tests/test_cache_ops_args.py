@@ -197,3 +197,19 @@ def test_binding_passes_each_argument_to_its_parameter(monkeypatch):
           dict(pool_rows=11, stride=15, n_seqs=3, max_kv_len=12, n_kv_heads=8, head_dim=128, budget=41, sink=42, recent=43,
                **sel("k_pool", "v_pool", "seq_row0", "weights_in", "weights_out", "positions_in", "positions_out",
                      "kv_len_in", "kv_len_out", "seq_pos")))
+
+
+@pytest.mark.parametrize("over", [dict(max_kv_len=(1 << 29) + 1, weights_stride=1 << 30), dict(max_prefix_len=(1 << 29) + 1),
+                                  dict(max_prefix_len=(1 << 31) - 1)])
+def test_shared_refuses_lengths(over):
+    assert smol_b200.lib().smol_b200_decode_attention_shared(*shared_args(**over)) == ARGS
+    smol_b200.clear_error()
+
+
+@pytest.mark.parametrize("n_prefixes,most,hq,hkv", [(1, 1, 16, 8), (1, 8, 16, 8), (1, 9, 16, 8), (40, 2, 8, 1), (40, 3, 8, 1)])
+def test_shared_workspaces_never_shrink(n_prefixes, most, hq, hkv):
+    prev = 0
+    for n in sorted(set(range(0, 20001, 37)) | {1023, 1024, 1025, 9409, 9472, 65536, 500000}):
+        size = smol_b200.decode_shared_workspace_bytes(n_prefixes * most, 100, n_prefixes, n, most, hq, hkv, 128)
+        assert size >= prev
+        prev = size
