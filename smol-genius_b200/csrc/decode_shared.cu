@@ -52,6 +52,7 @@ struct SharedParams {
     unsigned *err;
     int q_is_bf16, out_is_bf16;
     int n_seqs, n_heads, n_kv_heads, group, n_qgroups;
+    unsigned group_inv;             // ceil(2^31 / group): (u * group_inv) >> 31 is u / group while u * group < 2^31
     int n_prefixes, max_prefix_len, max_prefix_seqs;
     int prefix_chunk, prefix_slots; // keys of one prefix part; parts of the longest prefix
     int prefix_qtiles;              // query tiles of the largest group (few rows: of 8 rows)
@@ -178,6 +179,7 @@ __device__ __forceinline__ int prefix_parts_of(const SharedParams &p, int plen)
 struct PrefixItem {
     int qt, kvh, c, g;
     int s0, s1, plen;        // sequences and length of the prefix
+    int b0, h0, rows;        // row 0 of the tile is head h0 of the group of sequence b0; its rows in use
     int key_lo, key_hi;      // keys of the part
     int n_tiles;
 };
@@ -212,6 +214,15 @@ __device__ __forceinline__ PrefixTable prefix_table(const SharedParams &p, bool 
     return t;
 }
 
+// (sequence, query head) of row r < 128 of the tile; a division would take some 30 instructions,
+// and a call this short fetches most of its instructions from memory.
+__device__ __forceinline__ long long packed_row(const SharedParams &p, const PrefixItem &it, int r)
+{
+    const unsigned u = static_cast<unsigned>(it.h0 + r);
+    const int q = static_cast<int>((static_cast<unsigned long long>(u) * p.group_inv) >> 31);
+    return static_cast<long long>(it.b0 + q) * p.n_heads + it.kvh * p.group + (static_cast<int>(u) - q * p.group);
+}
+
 template <int BN>
 __device__ __forceinline__ PrefixItem prefix_item(const SharedParams &p, const PrefixTable &t, int k, bool flag)
 {
@@ -239,14 +250,16 @@ __device__ __forceinline__ PrefixItem prefix_item(const SharedParams &p, const P
     }
     it.n_tiles = 0;
     it.key_lo = it.key_hi = 0;
-    const int b0 = it.s0 + it.qt * kBM / p.group;   // sequences of the tile: [b0, b1)
-    if (b0 >= it.s1) return it;
+    it.b0 = it.s0 + it.qt * kBM / p.group;
+    it.h0 = it.qt * kBM - (it.b0 - it.s0) * p.group;
+    it.rows = min(kBM, (it.s1 - it.s0) * p.group - it.qt * kBM);
+    if (it.rows <= 0) return it;
     // parts count from the first key any row of the tile sees
     int lo = 0;
     if (p.window > 0) {
-        const int b1 = min(it.s1, it.s0 + (it.qt * kBM + kBM - 1) / p.group + 1);
+        const int b1 = it.b0 + (it.h0 + it.rows - 1) / p.group + 1;   // sequences of the tile: [b0, b1)
         lo = it.plen;
-        for (int b = b0 + static_cast<int>(threadIdx.x % 32); b < b1; b += 32) {
+        for (int b = it.b0 + static_cast<int>(threadIdx.x % 32); b < b1; b += 32) {
             int ks, n;
             own_range(p, b, ks, n);
             lo = min(lo, max(0, it.plen + n - p.window));
@@ -430,11 +443,8 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
         for (int k = blockIdx.x; k < table.all; k += gridDim.x) {
             const PrefixItem it = prefix_item<BN>(p, table, k, false);
             // this thread's packed row
-            const int pr = it.qt * kBM + tid;
-            const int b = it.s0 + pr / p.group;
-            const bool row_valid = b < it.s1;
-            const long long slot =
-                (static_cast<long long>(b) * p.n_heads + it.kvh * p.group + pr % p.group) * p.slots + it.c;
+            const bool row_valid = tid < it.rows;
+            const long long row = packed_row(p, it, tid), slot = row * p.slots + it.c;
             if (it.n_tiles == 0) {
                 if (row_valid && wg == 0) p.part_ml[slot] = make_float2(-INFINITY, 0.f);
                 continue;
@@ -442,7 +452,7 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
             int lo = 0;   // the row's first visible prefix key
             if (row_valid && p.window > 0) {
                 int ks, n;
-                own_range(p, b, ks, n);
+                own_range(p, static_cast<int>(row / p.n_heads), ks, n);
                 lo = max(0, it.plen + n - p.window);
             }
             // This warp's share of the query rows as QT bf16 terms in the 128B-swizzled K-major
@@ -452,17 +462,16 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
             if (n_items > 0) named_bar_sync(1, S::kSoftmax);   // the last item's staging has been read
             constexpr int kVecs = HD / 8, kLoad = QT == 1 ? 8 : 4, kRows = 32 / NG;   // rows loaded by a warp
             const int lr = warp * kRows;
-            if (it.s0 + (it.qt * kBM + lr) / p.group < it.s1) {
+            if (lr < it.rows) {
 #pragma unroll 1
                 for (int i0 = lane; i0 < kRows * kVecs; i0 += 32 * kLoad) {
                     uint4 raw[kLoad][QT == 1 ? 1 : 2];
 #pragma unroll
                     for (int n = 0; n < kLoad; ++n) {
                         const int i = i0 + 32 * n;
-                        const int rr = it.qt * kBM + lr + i / kVecs;
-                        const int rb = it.s0 + rr / p.group, rh = it.kvh * p.group + rr % p.group;
-                        const long long off = (static_cast<long long>(rb) * p.n_heads + rh) * HD + (i % kVecs) * 8;
-                        if (i < kRows * kVecs && rb < it.s1) {
+                        const int r = lr + i / kVecs;
+                        if (i < kRows * kVecs && r < it.rows) {
+                            const long long off = packed_row(p, it, r) * HD + (i % kVecs) * 8;
                             if constexpr (QT == 1) {
                                 raw[n][0] =
                                     __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + off));
@@ -477,7 +486,7 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
                     for (int n = 0; n < kLoad; ++n) {
                         const int i = i0 + 32 * n;
                         const int r = lr + i / kVecs, e = (i % kVecs) * 8;
-                        if (i >= kRows * kVecs || it.s0 + (it.qt * kBM + r) / p.group >= it.s1) continue;
+                        if (i >= kRows * kVecs || r >= it.rows) continue;
                         uint8_t *at = smem + (e / 64) * S::kQSubBytes + sw128_offset(r, (e % 64) / 8);
                         if constexpr (QT == 1) {
                             *reinterpret_cast<uint4 *>(at) = raw[n][0];
@@ -499,7 +508,7 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
             fence_proxy_async_smem();
             tc_fence_before();
             mbar_arrive(smem_u32(&bars->q_full));
-            const bool warp_live = it.s0 + (it.qt * kBM + (warp % 4) * 32) / p.group < it.s1;
+            const bool warp_live = (warp % 4) * 32 < it.rows;
             float m = -INFINITY, l = 0.f;
             // this warpgroup's tiles: numbers g with g % NG == wg; the first of the item is the
             // wg'th or, where the item starts on an odd number, the other
@@ -645,11 +654,8 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
                 long long off[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {   // rows written by this lane: 8 i + lane / 4
-                    const int rr = it.qt * kBM + (warp % 4) * 32 + 8 * i + lane / 4;
-                    const int rb = it.s0 + rr / p.group;
-                    off[i] = rb < it.s1 ? ((static_cast<long long>(rb) * p.n_heads + it.kvh * p.group + rr % p.group) *
-                                               p.slots + it.c) * HD + lane % 4 * 4
-                                        : -1;
+                    const int r = (warp % 4) * 32 + 8 * i + lane / 4;
+                    off[i] = r < it.rows ? (packed_row(p, it, r) * p.slots + it.c) * HD + lane % 4 * 4 : -1;
                 }
 #pragma unroll 1
                 for (int c0 = wg * (HD / NG); c0 < (wg + 1) * (HD / NG); c0 += 16) {
@@ -1457,9 +1463,13 @@ int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const v
     SharedParams p;
     memset(&p, 0, sizeof(p));
     const long long units = own_units(n_seqs, n_heads, n_kv_heads);
-    if (n_kv_heads * ((n_heads / n_kv_heads + 7) / 8) > 65535) return SMOL_B200_ERR_ARGS;
+    // grids; row numbers, and those of a tile times the group, stay within an int
+    if (n_kv_heads * ((n_heads / n_kv_heads + 7) / 8) > 65535 || static_cast<long long>(n_seqs) * n_heads > (1 << 30) ||
+        n_heads / n_kv_heads > 32768)
+        return SMOL_B200_ERR_ARGS;
     p.group = n_heads / n_kv_heads;
     p.n_qgroups = (p.group + 7) / 8;
+    p.group_inv = static_cast<unsigned>(((1ll << 31) + p.group - 1) / p.group);
     p.chunk = part_keys(units, max_kv_len, kOwnPerSm);
     p.max_chunks = max_kv_len > 0 ? div_up(max_kv_len, p.chunk) : 0;
     if (few_rows(n_seqs, n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads)) {
