@@ -57,6 +57,7 @@ struct SharedParams {
     int prefix_chunk, prefix_slots; // keys of one prefix part; parts of the longest prefix
     int prefix_qtiles;              // query tiles of the largest group (few rows: of 8 rows)
     int prefix_items;               // query tiles x parts x KV heads x prefixes; 0: few rows
+    int prefix_ctas;                // CTAs of the prefix kernel at most
     int prefix_units;               // few rows: query tiles x prefixes, taken by the split kernel
     int chunk, max_chunks;          // the same for own rows
     int slots;                      // prefix_slots + max_chunks
@@ -1272,16 +1273,16 @@ int most_parts(long long units, int max_len, int per_sm)
 constexpr int kOwnPerSm = 3;
 constexpr int kFewPerSm = 2;   // a prefix in the split kernel: one wave (4096 keys, 8 rows: 15.7 us; with 4: 23.6)
 
-// Parts of a prefix: one CTA per SM over the query tiles and KV heads of all prefixes, no
+// Parts of a prefix: one CTA on each of `sms` SMs over the query tiles and KV heads of all prefixes, no
 // part under 128 keys, and none over kMaxPart: the tensor core truncates when it adds to an
 // accumulator, which left a part of 6208 keys 1.3e-5 off (1024: 2e-6).
 constexpr int kMaxPart = 1024;
-int prefix_parts(int n_prefixes, int max_prefix_len, int max_prefix_seqs, int n_heads, int n_kv_heads)
+int prefix_parts(int n_prefixes, int max_prefix_len, int max_prefix_seqs, int n_heads, int n_kv_heads, int sms)
 {
     if (n_prefixes <= 0 || max_prefix_len <= 0 || max_prefix_seqs <= 0) return 0;
     const long long units = static_cast<long long>(n_prefixes) * n_kv_heads *
                             div_up(static_cast<long long>(max_prefix_seqs) * (n_heads / n_kv_heads), kBM);
-    int parts = static_cast<int>(kSms / units);
+    int parts = static_cast<int>(sms / units);
     if (parts < 1) parts = 1;
     const int most = div_up(max_prefix_len, 128), least = div_up(max_prefix_len, kMaxPart);
     return parts < least ? least : parts < most ? parts : most;
@@ -1306,18 +1307,34 @@ long long few_units(int n_prefixes, int max_prefix_seqs, int n_heads, int n_kv_h
     return static_cast<long long>(n_prefixes) * n_kv_heads * ((max_prefix_seqs * (n_heads / n_kv_heads) + 7) / 8);
 }
 
-// CTAs of the prefix kernel: every SM, or half of them where the own rows have enough to do
-// beside it -- the split kernel keeps HBM busy from the other half while the prefix kernel,
-// bound by its products and exponentials, works (64 sequences on 8192 shared and 100 to 1024
-// own keys: 52.9 us with all SMs, 48.3 with half; four prefixes, 200 sequences: 233 and 207).
-int prefix_ctas(const SharedParams &p, int hd)
+// CTAs of the prefix kernel, and the SMs its parts are made for.  The CTAs are one per SM, or as
+// many as the own rows leave SMs, but no fewer than half: the split kernel keeps HBM busy from
+// the others while the prefix kernel, bound by its products and exponentials, works; with all SMs
+// the own rows come after it.  Parts are made for the CTAs, except where the own rows take
+// longer anyway: then shorter ones.  Estimates in us: own rows at HBM's rate, half of the bound in
+// use; an item 5 and 15 for every 1024 keys of 128.  16/8 heads of 128, bf16, us with all SMs /
+// with half / so:  64 sequences, 8192 shared and 100 to 1024 own keys 52.9 / 46.5 / 45.3;  20
+// sequences, 20000 and 500 to 2000 78.9 / - / 55.8.
+struct PrefixGrid {
+    int ctas, sms;
+};
+PrefixGrid prefix_grid(const SharedParams &p, int n_prefixes, int max_prefix_len, int max_prefix_seqs, int hd)
 {
-    // own rows at HBM's rate, half of the bound in use, against items of 5 us and 15 more for
-    // every 512 KB they read
+    const long long own_ctas = static_cast<long long>(p.n_seqs) * p.n_kv_heads * p.n_qgroups * p.max_chunks;
+    const int left = own_ctas < kSms ? kSms - static_cast<int>(own_ctas + 1) / 2 : kSms / 2;   // two of them share an SM
     const double own_us = 0.5 * p.n_seqs * p.max_kv_len * 4.0 * p.n_kv_heads * hd / 6.3e6;
-    const double part_us = 5.0 + p.prefix_chunk * 4.0 * hd / 512e3 * 15.0;
-    const double prefix_us = static_cast<double>(p.prefix_items) / kSms * part_us;
-    return own_us > 0.5 * prefix_us ? kSms / 2 : kSms;
+    double prefix_us[2], us[2];
+    for (int i = 0; i < 2; ++i) {
+        const int sms = i == 0 ? kSms : left;
+        const int parts = prefix_parts(n_prefixes, max_prefix_len, max_prefix_seqs, p.n_heads, p.n_kv_heads, sms);
+        const long long items = static_cast<long long>(p.prefix_qtiles) * parts * p.n_kv_heads * n_prefixes;
+        const double item_us = 5.0 + div_up(max_prefix_len, parts) * (hd < 128 ? 128 : hd) / 131072.0 * 15.0;
+        us[i] = prefix_us[i] = static_cast<double>((items + sms - 1) / sms) * item_us;
+        if (i == 1) us[i] = us[i] > 1.05 * own_us ? us[i] : 1.05 * own_us;
+        else if (items > left) us[i] += own_us > 5.0 ? own_us : 5.0;
+    }
+    if (us[0] <= us[1]) return {kSms, kSms};
+    return {left, own_us > 2.0 * prefix_us[1] ? kSms : left};
 }
 
 struct SharedLayout {
@@ -1384,8 +1401,7 @@ int launch_shared(cudaStream_t st, SharedParams &p, const uint16_t *k_pool, cons
         if (!maps(box_rows = S::kBoxRows) ||
             !allow_smem(reinterpret_cast<const void *>(prefix_kernel<HD, QT, PT>), S::kSmemBytes))
             return SMOL_B200_ERR_CUDA;
-        const int at_most = prefix_ctas(p, HD);
-        const dim3 grid(static_cast<unsigned>(p.prefix_items < at_most ? p.prefix_items : at_most));
+        const dim3 grid(static_cast<unsigned>(p.prefix_items < p.prefix_ctas ? p.prefix_items : p.prefix_ctas));
         if (launch_kernel(prefix_kernel<HD, QT, PT>, grid, dim3(S::kThreads), S::kSmemBytes, st, p) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
     }
@@ -1434,7 +1450,7 @@ size_t decode_shared_workspace_bytes(int n_seqs, int max_kv_len, int n_prefixes,
         most_parts(own_units(n_seqs, n_heads, n_kv_heads), max_kv_len, kOwnPerSm) +
         (few_rows(n_seqs, n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads)
              ? most_parts(few_units(n_prefixes, max_prefix_seqs, n_heads, n_kv_heads), max_prefix_len, kFewPerSm)
-             : prefix_parts(n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads));
+             : prefix_parts(n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads, kSms));
     return shared_layout(n_seqs, max_kv_len, slots, n_heads, n_kv_heads, head_dim, weights).total;
 }
 
@@ -1462,6 +1478,10 @@ int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const v
 
     SharedParams p;
     memset(&p, 0, sizeof(p));
+    p.n_seqs = n_seqs;
+    p.n_heads = n_heads;
+    p.n_kv_heads = n_kv_heads;
+    p.max_kv_len = max_kv_len;
     const long long units = own_units(n_seqs, n_heads, n_kv_heads);
     // grids; row numbers, and those of a tile times the group, stay within an int
     if (n_kv_heads * ((n_heads / n_kv_heads + 7) / 8) > 65535 || static_cast<long long>(n_seqs) * n_heads > (1 << 30) ||
@@ -1478,9 +1498,12 @@ int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const v
         p.prefix_qtiles = (max_prefix_seqs * p.group + 7) / 8;
         p.prefix_units = n_prefixes * p.prefix_qtiles;
     } else {
-        p.prefix_slots = prefix_parts(n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads);
-        if (p.prefix_slots > 0) p.prefix_chunk = (div_up(max_prefix_len, p.prefix_slots) + 63) / 64 * 64;
         p.prefix_qtiles = div_up(static_cast<long long>(max_prefix_seqs) * p.group, kBM);
+        PrefixGrid grid = {kSms, kSms};
+        if (n_prefixes > 0) grid = prefix_grid(p, n_prefixes, max_prefix_len, max_prefix_seqs, head_dim);
+        p.prefix_ctas = grid.ctas;
+        p.prefix_slots = prefix_parts(n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads, grid.sms);
+        if (p.prefix_slots > 0) p.prefix_chunk = (div_up(max_prefix_len, p.prefix_slots) + 63) / 64 * 64;
         const long long items = static_cast<long long>(p.prefix_qtiles) * p.prefix_slots * n_kv_heads * n_prefixes;
         if (items > 0x7fffff00LL) return SMOL_B200_ERR_ARGS;
         p.prefix_items = static_cast<int>(items);
@@ -1513,13 +1536,9 @@ int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const v
     p.weights_stride = weights_stride;
     p.err = device_error_word();
     if (!p.err) return SMOL_B200_ERR_CUDA;
-    p.n_seqs = n_seqs;
-    p.n_heads = n_heads;
-    p.n_kv_heads = n_kv_heads;
     p.n_prefixes = n_prefixes;
     p.max_prefix_len = max_prefix_len;
     p.max_prefix_seqs = max_prefix_seqs;
-    p.max_kv_len = max_kv_len;
     p.window = window;
     p.scale = scale;
     p.softcap = softcap;
