@@ -584,8 +584,7 @@ def decode_attention_shared(out, q, k_pool, v_pool, pool_rows, prefix_row0, pref
         max_prefix_len, max_prefix_seqs, _dev(seq_row0), _dev(kv_len), n_seqs, max_kv_len, n_heads, n_kv_heads,
         head_dim, scale, window, softcap, _dev(weights_in), _dev(weights_out), weights_stride, _dev(workspace),
         workspace.nbytes)
-    if rc:
-        check(rc, "smol_b200_decode_attention_shared")
+    check(rc, "smol_b200_decode_attention_shared")
 
 
 def decode_weights_workspace_bytes(n_seqs, max_kv_len, n_heads, n_kv_heads, head_dim) -> int:
