@@ -402,10 +402,16 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
             // Q is written after the item before was read out, so its O may be overwritten too
             ok = mbar_wait_warp(smem_u32(&bars->q_full), n_items & 1, p.err, kErrWaitSoftmax);
             // Two warpgroups: P V of tile j - 2, whose P lies in the buffer of S(j), goes before
-            // S(j).  One: S(j) goes first, so that it runs during the softmax of tile j - 1.
+            // S(j).  One: S(j) goes first, so that it runs during the softmax of tile j - 1.  But
+            // the softmax clears V rows of a last tile that the keys do not fill, and tells by the
+            // parity of v_full that they have landed.  With one V slot that parity is the one of
+            // tile j - 2, so tile j - 1 must have landed before S(j) can be seen: P V of tile
+            // j - 1, issued after a wait for it, goes first there.
+            const bool v_first = NG == 1 && ST == 1 && (it.key_hi - it.key_lo) % BN != 0;
             for (int j = 0; j < it.n_tiles && ok; ++j) {
                 const int g = g0 + j, st = g % ST;
-                if (NG == 2 && j >= 2 && !(ok = issue_pv(j - 2))) break;
+                const bool pv_first = NG == 2 ? j >= 2 : v_first && j >= 1 && j + 1 == it.n_tiles;
+                if (pv_first && !(ok = issue_pv(j - NG))) break;
                 if (!(ok = mbar_wait_warp(smem_u32(&bars->k_full[st]), (g / ST) & 1, p.err, kErrWaitTmaFull))) break;
                 tc_fence_after();
                 const uint32_t k_addr = smem_u32(sK + st * S::kKvBytes);
@@ -422,7 +428,7 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
                     }
                 umma_commit_elect(smem_u32(&bars->s_full[g & 1]));
                 umma_commit_elect(smem_u32(&bars->k_empty[st]));
-                if (NG == 1 && j >= 1) ok = issue_pv(j - 1);
+                if (NG == 1 && j >= 1 && !pv_first) ok = issue_pv(j - 1);
             }
             if (ok && NG == 2 && it.n_tiles >= 2) ok = issue_pv(it.n_tiles - 2);
             if (ok) ok = issue_pv(it.n_tiles - 1);
@@ -614,6 +620,8 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
                 l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
                 // Rows of the V tile past the part's last key may hold anything (another
                 // sequence's rows, unwritten memory): 0 * NaN would reach O, so they are zeroed.
+                // (P V of the tile before in this slot was issued before S(g), so its phase of
+                // v_full is over and the parity names this tile's.)
                 if (nv < BN) {
                     ok = mbar_wait_warp(smem_u32(&bars->v_full[g % ST]), (g / ST) & 1, p.err, kErrWaitTmaFull);
                     if (!ok) break;
