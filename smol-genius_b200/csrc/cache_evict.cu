@@ -148,6 +148,9 @@ __global__ void __launch_bounds__(kMaxThreads) evict_kernel(const __grid_constan
         return;
     }
 
+    // A CTA's shared memory may be written from another one only once it runs: the first join()
+    // waits for every CTA of the cluster, whose arrivals pass while the slots are loaded.
+    if (C > 1) cluster_arrive();
     uint32_t key[ITEMS];   // 0 past the last slot: below every candidate
     {
         float w[ITEMS];
@@ -165,6 +168,7 @@ __global__ void __launch_bounds__(kMaxThreads) evict_kernel(const __grid_constan
             key[i] = j >= n ? 0u : pos < p.sink || pos >= seen - p.recent ? 0xffffffffu : weight_key(w[i]);
         }
     }
+    if (C > 1) cluster_wait();
     // Six sums (and, for `maxima`, two maxima) over all threads of the cluster.  A warp-wide
     // reduction takes a scheduler some 35 cycles, so a warp's six counts go in two of them and
     // one warp each adds up the warps' results.

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import smol_b200
+from test_cache_evict_gpu import Evict
 from test_cache_shared_gpu import Case, no_error
 
 pytestmark = pytest.mark.gpu
@@ -54,4 +55,56 @@ def test_last_tile_of_a_ragged_prefix(cuda, plen, hq, hkv, hd, bf16):
         c.out.fill_(7.0)
         call()
         assert torch.equal(c.out, first)
+    no_error()
+
+
+# ---------------------------------------------------------------------------
+# eviction by clusters
+# ---------------------------------------------------------------------------
+class EvictCall:
+    """The eviction of an Evict case as a call without arguments, and its buffers."""
+
+    def __init__(self, c, budget, sink=0, recent=0, in_place=True, max_len=None):
+        self.c, maxl = c, c.max_len if max_len is None else max_len
+        self.start = [c.k.clone(), c.v.clone(), c.dev(c.w, torch.float32), c.dev(c.pos, torch.int32),
+                      c.dev(c.lens, torch.int32)]
+        w, pos, lens = (x.clone() for x in self.start[2:])
+        wo, po, lo = (w, pos, lens) if in_place else (torch.full_like(w, 7.0), torch.full_like(pos, 77), lens.clone())
+        self.ins, self.outs = [c.k, c.v, w, pos, lens], [c.k, c.v, wo, po, lo]
+        ws = torch.full((smol_b200.cache_evict_workspace_bytes(c.n, maxl, c.hkv),), 255, dtype=torch.uint8, device=c.cuda)
+        self.args = (c.k, c.v, c.rows, c.dev(c.row0, torch.int64), w, wo, pos, po, c.stride, lens, lo,
+                     c.dev(c.seen, torch.int32), c.n, maxl, c.hkv, c.hd, budget, sink, recent, ws)
+
+    def reset(self):
+        for x, x0 in zip(self.ins, self.start):
+            x.copy_(x0)
+
+    def __call__(self):
+        smol_b200.cache_evict(*self.args)
+
+    def results(self):
+        return [x.clone() for x in self.outs]
+
+
+@pytest.mark.parametrize("units,n,budget", [(1, 5000, 4000), (8, 17000, 2048), (18, 9000, 100), (40, 3000, 2999),
+                                            (3, 140000, 70000)])
+def test_evict_clusters_many_times(cuda, units, n, budget):
+    # the CTAs of many clusters start at different times: other work holds SMs while they are launched
+    c = Evict(cuda, [n], units, 8, seed=units)
+    call = EvictCall(c, budget, 4, 30)
+    c.run(budget, 4, 30, in_place=True)      # against the plain form; moves c's rows in place
+    want = [c.k.clone(), c.v.clone()]
+    other, busy = torch.cuda.Stream(), torch.randn((3001, 3001), device=cuda)
+    for i in range(100):
+        call.reset()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            busy * 1.5 if i % 2 else busy @ busy
+        call()
+        torch.cuda.synchronize()
+        got = call.results()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        if i == 0:
+            want += got[2:]
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(got, want))
     no_error()
