@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kMaxThreads) evict_kernel(const __grid_constan
     const int seen = p.seq_pos[b];
     const int n = min(max(length, 0), p.max_kv_len);
     // a length or rows that cannot be: the sequence is left as it is
-    const bool bad = n != length || (n > p.budget && (row0 < 0 || row0 + n > p.pool_rows));
+    const bool bad = n != length || (n > p.budget && (row0 < 0 || row0 > p.pool_rows - n));
     const bool keep_all = bad || n <= p.budget;
     const int B = keep_all ? length : p.budget;
     const long long unit = static_cast<long long>(b) * p.n_kv_heads + h;

@@ -108,3 +108,20 @@ def test_evict_clusters_many_times(cuda, units, n, budget):
             want += got[2:]
         assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(got, want))
     no_error()
+
+
+@pytest.mark.parametrize("row0", [-1, -(1 << 63), (1 << 63) - 1, (1 << 63) - 300, 1 << 32])
+def test_evict_flags_rows_anywhere_outside_the_pool(cuda, row0):
+    c = Evict(cuda, [300, 200], 2, 16, seed=33)
+    k0, v0 = c.k.clone(), c.v.clone()
+    call = EvictCall(c, 50, 0, 4)
+    call.args[3][0] = row0
+    call()
+    torch.cuda.synchronize()
+    assert smol_b200.device_error() == 1 << 5
+    smol_b200.clear_error()
+    k, v, w, pos, lens = call.results()
+    r1 = int(c.row0[1])
+    assert torch.equal(k[:r1], k0[:r1]) and torch.equal(v[:r1], v0[:r1]) and not torch.equal(k[r1:], k0[r1:])
+    assert lens.tolist() == [300, 50]
+    assert torch.equal(w[0].cpu(), torch.from_numpy(c.w[0])) and torch.equal(pos[0].cpu(), torch.from_numpy(c.pos[0]))
