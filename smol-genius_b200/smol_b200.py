@@ -561,8 +561,22 @@ def layer_norm(out, x, w, b, rows, hidden, eps, out_bf16=False, stream=None):
 # Part 6: shared prefixes, attention weights, eviction
 # ---------------------------------------------------------------------------
 def _dev(t) -> int | None:
-    """Address of a tensor (None -> NULL); what _ptr does, for tensors alone."""
-    return None if t is None else t.data_ptr()
+    """Address of a tensor, or a raw device address (None -> NULL); _ptr without the tests that a tensor needs none of."""
+    try:
+        return t.data_ptr()
+    except AttributeError:
+        if t is None or isinstance(t, int):
+            return t
+        raise
+
+
+def _is_bf16(torch, t, what) -> bool:
+    """Whether a query or output tensor is bf16; any type but bf16 and fp32 would be read or written as if it were fp32."""
+    if t.dtype == torch.bfloat16:
+        return True
+    if t.dtype == torch.float32:
+        return False
+    raise TypeError(f"{what} must be float32 or bfloat16, not {t.dtype}")
 
 
 def decode_shared_workspace_bytes(n_seqs, max_kv_len, n_prefixes, max_prefix_len, max_prefix_seqs, n_heads, n_kv_heads,
@@ -579,7 +593,7 @@ def decode_attention_shared(out, q, k_pool, v_pool, pool_rows, prefix_row0, pref
     [n_prefixes], prefix_seq0 int32 [n_prefixes + 1]; weights fp32 [n_seqs, n_kv_heads, weights_stride] or None."""
     import torch
     rc = lib().smol_b200_decode_attention_shared(
-        _stream(stream), _dev(out), out.dtype == torch.bfloat16, _dev(q), q.dtype == torch.bfloat16,
+        _stream(stream), _dev(out), _is_bf16(torch, out, "out"), _dev(q), _is_bf16(torch, q, "q"),
         _dev(k_pool), _dev(v_pool), pool_rows, _dev(prefix_row0), _dev(prefix_len), _dev(prefix_seq0), n_prefixes,
         max_prefix_len, max_prefix_seqs, _dev(seq_row0), _dev(kv_len), n_seqs, max_kv_len, n_heads, n_kv_heads,
         head_dim, scale, window, softcap, _dev(weights_in), _dev(weights_out), weights_stride, _dev(workspace),
@@ -598,7 +612,7 @@ def decode_attention_weights(out, q, k_pool, v_pool, pool_rows, seq_row0, kv_len
     head) to weights_in (None: zero), into weights_out (may be weights_in)."""
     import torch
     rc = lib().smol_b200_decode_attention_weights(
-        _stream(stream), _dev(out), out.dtype == torch.bfloat16, _dev(q), q.dtype == torch.bfloat16,
+        _stream(stream), _dev(out), _is_bf16(torch, out, "out"), _dev(q), _is_bf16(torch, q, "q"),
         _dev(k_pool), _dev(v_pool), pool_rows, _dev(seq_row0), _dev(kv_len), n_seqs, max_kv_len, n_heads, n_kv_heads,
         head_dim, scale, window, softcap, _dev(weights_in), _dev(weights_out), weights_stride, _dev(workspace),
         workspace.nbytes)

@@ -213,3 +213,44 @@ def test_shared_workspaces_never_shrink(n_prefixes, most, hq, hkv):
         size = smol_b200.decode_shared_workspace_bytes(n_prefixes * most, 100, n_prefixes, n, most, hq, hkv, 128)
         assert size >= prev
         prev = size
+
+
+@pytest.mark.parametrize("which", ["out", "q"])
+@pytest.mark.parametrize("dtype", ["float16", "float64", "int32", "uint8"])
+@pytest.mark.parametrize("call", ["shared", "weights"])
+def test_binding_refuses_types_of_queries_and_outputs(monkeypatch, which, dtype, call):
+    import torch
+    rec = Recorder()
+    monkeypatch.setattr(smol_b200, "_lib", rec)
+    t = dict(out=torch.zeros(8), q=torch.zeros(8, dtype=torch.bfloat16))
+    ws = torch.zeros(40, dtype=torch.uint8)
+
+    def run():
+        if call == "shared":
+            smol_b200.decode_attention_shared(t["out"], t["q"], P, P, 11, P, P, P, 2, 21, 22, P, P, 3, 12, 16, 8, 128, 0.5,
+                                              ws)
+        else:
+            smol_b200.decode_attention_weights(t["out"], t["q"], P, P, 11, P, P, 3, 12, 16, 8, 128, 0.5, None, P, 15, ws)
+
+    run()
+    assert rec.last[1][2] == 0 and rec.last[1][4] == 1      # out fp32, q bf16
+    del rec.last
+    t[which] = t[which].to(getattr(torch, dtype))
+    with pytest.raises(TypeError, match=which):
+        run()
+    assert "last" not in vars(rec)      # the library was not called
+
+
+def test_binding_takes_raw_addresses(monkeypatch):
+    import numpy as np
+    import torch
+    rec = Recorder()
+    monkeypatch.setattr(smol_b200, "_lib", rec)
+    ws = torch.zeros(40, dtype=torch.uint8)
+    smol_b200.prefill_attention_weights(None, P, 15, P + 16, P + 32, 4, 5, 6, 16, 8, 128, 0.5, ws)
+    name, args = rec.last
+    assert name == "smol_b200_prefill_attention_weights" and (args[1], args[2], args[4], args[7]) == (None, P, P + 16, P + 32)
+    smol_b200.cache_evict(P, P + 16, 11, P, P, P, P, P, 15, P, P, P, 3, 12, 8, 128, 41, 42, 43, ws)
+    assert rec.last[1][1] == P and rec.last[1][2] == P + 16
+    with pytest.raises(AttributeError):     # a host array is no device address
+        smol_b200.cache_evict(np.zeros(4), P, 11, P, P, P, P, P, 15, P, P, P, 3, 12, 8, 128, 41, 42, 43, ws)
