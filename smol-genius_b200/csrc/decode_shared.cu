@@ -20,8 +20,10 @@
 // Precision.  Scores, maxima, sums and outputs of the parts are fp32.  K is bf16 and V
 // fp16 in the cache.  fp32 queries enter the bf16 products as three bf16 terms (24 bits:
 // two left the scores 4e-6 off), bf16 queries as they are.  The probabilities multiply V
-// as fp16: one term (2^-12) where the output is rounded to bf16 (2^-9) anyway, the value
-// and its remainder (2^-23) where the output is fp32.
+// as an fp16 value and its remainder (2^-23), for bf16 outputs too: their one rounding is
+// that of the output.  (The value alone is 2^-12 off, which turned one bf16 output in 25 to
+// its neighbour; the remainder costs 64 sequences on 8192 shared keys 48.6 us against 46.4,
+// 64 sequences of 1024 to 8192 own keys 202.6 against 201.2.)
 #include <string.h>
 
 #include <mutex>
@@ -122,7 +124,7 @@ __device__ __forceinline__ void own_range(const SharedParams &p, int b, int &ks,
 // softmax warpgroups of one packed row per thread (thread = TMEM lane), a TMA producer warp
 // that runs ahead into the next item, and a tcgen05 issuer warp.
 //   S = Q K^T  (QT bf16 terms of Q, fp32 in TMEM, two buffers)
-//   P = 2^(S*scale*log2e - m) as PT fp16 terms over S's columns
+//   P = 2^(S*scale*log2e - m) as an fp16 value and its remainder over S's columns
 //   O += P V
 // Head dims 64 and 128 run two softmax warpgroups on alternate key tiles, each with an O
 // and a reference point of its own, joined at the end: the exponentials of a tile take
@@ -273,7 +275,7 @@ __device__ __forceinline__ PrefixItem prefix_item(const SharedParams &p, const P
     return it;
 }
 
-template <int HD, int QT, int PT>
+template <int HD, int QT>
 __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kernel(const __grid_constant__ SharedParams p)
 {
     using S = PrefixShape<HD, QT>;
@@ -383,13 +385,13 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
             tc_fence_after();
             const uint32_t v_addr = smem_u32(sV + st * S::kKvBytes);
 #pragma unroll
-            for (int t = PT - 1; t >= 0; --t)   // the remainders first: the smaller sums
+            for (int t = 1; t >= 0; --t)   // the remainders first: the smaller sums
 #pragma unroll
                 for (int kk = 0; kk < BN / 16; ++kk) {
                     const uint64_t bd = umma_sdesc_sw128(v_addr + kk * 16 * 128, S::kKvSubBytes, 1024);
                     // columns of P: see the softmax (32-key groups: 16 of values, 16 of remainders)
                     umma_ts_elect(tmem + S::kTmO + (g % NG) * HD, tmem + sb * BN + (kk >> 1) * 32 + t * 16 + (kk & 1) * 8, bd,
-                                  idesc_pv, (j >= NG || t < PT - 1 || kk > 0) ? 1u : 0u);
+                                  idesc_pv, (j >= NG || t < 1 || kk > 0) ? 1u : 0u);
                 }
             umma_commit_elect(smem_u32(&bars->o_done[g % NG]));
             umma_commit_elect(smem_u32(&bars->v_empty[st]));
@@ -593,7 +595,7 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
                 if (move) m = mx;
                 const float negm = m != -INFINITY ? -m : 0.f;
                 // P over S, in place by groups: columns 32q .. 32q+15 take the fp16 pairs of the
-                // group's 32 keys, 32q+16 .. 32q+31 what their rounding left (PT == 2).
+                // group's 32 keys, 32q+16 .. 32q+31 what their rounding left.
                 float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
                 for (int q = 0; q < BN / 32; ++q) {
@@ -612,8 +614,7 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
                         const float e0 = fast_exp2f(fmaf(__uint_as_float(rr[2 * i]), mul, negm));
                         const float e1 = fast_exp2f(fmaf(__uint_as_float(rr[2 * i + 1]), mul, negm));
                         acc[i & 3] += e0 + e1;
-                        if (PT == 2) split_f16(e0, e1, w[i], w[16 + i]);
-                        else w[i] = pack_f16x2(e0, e1), w[16 + i] = 0u;
+                        split_f16(e0, e1, w[i], w[16 + i]);
                     }
                     tmem_st32(s_col + q * 32, w);
                 }
@@ -734,7 +735,7 @@ struct SplitShape {
     static constexpr int kSmemBytes = kStages * kStageBytes + kQBytes + 256 + 1024;
 };
 
-template <int HD, int QT, int PT>
+template <int HD, int QT>
 __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_constant__ SharedParams p)
 {
     using S = SplitShape<HD>;
@@ -952,18 +953,13 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
                 o[i][2] *= corr0;
                 o[i][3] *= corr1;
             }
-            uint32_t pb[PT][2];   // P^T as B fragments, keys 0-7 and 8-15
+            uint32_t pb[2][2];   // P^T as B fragments, keys 0-7 and 8-15: values, remainders
             {
-                uint32_t h0, h1, r0 = 0, r1 = 0;
-                if (PT == 2) {
-                    split_f16(p0, p1, h0, r0);
-                    split_f16(p2, p3, h1, r1);
-                    pb[PT - 1][0] = movmatrix_t(r0);
-                    pb[PT - 1][1] = movmatrix_t(r1);
-                } else {
-                    h0 = pack_f16x2(p0, p1);
-                    h1 = pack_f16x2(p2, p3);
-                }
+                uint32_t h0, h1, r0, r1;
+                split_f16(p0, p1, h0, r0);
+                split_f16(p2, p3, h1, r1);
+                pb[1][0] = movmatrix_t(r0);
+                pb[1][1] = movmatrix_t(r1);
                 pb[0][0] = movmatrix_t(h0);
                 pb[0][1] = movmatrix_t(h1);
             }
@@ -984,7 +980,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
                     a3 &= mhi;
                 }
 #pragma unroll
-                for (int q = PT - 1; q >= 0; --q) mma_f16_16816(o[db], a0, a1, a2, a3, pb[q][0], pb[q][1]);
+                for (int q = 1; q >= 0; --q) mma_f16_16816(o[db], a0, a1, a2, a3, pb[q][0], pb[q][1]);
             }
         }
         __syncwarp();
@@ -1386,7 +1382,7 @@ bool allow_smem(const void *kernel, int bytes)
     return true;
 }
 
-template <int HD, int QT, int PT>
+template <int HD, int QT>
 int launch_shared(cudaStream_t st, SharedParams &p, const uint16_t *k_pool, const uint16_t *v_pool, int64_t pool_rows)
 {
     const int kv_dim = p.n_kv_heads * HD;
@@ -1407,20 +1403,20 @@ int launch_shared(cudaStream_t st, SharedParams &p, const uint16_t *k_pool, cons
     if (p.prefix_items > 0) {
         using S = PrefixShape<HD, QT>;
         if (!maps(box_rows = S::kBoxRows) ||
-            !allow_smem(reinterpret_cast<const void *>(prefix_kernel<HD, QT, PT>), S::kSmemBytes))
+            !allow_smem(reinterpret_cast<const void *>(prefix_kernel<HD, QT>), S::kSmemBytes))
             return SMOL_B200_ERR_CUDA;
         const dim3 grid(static_cast<unsigned>(p.prefix_items < p.prefix_ctas ? p.prefix_items : p.prefix_ctas));
-        if (launch_kernel(prefix_kernel<HD, QT, PT>, grid, dim3(S::kThreads), S::kSmemBytes, st, p) != cudaSuccess)
+        if (launch_kernel(prefix_kernel<HD, QT>, grid, dim3(S::kThreads), S::kSmemBytes, st, p) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
     }
     if (p.max_kv_len > 0 || p.prefix_units > 0) {
         using S = SplitShape<HD>;
         if ((box_rows != kKeysPerTile && !maps(kKeysPerTile)) ||
-            !allow_smem(reinterpret_cast<const void *>(split_kernel<HD, QT, PT>), S::kSmemBytes))
+            !allow_smem(reinterpret_cast<const void *>(split_kernel<HD, QT>), S::kSmemBytes))
             return SMOL_B200_ERR_CUDA;
         const int parts = p.prefix_units > 0 && p.prefix_slots > p.max_chunks ? p.prefix_slots : p.max_chunks;
         const dim3 grid(parts, p.n_kv_heads * p.n_qgroups, p.prefix_units + p.n_seqs);
-        if (launch_kernel(split_kernel<HD, QT, PT>, grid, dim3(kSplitThreads), S::kSmemBytes, st, p) != cudaSuccess)
+        if (launch_kernel(split_kernel<HD, QT>, grid, dim3(kSplitThreads), S::kSmemBytes, st, p) != cudaSuccess)
             return SMOL_B200_ERR_CUDA;
     }
     if (launch_kernel(merge_kernel<HD>, dim3(static_cast<unsigned>(out_blocks + key_blocks)), dim3(kMergeThreads), 0, st, p,
@@ -1432,9 +1428,7 @@ int launch_shared(cudaStream_t st, SharedParams &p, const uint16_t *k_pool, cons
 template <int HD>
 int launch_shared_hd(cudaStream_t st, SharedParams &p, const uint16_t *k, const uint16_t *v, int64_t rows)
 {
-    if (p.q_is_bf16)
-        return p.out_is_bf16 ? launch_shared<HD, 1, 1>(st, p, k, v, rows) : launch_shared<HD, 1, 2>(st, p, k, v, rows);
-    return p.out_is_bf16 ? launch_shared<HD, 3, 1>(st, p, k, v, rows) : launch_shared<HD, 3, 2>(st, p, k, v, rows);
+    return p.q_is_bf16 ? launch_shared<HD, 1>(st, p, k, v, rows) : launch_shared<HD, 3>(st, p, k, v, rows);
 }
 
 bool sizes_ok(int n_seqs, int max_kv_len, int n_heads, int n_kv_heads, int head_dim)
