@@ -21,7 +21,7 @@
 // fp16 in the cache.  fp32 queries enter the bf16 products as three bf16 terms (24 bits:
 // two left the scores 4e-6 off), bf16 queries as they are.  The probabilities multiply V
 // as an fp16 value and its remainder (2^-23), for bf16 outputs too: their one rounding is
-// that of the output.  (The value alone is 2^-12 off, which turned one bf16 output in 25 to
+// that of the output.  (The value alone is 2^-12 off, which turned one bf16 output in 11 to
 // its neighbour; the remainder costs 64 sequences on 8192 shared keys 48.6 us against 46.4,
 // 64 sequences of 1024 to 8192 own keys 202.6 against 201.2.)
 #include <string.h>
@@ -132,7 +132,11 @@ __device__ __forceinline__ void own_range(const SharedParams &p, int b, int &ks,
 // whose O fills half of TMEM, runs one.
 // Row r of tile t is query head (r' % group) of sequence s0 + r'/group, r' = 128 t + r.
 constexpr int kBM = 128;
-constexpr float kMoveLog2 = 8.0f;
+// A row's reference point lies kHeadLog2 below the maximum it is taken from and moves when a
+// later maximum lies kMoveLog2 above that one, so the largest probability of a row is 2^7 to 2^15:
+// fp16 holds 65504, and what its steps of 2^-24 below 2^-14 cost a small probability counts
+// against 2^7 (with the maximum at 1, 900 keys at 2^-22.3 beside a sink without value were 8 % off).
+constexpr float kHeadLog2 = 7.0f, kMoveLog2 = 8.0f;
 
 template <int HD, int QT>
 struct PrefixShape {
@@ -570,9 +574,10 @@ __global__ void __launch_bounds__(PrefixShape<HD, QT>::kThreads, 1) prefix_kerne
                 } else {
                     mx *= mul;
                 }
-                // The reference m of a row is the first maximum it meets; it moves only when a
-                // maximum passes it by more than 2^8 (P stays below 256 in fp16), so O is rescaled
-                // rarely.  NaN scores keep m and reach P.
+                // The reference m of a row comes from the first maximum it meets; it moves only when
+                // a maximum passes that one by more than 2^8 (P stays below 2^15 in fp16), so O is
+                // rescaled rarely.  NaN scores keep m and reach P.
+                mx -= kHeadLog2;
                 const bool fresh = m == -INFINITY;
                 const bool move = mx > m + kMoveLog2 || (fresh && mx != -INFINITY);
                 if (j >= NG && __any_sync(0xffffffffu, move && !fresh)) {
@@ -721,6 +726,7 @@ constexpr int kKeysPerTile = 64;
 constexpr int kConsumerWarps = 4;
 constexpr int kSplitThreads = (kConsumerWarps + 1) * 32;
 constexpr int kSubtileBytes = kKeysPerTile * 128;
+constexpr float kTopLog2 = 15.0f;   // the largest probability so far is 2^15 (fp16 holds 65504): see kHeadLog2
 
 template <int HD>
 struct SplitShape {
@@ -936,7 +942,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
                 mb0 = fmaxf(mb0, __shfl_xor_sync(0xffffffffu, mb0, off));
                 mb1 = fmaxf(mb1, __shfl_xor_sync(0xffffffffu, mb1, off));
             }
-            const float mn0 = fmaxf(m_run[0], mb0), mn1 = fmaxf(m_run[1], mb1);
+            // reference points: the maximum less kTopLog2
+            const float mn0 = fmaxf(m_run[0], mb0 - kTopLog2), mn1 = fmaxf(m_run[1], mb1 - kTopLog2);
             // a row whose scores are all -inf so far keeps exponentials of exactly 0
             const float n0 = mn0 == -INFINITY ? 0.f : -mn0, n1 = mn1 == -INFINITY ? 0.f : -mn1;
             const float corr0 = fast_exp2f(m_run[0] + n0), corr1 = fast_exp2f(m_run[1] + n1);

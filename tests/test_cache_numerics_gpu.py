@@ -66,3 +66,44 @@ def test_bf16_output_is_rounded_once(cuda, hq, hkv, hd, seqs, plen):
         bad = (got < lo) | (got > hi)
         assert not bad.any(), (b, int(bad.sum()), bad.numel())
     no_error()
+
+
+# ---------------------------------------------------------------------------
+# a key that takes nearly all of a row but has no value (an attention sink): the others, each far
+# below it, are the whole output
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("hq,hkv,hd", [(16, 8, 128), (8, 1, 256), (4, 2, 64)])
+@pytest.mark.parametrize("below", [6.3, 14.3, 19.3, 22.3])
+@pytest.mark.parametrize("seqs,where", [(3, "own"), (3, "prefix"), (30, "prefix")])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_values_far_below_a_sink(cuda, hq, hkv, hd, below, seqs, where, bf16):
+    # scores in log2 units are 0 for the sink and -below for every other key.  A probability multiplies V
+    # as an fp16 value and its remainder, both subnormal below 2^-14: the bound of test_cache_shared_gpu.py
+    # plus 2^-32 of the largest probability (that of a value of at least 2^7 before fp16's 2^-25) for
+    # each key that is visible
+    own, plen = (900, 40) if where == "own" else (3, 900)
+    c = Case(cuda, [own] * seqs, plens=[plen], cut=[0, seqs], hq=hq, hkv=hkv, hd=hd, q_bf16=bf16, out_bf16=bf16, seed=42)
+    q = torch.zeros_like(c.q).view(seqs, hq, hd)
+    q[..., 0] = 1.0
+    c.q = q.view(seqs, hq * hd)
+    step = below / 1.4426950408889634 / c.scale      # of a key's first element, q is 1 there
+    firsts = c.first if where == "own" else c.pfirst
+    for r, n in list(zip(c.pfirst, c.plens)) + list(zip(c.first, c.lens)):
+        k = torch.zeros((n, hkv, hd), device=cuda)
+        k[..., 0] = -step
+        v = 1.0 + torch.rand((n, hkv, hd), device=cuda)
+        if r in firsts:
+            k[0] = v[0] = 0.0
+        c.k[r:r + n] = k.view(n, -1).to(torch.bfloat16)
+        c.v[r:r + n] = v.view(n, -1).to(torch.float16)
+    c.run()
+    for b in range(seqs):
+        want, tol = head_bounds(c, b)
+        _, _, p, v = reference(c, b)
+        tol = tol + p.shape[-1] * 2.0 ** -32 * p.amax(dim=-1, keepdim=True) * float(v.max())
+        got = c.out[b].double().view(want.shape)
+        if bf16:
+            tol = tol + 2.0 ** -8 * want.abs()
+        bad = (got - want).abs() > tol
+        assert not bad.any(), (b, int(bad.sum()), float(((got - want).abs() / tol).max()))
+    no_error()
