@@ -1098,12 +1098,12 @@ __device__ __forceinline__ void head_sum(const SharedParams &p, const float2 *ml
         float mx = v.x;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        if (mx == -INFINITY) continue;
         const float top = fmaxf(M, mx);
-        float s = v.x == -INFINITY ? 0.f : fast_exp2f(v.x - top) * v.y;
+        // without a reference: an empty part (sum 0), or one whose scores are all NaN (sum NaN)
+        float s = v.x == -INFINITY ? v.y : fast_exp2f(v.x - top) * v.y;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        L = (M == -INFINITY ? 0.f : L * fast_exp2f(M - top)) + s;
+        L = (M == -INFINITY ? L : L * fast_exp2f(M - top)) + s;
         M = top;
     }
     inv = L != 0.f ? 1.f / L : 0.f;   // NaN stays NaN

@@ -107,3 +107,38 @@ def test_values_far_below_a_sink(cuda, hq, hkv, hd, below, seqs, where, bf16):
         bad = (got - want).abs() > tol
         assert not bad.any(), (b, int(bad.sum()), float(((got - want).abs() / tol).max()))
     no_error()
+
+
+# ---------------------------------------------------------------------------
+# NaN scores reach every output and weight that the formula gives NaN, and no other
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("hq,hkv,hd", [(16, 8, 128), (8, 1, 256), (4, 2, 64)])
+@pytest.mark.parametrize("kind", ["query", "own key alone in a part", "own key beside others", "only key", "first prefix key",
+                                  "prefix key alone in a part", "own key of one head"])
+@pytest.mark.parametrize("seqs", [2, 30])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_nan_scores(cuda, hq, hkv, hd, kind, seqs, bf16):
+    # 65 own keys: the last is alone in its tile, and in its part where a part is 64 keys; 129 prefix
+    # keys: alone in a part of 128 (tensor-core form) or in a tile
+    lens = [65, 1] + [7 + i % 3 for i in range(seqs - 2)]
+    plens = [] if kind == "only key" else [129]
+    c = Case(cuda, lens, plens=plens, cut=[0, seqs] if plens else [0], hq=hq, hkv=hkv, hd=hd, q_bf16=bf16, out_bf16=bf16,
+             seed=43)
+    nan = float("nan")
+    if kind == "query":
+        c.q[0, hd:2 * hd] = nan
+    elif kind == "only key":
+        c.k[c.first[1], :hd] = nan
+    elif kind.startswith("own key"):
+        at, cols = {"own key alone in a part": (64, slice(None)), "own key beside others": (3, slice(None)),
+                    "own key of one head": (64, slice((hkv - 1) * hd, hkv * hd))}[kind]
+        c.k[c.first[0] + at, cols] = nan
+    else:
+        c.k[c.pfirst[0] + (0 if kind.startswith("first") else 128), :hd] = nan
+    w = c.run("zero")
+    for b in range(seqs):
+        want, add, _, _ = reference(c, b)
+        got = c.out[b].view(want.shape)
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), b
+        assert torch.equal(torch.isnan(w[b, :, :lens[b]]), torch.isnan(add)), b
+    no_error()
