@@ -275,6 +275,17 @@ __device__ int step_pieces(const WParams &p, int mode, int kstay, int unit, int 
     return pieces_at(f, t1 - t0, p.run);
 }
 
+// A piece (reference, sum) of a row's statistics counted from M.  Without a reference its sum is
+// 0 (no key seen) or NaN (every score is), which has to reach the row.
+__device__ __forceinline__ float piece_sum(float2 v, float M)
+{
+    return v.x == -INFINITY ? v.y : v.y * fast_exp2f(v.x - M);
+}
+__device__ __forceinline__ float negative_lse(float M, float L)
+{
+    return M == -INFINITY && L == 0.f ? -INFINITY : -(M + log2f(L));
+}
+
 __device__ __forceinline__ const float *lse_of(const WParams &p, int unit, int row_tile)
 {
     return p.nlse + (static_cast<long long>(unit) * p.row_tiles + row_tile) * kTile;
@@ -569,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                         l = 0.f;
                         for (int i = 0; i < kGroups; ++i) {
                             const float2 v = box[i * kTile + r];
-                            if (v.x != -INFINITY) l += v.y * fast_exp2f(v.x - m);
+                            l += piece_sum(v, m);
                         }
                     }
                 }
@@ -596,11 +607,11 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                     if (row < rows)
                         for (int c = part; c < pieces; c += 4) {
                             const float2 v = src[c];
-                            if (v.x != -INFINITY) L += v.y * fast_exp2f(v.x - M);
+                            L += piece_sum(v, M);
                         }
                     L += __shfl_xor_sync(0xffffffffu, L, 1);
                     L += __shfl_xor_sync(0xffffffffu, L, 2);
-                    if (part == 0) ring[one_slot * kTile + row] = M == -INFINITY ? -INFINITY : -(M + log2f(L));
+                    if (part == 0) ring[one_slot * kTile + row] = negative_lse(M, L);
                     named_bar_sync(1, kExpThreads);   // the slot before is still read: two in turn
                 }
                 float sum = 0.f;
@@ -669,12 +680,11 @@ __global__ void __launch_bounds__(256) weights_lse_kernel(const __grid_constant_
     if (valid)
         for (int c = lane; c < n; c += width) {
             const float2 v = src[c];
-            if (v.x != -INFINITY) L += v.y * fast_exp2f(v.x - M);
+            L += piece_sum(v, M);
         }
     for (int o = width / 2; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     if (lane == 0)
-        p.nlse[(static_cast<long long>(unit) * p.row_tiles + tile) * kTile + in_tile] =
-            M == -INFINITY ? -INFINITY : -(M + log2f(L));
+        p.nlse[(static_cast<long long>(unit) * p.row_tiles + tile) * kTile + in_tile] = negative_lse(M, L);
 }
 
 // weights_out = weights_in + the pieces of each key tile, in order (kstay 0: a copy).

@@ -142,3 +142,38 @@ def test_nan_scores(cuda, hq, hkv, hd, kind, seqs, bf16):
         assert torch.equal(torch.isnan(got), torch.isnan(want)), b
         assert torch.equal(torch.isnan(w[b, :, :lens[b]]), torch.isnan(add)), b
     no_error()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,keys,mask,window,at", [
+    (129, 129, 0, 0, 128),      # the last row's own key, alone in its tile
+    (300, 300, 0, 0, 256), (257, 257, 3, 0, 256), (300, 513, 3, 0, 512), (300, 513, 0, 100, 511),
+    (1, 129, 0, 0, 128), (20, 257, 3, 0, 256), (40, 1025, 3, 0, 1024), (7, 300, 0, 3, 298), (3, 1, 3, 0, 0),
+    (300, 300, 1, 0, 299), (64, 64, 0, 0, 63)])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_prompt_nan_key(cuda, hd, rows, keys, mask, window, at, cap):
+    hq, hkv = 4, 2
+    g = torch.Generator(device=cuda).manual_seed(44)
+    q = torch.randn((1, rows, hq * hd), device=cuda, generator=g).to(torch.bfloat16)
+    k = torch.randn((1, keys, hkv * hd), device=cuda, generator=g).to(torch.bfloat16)
+    k[0, at, :hd] = float("nan")
+    w = torch.full((1, hkv, keys), -3.0, device=cuda)
+    ws = torch.full((smol_b200.prefill_weights_workspace_bytes(1, rows, keys, hq, hkv, hd),), 255, dtype=torch.uint8,
+                    device=cuda)
+    prefix = keys // 2 if mask == 1 else 0
+    smol_b200.prefill_attention_weights(None, w, keys, q, k, 1, rows, keys, hq, hkv, hd, hd ** -0.5, ws, mask_kind=mask,
+                                        q_offset=keys - rows, prefix_len=prefix, window=window, softcap=cap)
+    torch.cuda.synchronize()
+    j, pos = torch.arange(keys, device=cuda), torch.arange(keys - rows, keys, device=cuda)[:, None]
+    see = {0: j <= pos, 1: (j <= pos) | (j < prefix), 3: j < keys + 0 * pos}[mask]
+    if window > 0:
+        see = see & (j > pos - window)
+    for h in range(hkv):
+        want = torch.zeros(keys, dtype=torch.float64, device=cuda)
+        for hh in (2 * h, 2 * h + 1):
+            x = q[0, :, hh * hd:(hh + 1) * hd].double() @ k[0, :, h * hd:(h + 1) * hd].double().T * hd ** -0.5
+            x = cap * torch.tanh(x / cap) if cap > 0 else x
+            p = torch.softmax(x.masked_fill(~see, -float("inf")), dim=-1)
+            want += torch.where(see, p, torch.zeros_like(p)).sum(dim=0)
+        assert torch.equal(torch.isnan(w[0, h]), torch.isnan(want)), h
+    no_error()
