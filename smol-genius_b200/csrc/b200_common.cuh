@@ -424,6 +424,8 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 // and its writes are visible).  griddep_trigger() lets the successor launch; the
 // kernels here trigger after their own wait, so at most one grid waits ahead of the
 // running one (triggering on entry lets a chain of waiting grids fill the SMs).
+// One kernel skips its own wait: the split kernel of the shared decode, after a prefix kernel
+// whose CTAs all trigger behind their wait; it reads its inputs past L1.
 // Both are no-ops for a kernel launched without the attribute.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

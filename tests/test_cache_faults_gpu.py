@@ -125,3 +125,73 @@ def test_evict_flags_rows_anywhere_outside_the_pool(cuda, row0):
     assert torch.equal(k[:r1], k0[:r1]) and torch.equal(v[:r1], v0[:r1]) and not torch.equal(k[r1:], k0[r1:])
     assert lens.tolist() == [300, 50]
     assert torch.equal(w[0].cpu(), torch.from_numpy(c.w[0])) and torch.equal(pos[0].cpu(), torch.from_numpy(c.pos[0]))
+
+
+# ---------------------------------------------------------------------------
+# a step right behind the kernels that write its inputs
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("seqs", [3, 24])
+@pytest.mark.parametrize("hq,hkv,hd", [(16, 8, 128), (8, 1, 256)])
+def test_steps_read_what_the_kernels_before_them_wrote(cuda, seqs, hq, hkv, hd):
+    # append (K, V and the rotated queries), the counters, the decode: once with a wait after every
+    # launch, once replayed from a graph 30 steps in a row; few and many packed rows
+    steps, own = 30, [1 + 7 * i % 90 for i in range(seqs)]
+    g = torch.Generator(device=cuda).manual_seed(34)
+    bank = [torch.randn((steps, seqs, m * hd), device=cuda, generator=g) for m in (hq, hkv, hkv)]
+    angle = torch.rand((300, hd), device=cuda, generator=g) * 6
+    cos, sin = angle.cos(), angle.sin()
+
+    def run(captured):
+        c = Case(cuda, [150] * seqs, plens=[500], cut=[0, seqs], hq=hq, hkv=hkv, hd=hd, seed=35)
+        kv_len, step = c.i32(own), torch.zeros(1, dtype=torch.int64, device=cuda)
+        row0, q = c.i64(c.first), torch.empty((seqs, hq * hd), device=cuda)
+        outs = torch.zeros((steps, seqs, hq * hd), device=cuda)
+        weights = torch.zeros((seqs, hkv, c.stride), device=cuda)
+        ws = torch.full((smol_b200.decode_shared_workspace_bytes(seqs, 150, 1, 500, seqs, hq, hkv, hd),), 255,
+                        dtype=torch.uint8, device=cuda)
+        fixed = (c.i64(c.pfirst), c.i32(c.plens), c.i32(c.cut))
+
+        def one(wait):
+            x = [b.index_select(0, step)[0] for b in bank]
+            slots = row0 + kv_len
+            pos = kv_len.clone()
+            kv_len.add_(1)
+            wait()
+            smol_b200.qknorm_rope_append(*x, seqs, hq, hkv, hd, None, None, 1e-6, cos, sin, False, pos, slots, q, None, c.k,
+                                         c.v, c.rows)
+            wait()
+            smol_b200.decode_attention_shared(c.out, q, c.k, c.v, c.rows, *fixed, 1, 500, seqs, row0, kv_len, seqs, 150, hq,
+                                              hkv, hd, c.scale, ws, weights_in=weights, weights_out=weights,
+                                              weights_stride=c.stride)
+            wait()
+            outs.index_copy_(0, step, c.out[None])
+            step.add_(1)
+
+        if captured:
+            s = torch.cuda.Stream()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.stream(s):
+                one(lambda: None)      # first use outside the capture
+            torch.cuda.synchronize()
+            kv_len.copy_(c.i32(own))
+            step.zero_()
+            weights.zero_()
+            with torch.cuda.graph(graph, stream=s):
+                one(lambda: None)
+            for _ in range(steps):
+                graph.replay()
+        else:
+            for _ in range(steps):
+                one(torch.cuda.synchronize)
+        torch.cuda.synchronize()
+        # the last step against 64 bits (its weights: what the steps before left is not known here)
+        c.q, c.lens = q, kv_len.tolist()
+        assert c.lens == [x + steps for x in own]
+        c.check(None)
+        return outs, weights, kv_len
+
+    want = run(False)
+    for _ in range(3):
+        for a, b in zip(run(True), want):
+            assert torch.equal(a, b)
+    no_error()
