@@ -48,8 +48,10 @@ __device__ __forceinline__ f32x2 exp2_2(f32x2 x)
 }
 
 // 2^x for a pair on the FMA pipe: n = round(x) by adding 1.5 * 2^23, f = x - n in [-1/2, 1/2],
-// 2^f from a degree-5 polynomial fitted for relative error (7.5e-8; 2.1e-7 with its fp32
-// roundings, as ex2.approx), n added to the exponent field.  x outside [-126, 127] counts as
+// 2^f from a degree-5 polynomial, n added to the exponent field.  The polynomial is the minimax
+// one for relative error, fitted here by Lawson's reweighted least squares: 7.5e-8 off,
+// 1.55e-7 with its coefficients rounded to fp32 (the constant is a step above 1), 2.1e-7 with the
+// roundings of its evaluation, on a par with ex2.approx.  x outside [-126, 127] counts as
 // the nearer end; NaN gives the largest finite float, which no sum of probabilities reaches.
 __device__ __forceinline__ float clamp_exp(float x)
 {

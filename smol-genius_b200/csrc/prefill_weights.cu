@@ -622,7 +622,8 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                     const float before = kOne && p.weights_in && key < p.seq_k ? p.weights_in[at] : 0.f;
                     int lo, hi;
                     columns_of(key, rt, lo, hi);
-                    // columns past the tile's rows have lse = +inf: they add nothing
+                    // columns past the tile's rows have -lse = -inf: they add 0, or the polynomial's least value
+                    // 2^-126, which only a sum that is itself next to the smallest normal float shows
                     const bool whole = __all_sync(0xffffffffu, lo == 0 && hi == min(p.qp, p.seq_q - rt * p.qp) * p.group);
                     if (ok) ok = mbar_wait_warp(d_full, ((g0 + t) / kStep) & 1, p.err, kErrWaitMma);
                     float one = 0.f;
