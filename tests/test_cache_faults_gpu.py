@@ -5,6 +5,10 @@ Comparisons are with the 64-bit forms and derived bounds of test_cache_shared_gp
 test_cache_evict_gpu.py, or bit for bit with another run of the same call.
 """
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -194,4 +198,217 @@ def test_steps_read_what_the_kernels_before_them_wrote(cuda, seqs, hq, hkv, hd):
     for _ in range(3):
         for a, b in zip(run(True), want):
             assert torch.equal(a, b)
+    no_error()
+
+
+# ---------------------------------------------------------------------------
+# captured, repeated, on two streams, without programmatic launches
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("w_in_place", [False, True])
+@pytest.mark.parametrize("pos_in_place", [False, True])
+@pytest.mark.parametrize("len_in_place", [False, True])
+@pytest.mark.parametrize("n,budget", [(300, 70), (9000, 3000)])
+def test_evict_each_output_may_be_its_input(cuda, w_in_place, pos_in_place, len_in_place, n, budget):
+    c = Evict(cuda, [n, budget - 1], 2, 8, seed=36)
+    whole = EvictCall(c, budget, 4, 20, in_place=True)
+    whole()
+    k, v, w, pos, lens = whole.results()
+    whole.reset()
+    call = EvictCall(c, budget, 4, 20, in_place=False)
+    args, wo, po, lo = list(call.args), call.outs[2], call.outs[3], call.outs[4]
+    for flag, src, dst in ((w_in_place, 4, 5), (pos_in_place, 6, 7), (len_in_place, 9, 10)):
+        if flag:
+            args[dst] = args[src]
+    smol_b200.cache_evict(*args)
+    wo, po, lo = args[5], args[7], args[10]
+    assert torch.equal(c.k.view(torch.int16), k.view(torch.int16)) and torch.equal(c.v.view(torch.int16), v.view(torch.int16))
+    assert torch.equal(lo, lens)
+    for b, length in enumerate(c.lens):
+        assert torch.equal(wo[b, :, :length], w[b, :, :length]) and torch.equal(po[b, :, :length], pos[b, :, :length])
+        if not w_in_place:
+            assert torch.all(wo[b, :, length:] == 7.0)
+        if not pos_in_place:
+            assert torch.all(po[b, :, length:] == 77)
+    no_error()
+
+
+class PromptCall:
+    """Weights of prompt rows as a call without arguments (weights_in apart from weights_out)."""
+
+    def __init__(self, cuda, batch, rows, keys, hq, hkv, hd, seed=0, **kw):
+        g = torch.Generator(device=cuda).manual_seed(seed)
+        q = torch.randn((batch, rows, hq * hd), device=cuda, generator=g).to(torch.bfloat16)
+        k = torch.randn((batch, keys, hkv * hd), device=cuda, generator=g).to(torch.bfloat16)
+        self.win = torch.rand((batch, hkv, keys), device=cuda, generator=g)
+        self.out = torch.full_like(self.win, -3.0)
+        ws = torch.full((smol_b200.prefill_weights_workspace_bytes(batch, rows, keys, hq, hkv, hd),), 255, dtype=torch.uint8,
+                        device=cuda)
+        self.args = (self.win, self.out, keys, q, k, batch, rows, keys, hq, hkv, hd, hd ** -0.5, ws)
+        self.kw = dict(q_offset=keys - rows, **kw)
+
+    def __call__(self):
+        smol_b200.prefill_attention_weights(*self.args, **self.kw)
+
+
+PROMPTS = [(1, 32, 5000, 16, 8, 128), (2, 600, 600, 4, 2, 128), (1, 900, 1300, 8, 1, 256), (3, 130, 400, 15, 5, 64)]
+
+
+@pytest.mark.parametrize("shape", PROMPTS)
+def test_prompt_weights_repeat_and_are_captured(cuda, shape):
+    call = PromptCall(cuda, *shape)
+    call()
+    torch.cuda.synchronize()
+    want = call.out.clone()
+    assert torch.isfinite(want).all()
+    # every row hands out 1 per head
+    added = (want - call.win).double().sum(dim=(1, 2))
+    assert torch.all((added / (shape[1] * shape[3]) - 1).abs() < 1e-4)
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        call()
+        call()
+    for i in range(20):
+        call.out.fill_(-3.0)
+        graph.replay() if i % 2 else call()
+        assert torch.equal(call.out, want)
+    no_error()
+
+
+@pytest.mark.parametrize("n,budget,units", [(300, 40, 6), (20000, 6000, 3)])
+def test_evict_captured(cuda, n, budget, units):
+    for in_place in (False, True):
+        call = EvictCall(Evict(cuda, [n, n // 2], units, 8, seed=37), budget, 4, 30, in_place=in_place)
+        call()
+        want = call.results()
+        s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            call()
+        for _ in range(10):
+            call.reset()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(call.results(), want))
+    no_error()
+
+
+def test_weights_decode_captured_with_eviction(cuda):
+    """A step that appends, attends with weights and evicts in place, replayed, against the same step by step."""
+    seqs, hq, hkv, hd, budget, steps, rows = 5, 16, 8, 128, 60, 40, 80
+    g = torch.Generator(device=cuda).manual_seed(38)
+    bank = [torch.randn((steps, seqs, m * hd), device=cuda, generator=g) for m in (hq, hkv, hkv)]
+    cos, sin = torch.ones((300, hd), device=cuda), torch.zeros((300, hd), device=cuda)
+
+    def run(captured):
+        c = Case(cuda, [rows] * seqs, hq=hq, hkv=hkv, hd=hd, seed=39)
+        kv_len = c.i32([40 + 5 * b for b in range(seqs)])
+        seen, step = kv_len.clone(), torch.zeros(1, dtype=torch.int64, device=cuda)
+        start = kv_len.clone()
+        row0, q = c.i64(c.first), torch.empty((seqs, hq * hd), device=cuda)
+        weights = torch.zeros((seqs, hkv, rows), device=cuda)
+        positions = torch.full((seqs, hkv, rows), -1, dtype=torch.int32, device=cuda)
+        outs = torch.zeros((steps, seqs, hq * hd), device=cuda)
+        pools = c.k.clone(), c.v.clone()
+        dws = torch.full((smol_b200.decode_weights_workspace_bytes(seqs, rows, hq, hkv, hd),), 255, dtype=torch.uint8, device=cuda)
+        ews = torch.full((smol_b200.cache_evict_workspace_bytes(seqs, rows, hkv),), 255, dtype=torch.uint8, device=cuda)
+
+        def one(wait):
+            x = [b.index_select(0, step)[0] for b in bank]
+            wait()
+            smol_b200.qknorm_rope_append(*x, seqs, hq, hkv, hd, None, None, 1e-6, cos, sin, False, seen, row0 + kv_len, q, None,
+                                         c.k, c.v, c.rows)
+            kv_len.add_(1)
+            seen.add_(1)
+            wait()
+            smol_b200.decode_attention_weights(c.out, q, c.k, c.v, c.rows, row0, kv_len, seqs, rows, hq, hkv, hd, c.scale,
+                                               weights, weights, rows, dws)
+            wait()
+            smol_b200.cache_evict(c.k, c.v, c.rows, row0, weights, weights, positions, positions, rows, kv_len, kv_len, seen,
+                                  seqs, rows, hkv, hd, budget, 4, 16, ews)
+            wait()
+            outs.index_copy_(0, step, c.out[None])
+            step.add_(1)
+
+        if captured:
+            s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+            with torch.cuda.stream(s):
+                one(lambda: None)
+            torch.cuda.synchronize()
+            for x, x0 in ((kv_len, start), (seen, start), (c.k, pools[0]), (c.v, pools[1])):
+                x.copy_(x0)
+            step.zero_(), weights.zero_(), positions.fill_(-1)
+            with torch.cuda.graph(graph, stream=s):
+                one(lambda: None)
+            for _ in range(steps):
+                graph.replay()
+        else:
+            for _ in range(steps):
+                one(torch.cuda.synchronize)
+        torch.cuda.synchronize()
+        assert max(kv_len.tolist()) == budget
+        return outs, weights, positions, kv_len, c.k.view(torch.int16), c.v.view(torch.int16)
+
+    for a, b in zip(run(True), run(False)):
+        assert torch.equal(a, b)
+    no_error()
+
+
+def test_all_operators_on_two_streams(cuda):
+    # each stream its own tensors and workspaces: prompt weights and eviction beside the shared decode
+    shared = Case(cuda, [100 + 13 * i for i in range(40)], plens=[900], cut=[0, 40], seed=40)
+    calls = [shared_call(shared, shared.win, shared.wout), PromptCall(cuda, *PROMPTS[1]), PromptCall(cuda, *PROMPTS[0], seed=1),
+             EvictCall(Evict(cuda, [9000, 5000], 4, 64, seed=41), 2000, 4, 30, in_place=False)]
+
+    def outputs():
+        return [x.clone() for x in [shared.out, shared.wout, calls[1].out, calls[2].out] + calls[3].outs]
+
+    for call in calls:
+        call()
+    torch.cuda.synchronize()
+    want = outputs()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for r in range(30):
+        calls[3].reset()
+        for x in (shared.out, shared.wout, calls[1].out, calls[2].out):
+            x.fill_(-3.0)
+        torch.cuda.synchronize()
+        for i in range(4):
+            with torch.cuda.stream(streams[(i + r) % 2]):
+                calls[(i + r // 2) % 4]()
+        torch.cuda.synchronize()
+        for a, b in zip(outputs(), want):
+            assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+    no_error()
+
+
+@pytest.mark.parametrize("window", [0, 1, 150])
+@pytest.mark.parametrize("prefixes", [31, 33, 70])
+def test_many_prefixes_with_windows(cuda, prefixes, window):
+    cut = [0]
+    for i in range(prefixes):
+        cut.append(cut[-1] + (9 if i % 5 != 3 else 0))
+    c = Case(cuda, [i % 11 for i in range(cut[-1] + 1)], plens=[(i * 29 + 7) % 200 for i in range(prefixes)], cut=cut, hq=4,
+             hkv=2, hd=64, window=window, seed=42)
+    c.check(c.run())
+    no_error()
+
+
+def test_without_programmatic_launches(cuda):
+    """The operators' own tests in a process whose launches are all fully ordered (SMOL_API_PDL=0)."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, SMOL_API_PDL="0")
+    run = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-p", "no:cacheprovider", "-k",
+                          "serving_loop or captured or packed_rows or two_streams or prompt_shapes or evict_small or steps_read",
+                          os.path.join(here, "test_cache_shared_gpu.py"), os.path.join(here, "test_cache_evict_gpu.py"),
+                          os.path.abspath(__file__)], env=env, capture_output=True, text=True, timeout=600)
+    assert run.returncode == 0, run.stdout[-3000:] + run.stderr[-1000:]
+    assert " passed" in run.stdout and "skipped" not in run.stdout
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(50, 1, 128), (200, 1, 64), (130, 2, 256)])
+@pytest.mark.parametrize("seqs", [1, 3])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_large_groups(cuda, hq, hkv, hd, seqs, bf16):
+    # one sequence's heads fill a query tile and more, or a tile starts inside a group
+    c = Case(cuda, [70, 0, 9][:seqs], plens=[300], cut=[0, seqs], hq=hq, hkv=hkv, hd=hd, q_bf16=bf16, out_bf16=bf16, seed=43)
+    c.check(c.run())
     no_error()
