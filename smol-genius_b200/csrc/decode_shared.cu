@@ -88,16 +88,13 @@ __device__ __forceinline__ void split_f16(float p0, float p1, uint32_t &hi, uint
     lo = pack_f16x2(p0 - __low2float(h), p1 - __high2float(h));
 }
 
-// The inputs are read from L2 (__ldcg, TMA): the split kernel may start without a wait of its own
-// (see there), so an L1 line may be older than what an earlier kernel wrote.
-//
 // Sequences [s0, s1) of prefix g and its length, clipped to what the host announced
 // (kErrBadArgs is flagged where that cuts something off).
 __device__ __forceinline__ void prefix_range(const SharedParams &p, int g, int &s0, int &s1, int &len, bool flag)
 {
-    s0 = __ldcg(p.prefix_seq0 + g);
-    s1 = __ldcg(p.prefix_seq0 + g + 1);
-    len = __ldcg(p.prefix_len + g);
+    s0 = p.prefix_seq0[g];
+    s1 = p.prefix_seq0[g + 1];
+    len = p.prefix_len[g];
     bool bad = s0 < 0 || s1 > p.n_seqs || len < 0 || len > p.max_prefix_len;
     s0 = max(s0, 0);
     s1 = min(s1, p.n_seqs);
@@ -117,7 +114,7 @@ __device__ __forceinline__ void own_keys(const SharedParams &p, int kv_len, int 
 }
 __device__ __forceinline__ void own_range(const SharedParams &p, int b, int &ks, int &n)
 {
-    own_keys(p, __ldcg(p.kv_len + b), ks, n);
+    own_keys(p, p.kv_len[b], ks, n);
 }
 
 // ===========================================================================
@@ -753,8 +750,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
     constexpr int KSTEPS = HD / 16;
     // After a prefix kernel, whose CTAs have all passed their own wait and then triggered when
     // this grid starts, every earlier kernel has completed and nothing here depends on the prefix
-    // kernel: the two run side by side.  The inputs come from L2, where completed kernels have left
-    // them, and the outputs are slots that the prefix kernel does not touch.  This grid may not end before it, as the merge waits for this grid alone: the last CTA waits
+    // kernel: the two run side by side.  Its inputs then come from L2 (input(), TMA), where completed
+    // kernels have left them, past L1 lines that may be older; its outputs are slots that the prefix
+    // kernel does not touch.  This grid may not end before it, as the merge waits for this grid alone: the last CTA waits
     // (if every CTA did, finished ones would hold their SMs until the prefix kernel's end).
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -774,6 +772,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
     griddep_trigger();
     const bool last_cta =
         p.prefix_items > 0 && blockIdx.x + 1 == gridDim.x && blockIdx.y + 1 == gridDim.y && blockIdx.z + 1 == gridDim.z;
+    auto input = [&](auto *at) {   // always past L1: 9 sequences to 2500, 12 heads of 64, 17.5 us against 16.4
+        return p.prefix_items > 0 ? __ldcg(at) : *at;
+    };
     const int c = blockIdx.x;
     const bool of_prefix = static_cast<int>(blockIdx.z) < p.prefix_units;
     int b, kvh, h_first, nh, key0, n, plen = 0;   // nh head columns; row_of() says whose
@@ -785,14 +786,14 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
         kvh = blockIdx.y;
         h_first = t * 8;
         nh = kvh < p.n_kv_heads && c * p.prefix_chunk < plen ? min(8, (s1 - b) * p.group - h_first) : 0;
-        seq_row0 = __ldcg(p.prefix_row0 + u);
+        seq_row0 = p.prefix_row0[u];
     } else {
         b = blockIdx.z - p.prefix_units;
         kvh = blockIdx.y / p.n_qgroups;
         const int qg = blockIdx.y % p.n_qgroups;
         h_first = kvh * p.group + qg * 8;
         nh = min(8, p.group - qg * 8);
-        seq_row0 = __ldcg(p.seq_row0 + b);
+        seq_row0 = input(p.seq_row0 + b);
     }
     // (sequence, query head) of column i; the columns of a prefix run over its sequences' heads
     auto row_of = [&](int i) -> long long {
@@ -817,7 +818,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
             p.part_ml[row_of(threadIdx.x) * p.slots + c] = make_float2(-INFINITY, 0.f);
     } else {
         int ks;
-        own_range(p, b, ks, n);
+        own_keys(p, input(p.kv_len + b), ks, n);
         key0 = ks + c * p.chunk;
         n = min(n, key0 + p.chunk);
     }
@@ -862,7 +863,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
             float *dst = qs + (e / HD) * S::kQRowFloats + e % HD;
             const long long off = row_of(e / HD) * HD + e % HD;
             if (p.q_is_bf16) {
-                const uint4 w = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + off));
+                const uint4 w = input(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + off));
                 const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -871,8 +872,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
                 }
             } else {
                 const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + off);
-                reinterpret_cast<float4 *>(dst)[0] = __ldcg(src);
-                reinterpret_cast<float4 *>(dst)[1] = __ldcg(src + 1);
+                reinterpret_cast<float4 *>(dst)[0] = input(src);
+                reinterpret_cast<float4 *>(dst)[1] = input(src + 1);
             }
         }
         named_bar_sync(1, kConsumerWarps * 32);
