@@ -539,8 +539,11 @@ SMOL_B200_API int smol_b200_layer_norm(void *stream, void *out, int out_bf16, co
  * device error word.  The two lengths go up to 2^29.
  * q: [n_seqs, n_heads*head_dim] fp32 or bf16 (q_is_bf16); out: the same shape, fp32 or
  * bf16 (out_is_bf16); both and the pools 16-byte aligned.  fp32 queries enter with 24 bits,
- * and an fp32 output is computed to fp32 accuracy from the cached values; a bf16 output is
- * rounded once.  head_dim: 64, 128 or 256; scale > 0.  A row that a window hides from one
+ * and an fp32 output is computed to fp32 accuracy from the cached values: a probability is
+ * 2^-23 of itself off when it multiplies V, or 2^-32 of the row's largest where that is more.
+ * A bf16 output is that result, rounded once.  A NaN among the scores that a query head sees
+ * makes its outputs NaN, and the weights of the own rows it sees.  head_dim: 64, 128 or 256;
+ * scale > 0.  A row that a window hides from one
  * sequence is still multiplied by 0 if another sequence of the same prefix sees it, so
  * prefix rows must hold finite values (rows past every length may hold anything).
  * weights_out (or NULL): the attention probabilities of the own rows, summed over the
@@ -577,6 +580,9 @@ SMOL_B200_API int smol_b200_decode_attention_weights(
  * >= seq_k.  q, k, strides, scale, mask_kind (causal, prefix-LM or full), q_offset,
  * prefix_len, window and softcap as in smol_b200_prefill_attention, so k may be the cache
  * itself; to count the last rows of a prompt only, pass those rows with their q_offset.
+ * Probabilities are taken over the keys of this k alone: rows of a prompt whose sequence also
+ * has a shared prefix hand out 1 per head over their own keys, while a decode step over the
+ * prefix hands its own rows what the prefix leaves.
  * Rows that see no key add nothing; with seq_q == 0 weights_out is weights_in.  head_dim:
  * any multiple of 8 up to 256; at most 128 query heads to a KV head; scale > 0; lengths
  * and |q_offset| up to 2^29. */

@@ -19,7 +19,8 @@
 //
 // Bytes: 8 per slot to read (weight, position), as many to write where the outputs are
 // other arrays, and K and V of the moved rows.  32 sequences of 1025 slots to 1024, 8 heads of
-// 128: 7.6 us, latency; 8 of 16384 to 2048: 49.6 us, 13 of them selection (134 MB: 20 us).
+// 128: 7.6 us, latency (8.3 in place, with the launch that writes the lengths); 8 of 16384 to
+// 2048: 52.5 us, 13 of them selection (134 MB: 20 us).
 #include <string.h>
 
 #include "b200_common.cuh"

@@ -15,7 +15,7 @@
 //           sum_h e^(x_hj - M_h) / L_h to the weight of own key j.
 // Bound: HBM for large batches (decode weights, 64 sequences of 1024 to 8192 keys, 8 KV heads of
 // 128: 202 us for 1.23 GB, 0.93 of the copy rate), latency for small ones (one sequence of 513
-// keys: 6.4 us, two launches).
+// keys: 6.6 us, two launches).
 //
 // Precision.  Scores, maxima, sums and outputs of the parts are fp32.  K is bf16 and V
 // fp16 in the cache.  fp32 queries enter the bf16 products as three bf16 terms (24 bits:

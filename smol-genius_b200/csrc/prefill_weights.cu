@@ -11,7 +11,7 @@
 //          rows stay in shared memory, key tiles stream and each is complete by itself.
 // The probabilities themselves are never stored.  Bound: two exponentials per visible
 // (row, key) pair at 16 per clock and SM, 60 us for 4096 causal rows of 16/8 heads of 128,
-// which take 106; a pass's products alone take 800 clocks a 128 x 128 tile, its exponentials
+// which take 109; a pass's products alone take 800 clocks a 128 x 128 tile, its exponentials
 // 1000, one waits for the other for 1100 to 1360.  (256-column products, two buffers of S in
 // turn: 120 us.)
 //
