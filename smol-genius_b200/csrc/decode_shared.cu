@@ -95,9 +95,9 @@ __device__ __forceinline__ void prefix_range(const SharedParams &p, int g, int &
     s0 = p.prefix_seq0[g];
     s1 = p.prefix_seq0[g + 1];
     len = p.prefix_len[g];
-    bool bad = s0 < 0 || s1 > p.n_seqs || len < 0 || len > p.max_prefix_len;
-    s0 = max(s0, 0);
-    s1 = min(s1, p.n_seqs);
+    bool bad = s0 < 0 || s1 > p.n_seqs || s0 > s1 || len < 0 || len > p.max_prefix_len;
+    s0 = min(max(s0, 0), p.n_seqs);   // any values: 0 <= s0 <= s1 <= n_seqs
+    s1 = max(min(s1, p.n_seqs), s0);
     len = min(max(len, 0), p.max_prefix_len);
     if (s1 - s0 > p.max_prefix_seqs) {
         s1 = s0 + p.max_prefix_seqs;

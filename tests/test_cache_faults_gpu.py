@@ -412,3 +412,37 @@ def test_large_groups(cuda, hq, hkv, hd, seqs, bf16):
     c = Case(cuda, [70, 0, 9][:seqs], plens=[300], cut=[0, seqs], hq=hq, hkv=hkv, hd=hd, q_bf16=bf16, out_bf16=bf16, seed=43)
     c.check(c.run())
     no_error()
+
+
+# ---------------------------------------------------------------------------
+# device values that are no ranges
+# ---------------------------------------------------------------------------
+LOW, HIGH = -(1 << 31), (1 << 31) - 1
+
+
+@pytest.mark.parametrize("seqs", [3, 24])
+@pytest.mark.parametrize("ranges", [(HIGH, LOW), (HIGH, HIGH), (LOW, LOW), (1, 0), (5000, LOW), (HIGH - 1, LOW + 1), (-1, -1)])
+@pytest.mark.parametrize("prefixes", [1, 40])
+def test_ranges_that_are_none_count_as_empty(cuda, seqs, ranges, prefixes):
+    # one prefix (a table in registers) and 40 (found item by item), few packed rows and many
+    c = Case(cuda, [3 + i % 4 for i in range(seqs)], plens=[200] + [0] * (prefixes - 1), cut=[0, seqs] + [seqs] * (prefixes - 1),
+             seed=44)
+    n, maxl = seqs, max(c.lens)
+    ws = torch.full((smol_b200.decode_shared_workspace_bytes(n, maxl, prefixes, 200, n, 16, 8, 128),), 255, dtype=torch.uint8,
+                    device=cuda)
+
+    def run(cut):
+        smol_b200.decode_attention_shared(c.out, c.q, c.k, c.v, c.rows, c.i64(c.pfirst), c.i32(c.plens), c.i32(cut), prefixes,
+                                          200, n, c.i64(c.first), c.i32(c.lens), n, maxl, 16, 8, 128, c.scale, ws,
+                                          weights_in=c.win, weights_out=c.wout, weights_stride=c.stride)
+        torch.cuda.synchronize()
+        flagged = smol_b200.device_error() & (1 << 5)
+        smol_b200.clear_error()
+        return flagged
+
+    assert not run(c.cut)
+    c.check(c.wout)
+    # the first prefix has the bad range, the others (of no rows) whatever follows from its end
+    assert run(list(ranges) + [ranges[1]] * (prefixes - 1))
+    c.cut, c.plens = [0] * (prefixes + 1), [0] * prefixes
+    c.check(c.wout)
