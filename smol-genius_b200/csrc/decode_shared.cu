@@ -56,6 +56,7 @@ struct SharedParams {
     int n_seqs, n_heads, n_kv_heads, group, n_qgroups;
     unsigned group_inv;             // ceil(2^31 / group): (u * group_inv) >> 31 is u / group while u * group < 2^31
     int n_prefixes, max_prefix_len, max_prefix_seqs;
+    int idle_prefixes;              // prefixes announced without rows or sequences: only looked over
     int prefix_chunk, prefix_slots; // keys of one prefix part; parts of the longest prefix
     int prefix_qtiles;              // query tiles of the largest group (few rows: of 8 rows)
     int prefix_items;               // query tiles x parts x KV heads x prefixes; 0: few rows
@@ -1122,6 +1123,12 @@ __global__ void __launch_bounds__(kMergeThreads, 4) merge_kernel(const __grid_co
     griddep_wait();
     griddep_trigger();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (blockIdx.x == 0) {
+        for (int g = threadIdx.x; g < p.idle_prefixes; g += kMergeThreads) {
+            int s0, s1, len;
+            prefix_range(p, g, s0, s1, len, true);
+        }
+    }
     if (static_cast<int>(blockIdx.x) < out_blocks) {
         // unit u: 128 outputs from element 128 u of the output on (head dim 64: of two heads)
         __shared__ float4 red[kMergeThreads];
@@ -1490,6 +1497,7 @@ int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const v
     if (!(scale > 0.f)) return SMOL_B200_ERR_ARGS;
     if (weights_in && !weights_out) return SMOL_B200_ERR_ARGS;
     if (weights_out && weights_stride < max_kv_len) return SMOL_B200_ERR_ARGS;
+    const int announced = n_prefixes;
     if (max_prefix_len == 0 || max_prefix_seqs == 0) n_prefixes = 0;
 
     SharedParams p;
@@ -1553,6 +1561,7 @@ int decode_attention_shared(cudaStream_t st, void *out, int out_is_bf16, const v
     p.err = device_error_word();
     if (!p.err) return SMOL_B200_ERR_CUDA;
     p.n_prefixes = n_prefixes;
+    p.idle_prefixes = announced - n_prefixes;
     p.max_prefix_len = max_prefix_len;
     p.max_prefix_seqs = max_prefix_seqs;
     p.window = window;

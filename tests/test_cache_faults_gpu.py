@@ -14,7 +14,7 @@ import torch
 
 import smol_b200
 from test_cache_evict_gpu import Evict
-from test_cache_shared_gpu import Case, no_error
+from test_cache_shared_gpu import EPS, Case, no_error
 
 pytestmark = pytest.mark.gpu
 
@@ -446,3 +446,57 @@ def test_ranges_that_are_none_count_as_empty(cuda, seqs, ranges, prefixes):
     assert run(list(ranges) + [ranges[1]] * (prefixes - 1))
     c.cut, c.plens = [0] * (prefixes + 1), [0] * prefixes
     c.check(c.wout)
+
+
+@pytest.mark.parametrize("max_len,max_seqs", [(0, 2), (100, 0), (0, 0)])
+@pytest.mark.parametrize("plen,end", [(0, 0), (5, 2), (0, 2), (5, 0)])
+def test_prefixes_announced_as_none(cuda, max_len, max_seqs, plen, end):
+    # bounds of 0 are bounds: a prefix beyond them is left out and flagged
+    c = Case(cuda, [70, 9], plens=[5], cut=[0, 2], seed=45)
+    ws = torch.empty(smol_b200.decode_shared_workspace_bytes(2, 70, 1, max_len, max_seqs, 16, 8, 128), dtype=torch.uint8,
+                     device=cuda)
+    smol_b200.decode_attention_shared(c.out, c.q, c.k, c.v, c.rows, c.i64(c.pfirst), c.i32([plen]), c.i32([0, end]), 1, max_len,
+                                      max_seqs, c.i64(c.first), c.i32(c.lens), 2, 70, 16, 8, 128, c.scale, ws,
+                                      weights_in=c.win, weights_out=c.wout, weights_stride=c.stride)
+    torch.cuda.synchronize()
+    assert bool(smol_b200.device_error() & (1 << 5)) == (plen > max_len or end > max_seqs)
+    smol_b200.clear_error()
+    c.plens, c.cut = [0], [0, 0]
+    c.check(c.wout)
+
+
+def test_most_sequences(cuda):
+    # as many sequences as are accepted, one of a pool's few rows each, all on one prefix
+    n, hd, plen, rows = 65535, 64, 3, 40
+    g = torch.Generator(device=cuda).manual_seed(46)
+    k = torch.randn((rows, hd), device=cuda, generator=g).to(torch.bfloat16)
+    v = torch.randn((rows, hd), device=cuda, generator=g).to(torch.float16)
+    q = torch.randn((n, hd), device=cuda, generator=g)
+    row0 = torch.arange(n, device=cuda) % (rows - plen) + plen
+    lens = (torch.arange(n, device=cuda) % 3 > 0).to(torch.int32)
+    out, w = torch.full((n, hd), 7.0, device=cuda), torch.full((n, 1, 1), -3.0, device=cuda)
+    ws = torch.empty(smol_b200.decode_shared_workspace_bytes(n, 1, 1, plen, n, 1, 1, hd), dtype=torch.uint8, device=cuda)
+    i32 = dict(dtype=torch.int32, device=cuda)
+    smol_b200.decode_attention_shared(out, q, k, v, rows, torch.zeros(1, dtype=torch.int64, device=cuda),
+                                      torch.tensor([plen], **i32), torch.tensor([0, n], **i32), 1, plen, n, row0, lens, n, 1, 1, 1,
+                                      hd, 0.125, ws, weights_out=w, weights_stride=1)
+    torch.cuda.synchronize()
+    x = torch.cat([q.double() @ k[:plen].double().T, (q.double() * k[row0].double()).sum(1, keepdim=True)], 1) * 0.125
+    x[lens == 0, plen] = -float("inf")
+    p = torch.softmax(x, dim=1)
+    want = p[:, :plen] @ v[:plen].double() + p[:, plen:] * v[row0].double()
+    a = p[:, :plen] @ v[:plen].double().abs() + p[:, plen:] * v[row0].double().abs()
+    # the bound of test_cache_shared_gpu.py
+    mag = 0.125 * float((q.double().abs() @ k.double().abs().T).max())
+    d = EPS * ((hd / 16 * 3 + 4) * mag + 3 * float(x[:, :plen].abs().max()) + 2)
+    assert ((out.double() - want).abs() <= (2 * d + 2.0 ** -21 + 65 * EPS) * a).all()
+    seen = lens > 0
+    assert ((w[seen, 0, 0].double() - p[seen, plen]).abs() <= (2 * d + 65 * EPS) * p[seen, plen]).all()
+    assert torch.all(w[~seen] == -3.0)
+    no_error()
+
+
+@pytest.mark.parametrize("n,budget", [(262144, 100000), (262143, 262142)])
+def test_evict_longest(cuda, n, budget):
+    Evict(cuda, [n, 1000], 1, 8, seed=47).run(budget, 4, 100, True)
+    no_error()
